@@ -2178,3 +2178,207 @@ def matrix_memory(q, k, v, gate, i_rows, f_rows, i_bias, f_bias, cap, states, we
                                   c_float(q_scale), n_seq, *sizes, _stream()), "matrix_memory")
     _check(lib, lib.dk_mm_output(_dt(q), _p(o), _p(scal), _p(weight), c_float(eps), _p(gate), ld, c_float(out_scale), _p(out),
                                  c_longlong(out.stride(0)), _p(row_pos), T, n_heads, v_head_dim, _stream()), "matrix_memory output")
+
+
+# ------------------------------------------------------- branches: trees of drafted tokens, beams
+TREE_MAX_NODES = 1024       # nodes of one sequence's tree
+TREE_MAX_GROUP = 64         # query heads a kv head
+MAX_BEAMS, MAX_BEST = 32, 64
+
+
+def _same_device(what, *tensors):
+    """All on the device whose stream the launch goes to."""
+    for t in tensors:
+        if t is not None and t.is_cuda and t.device.index != torch.cuda.current_device():
+            raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _need_shape(t, name, shape):
+    if t is not None and tuple(t.shape) != tuple(shape):
+        raise KernelError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _need_tree(what, rows, n_seq, max_nodes, cu_q, row_pos):
+    if not 1 <= max_nodes <= TREE_MAX_NODES:
+        raise KernelError(f"{what}: max_nodes {max_nodes}, trees have 1 to {TREE_MAX_NODES} nodes")
+    _need(cu_q, "cu_q", torch.int32, 1), _need(row_pos, "row_pos", torch.int32, 1)
+    _need_shape(cu_q, "cu_q", (n_seq + 1,)), _need_shape(row_pos, "row_pos", (rows,))
+    if not 1 <= n_seq <= 65535:
+        raise KernelError(f"{what}: {n_seq} sequences, 1 to 65535 go in one call")
+
+
+@functools.lru_cache(maxsize=None)
+def _tree_blocks(head_dim, f32, max_nodes, group):
+    return _lib("attention_tree.cu", {"HD": head_dim}).dk_attn_tree_blocks(f32, max_nodes, group)
+
+
+def attention_tree(q, out, k_store, v_store, cu_q, seq_pos0, row_pos, tree, page_table, n_heads, n_kv_heads, head_dim, window, scale,
+                   max_nodes):
+    """Attention of trees of drafted tokens over the paged cache. Sequence s has ``seq_pos0[s]`` cached tokens and brings the nodes of
+    its tree as rows cu_q[s] .. cu_q[s + 1] (at most ``max_nodes``); node i's key and value lie in the cache at place seq_pos0[s] + i,
+    its position is row_pos (seq_pos0[s] + its depth; < 0: a padding row, which sees nothing). It sees the cached tokens and the nodes j
+    whose bit (word j / 32, bit j % 32) is set in its row of ``tree`` [rows, words] int32: of a drafted tree its ancestors and itself,
+    but any bits may be set. With a ``window`` it sees only what lies less than that many positions before it. Rows that see nothing
+    become zeros, rows behind cu_q's last are left as they were, and what lies at keys a row does not see, NaN included, does not reach
+    it. A page id outside the store holds no keys. q and out [rows, heads * head_dim] (rows of wider matrices, 16-byte boundaries),
+    float32 or bfloat16, head sizes in steps of 16 up to 256. The lengths are read on the device: a captured graph may be replayed
+    with other ones, as long as ``max_nodes`` and the table's width hold."""
+    _need_rows(q, "q"), _need_rows(out, "out", q.dtype)
+    rows, n_seq = q.shape[0], seq_pos0.shape[0]
+    _need_tree("attention_tree", rows, n_seq, max_nodes, cu_q, row_pos)
+    _need(seq_pos0, "seq_pos0", torch.int32, 1), _need(tree, "tree", torch.int32, 2), _need(page_table, "page_table", torch.int32, 2)
+    _need(k_store, "k_store", q.dtype, 4), _need(v_store, "v_store", q.dtype, 4)
+    if head_dim % 16 or not 16 <= head_dim <= 256 or n_kv_heads < 1 or n_heads % n_kv_heads or not 1 <= n_heads // n_kv_heads <= TREE_MAX_GROUP:
+        raise KernelError(f"attention_tree: head size {head_dim} (multiples of 16 up to 256) / heads {n_heads}:{n_kv_heads} (up to "
+                          f"{TREE_MAX_GROUP} a kv head) not supported")
+    _need_shape(q, "q", (rows, n_heads * head_dim)), _need_shape(out, "out", (rows, n_heads * head_dim))
+    _need_shape(k_store, "k_store", (k_store.shape[0], n_kv_heads, PAGE, head_dim)), _need_shape(v_store, "v_store", k_store.shape)
+    _need_shape(tree, "tree", (rows, tree.shape[1])), _need_shape(page_table, "page_table", (n_seq, page_table.shape[1]))
+    if k_store.shape[0] < 1 or page_table.shape[1] < 1 or tree.shape[1] < 1:
+        raise KernelError("attention_tree: an empty store, page table or row of tree bits")
+    if not scale > 0 or int(window or 0) < 0:
+        raise KernelError(f"attention_tree: scale {scale} must be positive, window {window} not negative")
+    size = q.element_size()
+    if any(t.data_ptr() % 16 or t.stride(0) * size % 16 for t in (q, out)):
+        raise KernelError("attention_tree: rows of q and out must lie on 16-byte boundaries")
+    _same_device("attention_tree", q, out, k_store, v_store, cu_q, seq_pos0, row_pos, tree, page_table)
+    if rows == 0:
+        return
+    group, f32 = n_heads // n_kv_heads, int(q.dtype == torch.float32)
+    _dt(q)
+    lib = _lib("attention_tree.cu", {"HD": head_dim})
+    blocks = _tree_blocks(head_dim, f32, max_nodes, group)
+    n = 2 * blocks * lib.dk_tree_tile_rows(max_nodes, group)
+    ws = torch.empty(n * (head_dim + 2), dtype=torch.float32, device=q.device)
+    _check(lib, lib.dk_attn_tree(f32, _p(q), c_longlong(q.stride(0)), _p(out), c_longlong(out.stride(0)), _p(k_store), _p(v_store),
+                                 k_store.shape[0], _p(cu_q), _p(seq_pos0), _p(row_pos), _p(tree), tree.shape[1], _p(page_table),
+                                 page_table.shape[1], n_seq, n_heads, n_kv_heads, int(window or 0), c_float(scale), max_nodes,
+                                 _p(ws), _p(ws[n * head_dim:]), blocks, _stream()), "attention_tree", 2)
+
+
+def tree_accept(logits, tok, parent, cu_q, row_pos, temperature, seeds, path, n_path, next_tok):
+    """Which path of its tree each sequence accepts. ``logits`` [rows, vocab] float32 of the nodes, ``tok`` [rows] their tokens,
+    ``parent`` [rows] the node each was drafted behind (within its tree, below its own number; node 0 is the sequence's last token, its
+    parent is not looked at), ``temperature`` [n_seq] and ``seeds`` [n_seq, 2] as for ``sample``. The token after a node is the one
+    ``sample`` chooses from its logits at row_pos; from node 0 on the path goes to the child that holds it (the lowest such child)
+    until there is none. ``path`` [n_seq, max_nodes] becomes the nodes on the way, node 0 first, -1 behind them, ``n_path`` [n_seq]
+    their number, ``next_tok`` [n_seq] the token chosen at the last of them. A sequence without nodes gets 0 nodes and token 0."""
+    _need(logits, "logits", torch.float32, 2), _need(tok, "tok", torch.int32, 1), _need(parent, "parent", torch.int32, 1)
+    _need(temperature, "temperature", torch.float32, 1), _need(seeds, "seeds", torch.int32, 2), _need(path, "path", torch.int32, 2)
+    _need(n_path, "n_path", torch.int32, 1), _need(next_tok, "next_tok", torch.int32, 1)
+    (rows, V), (n_seq, max_nodes) = logits.shape, path.shape
+    _need_tree("tree_accept", rows, n_seq, max_nodes, cu_q, row_pos)
+    for t, name, shape in ((tok, "tok", (rows,)), (parent, "parent", (rows,)), (temperature, "temperature", (n_seq,)),
+                           (seeds, "seeds", (n_seq, 2)), (n_path, "n_path", (n_seq,)), (next_tok, "next_tok", (n_seq,))):
+        _need_shape(t, name, shape)
+    if V < 1:
+        raise KernelError("tree_accept: logits without columns")
+    _same_device("tree_accept", logits, tok, parent, cu_q, row_pos, temperature, seeds, path, n_path, next_tok)
+    lib = _lib("tree_accept.cu")
+    n = max(1, rows * lib.dk_tree_accept_pieces(V))
+    ws_val = torch.empty(n, dtype=torch.float32, device=logits.device)
+    ws_idx = torch.empty(n, dtype=torch.int32, device=logits.device)
+    _check(lib, lib.dk_tree_accept(_p(logits), V, _p(tok), _p(parent), _p(cu_q), _p(row_pos), _p(temperature), _p(seeds), n_seq, max_nodes,
+                                   _p(ws_val), _p(ws_idx), _p(path), _p(n_path), _p(next_tok), _stream()), "tree_accept", 2)
+
+
+def beam_select(logits, scores, ended, scores_out, beam_out, tok_out):
+    """The best continuations of each request's beams: of all values scores[r, b] + log softmax(logits[r * beams + b])[v] the
+    ``scores_out.shape[1]`` largest, ties by the lower beam, then the lower token, into ``scores_out`` (float32), ``beam_out`` and
+    ``tok_out`` (int32), all [requests, best]. ``ended`` [requests, beams] int32 or None: a beam with a number other than 0 is at its
+    end and stands for itself alone, its own score with token 0. A logit that is not finite is no candidate and weighs nothing, a beam
+    whose score is not finite brings no candidates; where there are fewer than asked for the rest is (-infinity, 0, 0). Up to 32 beams
+    and 64 results, which may not lie in ``scores``."""
+    _need(logits, "logits", torch.float32, 2), _need(scores, "scores", torch.float32, 2), _need(ended, "ended", torch.int32, 2)
+    _need(scores_out, "scores_out", torch.float32, 2), _need(beam_out, "beam_out", torch.int32, 2), _need(tok_out, "tok_out", torch.int32, 2)
+    (requests, beams), best, V = scores.shape, scores_out.shape[1], logits.shape[1]
+    if requests < 1 or not 1 <= beams <= MAX_BEAMS or not 1 <= best <= MAX_BEST or V < 1:
+        raise KernelError(f"beam_select: {requests} requests, {beams} beams (1 to {MAX_BEAMS}), {best} results (1 to {MAX_BEST}), {V} tokens")
+    if requests * beams > 65535 or beams * V >= 1 << 31:
+        raise KernelError(f"beam_select: {requests} requests of {beams} beams over {V} tokens are too many for one call")
+    _need_shape(logits, "logits", (requests * beams, V)), _need_shape(ended, "ended", (requests, beams))
+    for t, name in ((scores_out, "scores_out"), (beam_out, "beam_out"), (tok_out, "tok_out")):
+        _need_shape(t, name, (requests, best))
+    _same_device("beam_select", logits, scores, ended, scores_out, beam_out, tok_out)
+    lib = _lib("beam_select.cu")
+    pieces = lib.dk_beam_pieces(V)
+    if not lib.dk_beam_select_takes(V, beams, best):
+        raise KernelError(f"beam_select: {best} of {beams} beams over {V} tokens need more shared memory than a block has")
+    ws_key = torch.empty(requests * beams * pieces * best, dtype=torch.int64, device=logits.device)
+    ws_sum = torch.empty(requests * beams * pieces * 2, dtype=torch.float64, device=logits.device)
+    _check(lib, lib.dk_beam_select(_p(logits), V, requests, beams, best, _p(scores), _p(ended), _p(ws_key), _p(ws_sum), _p(scores_out),
+                                   _p(beam_out), _p(tok_out), _stream()), "beam_select", 2)
+
+
+def _need_store(store, page_table, what):
+    """(outer, pages, kv heads, bytes of a row) of a store [.., pages, n_kv, PAGE, size]."""
+    if not store.is_cuda or not store.is_contiguous() or store.dim() < 4 or store.shape[-2] != PAGE or store.numel() == 0:
+        raise KernelError(f"{what}: store must be a contiguous CUDA tensor [.., pages, kv heads, {PAGE}, size], got {tuple(store.shape)}")
+    row = store.shape[-1] * store.element_size()
+    if row % 2 or store.data_ptr() % 2:
+        raise KernelError(f"{what}: rows of {row} bytes, which must be even")
+    _need(page_table, "page_table", torch.int32, 2)
+    pages, nkv = store.shape[-4], store.shape[-3]
+    return store.numel() // (pages * nkv * PAGE * store.shape[-1]), pages, nkv, row
+
+
+def kv_keep(store, page_table, seq_pos0, path, n_path):
+    """The accepted nodes' rows close up behind each sequence's cached tokens, in place: row seq_pos0[s] + path[s, k] goes to
+    seq_pos0[s] + k for k < n_path[s]. ``store`` [.., pages, n_kv, PAGE, size] of any type, keys and values of all layers at once;
+    ``path`` [n_seq, up to 1024] rising, as ``tree_accept`` leaves it (a row whose path[s, k] <= k stays where it is). All other rows
+    keep what they hold. Places outside the table and pages outside the store are left out."""
+    outer, pages, nkv, row = _need_store(store, page_table, "kv_keep")
+    _need(seq_pos0, "seq_pos0", torch.int32, 1), _need(path, "path", torch.int32, 2), _need(n_path, "n_path", torch.int32, 1)
+    n_seq, width = path.shape
+    if not 1 <= width <= TREE_MAX_NODES or not 1 <= n_seq <= 65535 or page_table.shape[1] < 1:
+        raise KernelError(f"kv_keep: paths of {width} nodes (1 to {TREE_MAX_NODES}) of {n_seq} sequences")
+    for t, name, shape in ((seq_pos0, "seq_pos0", (n_seq,)), (n_path, "n_path", (n_seq,)), (page_table, "page_table", (n_seq, page_table.shape[1]))):
+        _need_shape(t, name, shape)
+    _same_device("kv_keep", store, page_table, seq_pos0, path, n_path)
+    lib = _lib("cache_moves.cu")
+    _check(lib, lib.dk_kv_keep(_p(store), outer, pages, nkv, c_longlong(row), _p(page_table), page_table.shape[1], n_seq, _p(seq_pos0),
+                               _p(path), width, _p(n_path), _stream()), "kv_keep")
+
+
+def _need_parents(parent, what):
+    _need(parent, "parent", torch.int32, 2)
+    requests, beams = parent.shape
+    if not 1 <= requests <= 65535 or not 1 <= beams <= MAX_BEAMS:
+        raise KernelError(f"{what}: {requests} requests of {beams} beams (1 to {MAX_BEAMS})")
+    return requests, beams
+
+
+def kv_reorder(store, page_table, parent, first, last):
+    """Every beam takes its parent's cache rows, in place: beam b of request r, sequence r * beams + b of ``page_table``, gets the rows
+    [first[r], last[r]) of sequence r * beams + parent[r, b] as they were before the call. ``store`` [.., pages, n_kv, PAGE, size] of
+    any type. The sequences' pages are their own; rows outside [first, last), beams that are their own parents (or whose parent is
+    none of the request's), places outside the table and pages outside the store are left as they were."""
+    outer, pages, nkv, row = _need_store(store, page_table, "kv_reorder")
+    requests, beams = _need_parents(parent, "kv_reorder")
+    _need(first, "first", torch.int32, 1), _need(last, "last", torch.int32, 1)
+    if outer > 65535 or page_table.shape[1] < 1:
+        raise KernelError(f"kv_reorder: {outer} stores in one call, or a table without columns")
+    for t, name, shape in ((first, "first", (requests,)), (last, "last", (requests,)),
+                           (page_table, "page_table", (requests * beams, page_table.shape[1]))):
+        _need_shape(t, name, shape)
+    _same_device("kv_reorder", store, page_table, parent, first, last)
+    lib = _lib("cache_moves.cu")
+    _check(lib, lib.dk_kv_reorder(_p(store), outer, pages, nkv, c_longlong(row), _p(page_table), page_table.shape[1], requests, beams,
+                                  _p(parent), _p(first), _p(last), _stream()), "kv_reorder")
+
+
+def state_reorder(store, seq_slot, parent):
+    """Every beam takes its parent's state, in place: in each entry of ``store`` [entries, slots, ..] of any type, slot
+    seq_slot[r * beams + b] gets what slot seq_slot[r * beams + parent[r, b]] held before the call. The slots are distinct; beams that
+    are their own parents (or whose parent is none of the request's) and slots outside the store are left as they were."""
+    requests, beams = _need_parents(parent, "state_reorder")
+    _need(seq_slot, "seq_slot", torch.int32, 1), _need_shape(seq_slot, "seq_slot", (requests * beams,))
+    if not store.is_cuda or not store.is_contiguous() or store.dim() < 2 or store.numel() == 0 or store.shape[0] > 65535:
+        raise KernelError(f"state_reorder: store must be a contiguous CUDA tensor [entries, slots, ..], got {tuple(store.shape)}")
+    size = store.numel() // (store.shape[0] * store.shape[1]) * store.element_size()
+    if size % 2 or store.data_ptr() % 2:
+        raise KernelError(f"state_reorder: states of {size} bytes, which must be even")
+    _same_device("state_reorder", store, seq_slot, parent)
+    lib = _lib("cache_moves.cu")
+    _check(lib, lib.dk_state_reorder(_p(store), store.shape[0], store.shape[1], c_longlong(size), _p(seq_slot), requests, beams, _p(parent),
+                                     _stream()), "state_reorder")

@@ -1,0 +1,141 @@
+// Which path of a tree of drafted tokens the model itself would have taken.
+//
+// Node i of a sequence's tree holds a drafted token tok[i], drafted to follow node parent[i] (< i; node 0 is the last token of the
+// sequence, whose own place is settled). The model's token after node i is what the sampler (sampling.cu) draws from logits[i] at the
+// position after the node's, with the sequence's temperature and seed: greedy, or argmax(logit / T + noise) with noise that hangs on
+// seed, position and token alone. So the tokens that come out are those that one token a step would have drawn, and drafting changes
+// how many steps they take, not which they are. From node 0 on the path goes to the child that holds the chosen token (the lowest
+// one, if several do) until there is none; the token chosen there is the sequence's next.
+//
+// Two launches: the best token of each piece of 4,096 logits, over all nodes and pieces side by side (one pass over the logits: bound
+// by reading them); then a block a sequence puts the pieces together and walks the path.
+#include "sampling_kernels.cuh"
+
+namespace {
+
+constexpr int THREADS = 256, EACH = 16, CHUNK = THREADS * EACH, MAX_NODES = 1024;
+
+// grid (pieces, max_nodes, sequences)
+template <bool WIDE>
+__global__ void __launch_bounds__(THREADS)
+accept_pieces_kernel(const float* logits, int V, const int* cu_q, const int* row_pos, const float* temperature, const uint32_t* seeds,
+                     float* ws_val, int* ws_idx) {
+    __shared__ float sv[THREADS / 32];
+    __shared__ int si[THREADS / 32];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int s = blockIdx.z, row = cu_q[s] + blockIdx.y;
+    if (row >= cu_q[s + 1]) return;
+    const float* z = logits + (size_t)row * V;
+    const int begin = blockIdx.x * CHUNK, end = min(V, begin + CHUNK);
+    auto index = [&](int k) { return WIDE ? begin + ((k / 4) * THREADS + (int)threadIdx.x) * 4 + k % 4 : begin + k * THREADS + (int)threadIdx.x; };
+    float v[EACH];
+    if (WIDE) {
+#pragma unroll
+        for (int k = 0; k < EACH; k += 4)
+            *reinterpret_cast<float4*>(v + k) = index(k) < end ? *reinterpret_cast<const float4*>(z + index(k))
+                                                              : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    } else {
+#pragma unroll
+        for (int k = 0; k < EACH; k++) v[k] = index(k) < end ? z[index(k)] : -INFINITY;
+    }
+    const int pos = row_pos[row];
+    const float temp = temperature[s];
+    float bv = -INFINITY;
+    int bi = 0x7fffffff;
+    if (pos >= 0) {
+        const float inv_t = temp > 0.f ? 1.f / temp : 1.f;
+        const uint32_t lo = seeds[2 * s], hi = seeds[2 * s + 1];
+#pragma unroll
+        for (int k = 0; k < EACH; k++) {
+            const int i = index(k);
+            if (i < end) better(bv, bi, temp > 0.f ? v[k] * inv_t + gumbel(lo, hi, (uint32_t)(pos + 1), (uint32_t)i) : v[k], i);
+        }
+    }
+    auto reduce = [&](int lanes) {
+        for (int o = lanes / 2; o > 0; o >>= 1) {
+            const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
+            const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
+            better(bv, bi, ov, oi);
+        }
+    };
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    reduce(32);
+    if (lane == 0) sv[w] = bv, si[w] = bi;
+    __syncthreads();
+    if (w == 0) {
+        bv = lane < THREADS / 32 ? sv[lane] : -INFINITY;
+        bi = lane < THREADS / 32 ? si[lane] : 0x7fffffff;
+        reduce(THREADS / 32);
+        if (lane == 0) {
+            const size_t at = (size_t)row * gridDim.x + blockIdx.x;
+            ws_val[at] = bv, ws_idx[at] = bi;
+        }
+    }
+}
+
+// grid (sequences)
+__global__ void __launch_bounds__(THREADS)
+accept_path_kernel(const float* ws_val, const int* ws_idx, int pieces, const int* cu_q, const int* tok, const int* parent, int max_nodes,
+                   int* path, int* n_path, int* next_tok) {
+    __shared__ int choice[MAX_NODES], toks[MAX_NODES], up[MAX_NODES];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int s = blockIdx.x, row0 = cu_q[s], n = min(max_nodes, cu_q[s + 1] - row0);
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    for (int i = threadIdx.x; i < n; i += THREADS) toks[i] = tok[row0 + i], up[i] = parent[row0 + i];
+    for (int i = w; i < n; i += THREADS / 32) {
+        float bv = -INFINITY;
+        int bi = 0x7fffffff;
+        const size_t at = (size_t)(row0 + i) * pieces;
+        for (int c = lane; c < pieces; c += 32) better(bv, bi, ws_val[at + c], ws_idx[at + c]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
+            const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
+            better(bv, bi, ov, oi);
+        }
+        if (lane == 0) choice[i] = bi == 0x7fffffff ? 0 : bi;
+    }
+    __syncthreads();
+    if (w != 0) return;
+    int at = 0, len = 0;
+    int* out = path + (size_t)s * max_nodes;
+    if (n > 0) {
+        if (lane == 0) out[0] = 0;
+        len = 1;
+        for (int i0 = 1; i0 < n;) {                                    // a child stands behind its parent: one run over the nodes
+            const int i = i0 + lane;
+            const unsigned hit = __ballot_sync(0xffffffffu, i < n && up[i] == at && toks[i] == choice[at]);
+            if (!hit) {
+                i0 += 32;
+                continue;
+            }
+            at = i0 + __ffs(hit) - 1;
+            if (lane == 0) out[len] = at;
+            len++;
+            i0 = at + 1;
+        }
+    }
+    for (int i = len + lane; i < max_nodes; i += 32) out[i] = -1;
+    if (lane == 0) n_path[s] = len, next_tok[s] = n > 0 ? choice[at] : 0;
+}
+
+}  // namespace
+
+DK_EXPORT int dk_tree_accept_pieces(int V) { return (V + CHUNK - 1) / CHUNK; }
+
+// logits [rows, V] float32; temperature [n_seq], seeds [n_seq][2]; ws_val, ws_idx: rows * dk_tree_accept_pieces(V) elements;
+// path [n_seq, max_nodes], n_path [n_seq], next_tok [n_seq].
+DK_EXPORT int dk_tree_accept(const float* logits, int V, const int* tok, const int* parent, const int* cu_q, const int* row_pos,
+                             const float* temperature, const uint32_t* seeds, int n_seq, int max_nodes, float* ws_val, int* ws_idx,
+                             int* path, int* n_path, int* next_tok, cudaStream_t st) {
+    if (V < 1 || max_nodes < 1 || max_nodes > MAX_NODES || n_seq < 1 || n_seq > 65535) return (int)cudaErrorInvalidValue;
+    const int pieces = dk_tree_accept_pieces(V);
+    const bool wide = V % 4 == 0 && ((uintptr_t)logits & 15) == 0;      // rows on 16-byte boundaries: 16 bytes a load
+    int e = dk_launch(wide ? accept_pieces_kernel<true> : accept_pieces_kernel<false>, dim3(pieces, max_nodes, n_seq), dim3(THREADS), 0, st,
+                      logits, V, cu_q, row_pos, temperature, seeds, ws_val, ws_idx);
+    if (e) return e;
+    return dk_launch(accept_path_kernel, dim3(n_seq), dim3(THREADS), 0, st, (const float*)ws_val, (const int*)ws_idx, pieces, cu_q, tok,
+                     parent, max_nodes, path, n_path, next_tok);
+}
