@@ -857,7 +857,7 @@ def gemm_tc_check():
             _tc_err.zero_()
             for t in _attn_sched.values():
                 t.zero_()
-            kernel = "gemm_f32_tc" if 11 <= code <= 15 else "gemm_tc or attention_prefill_tc"
+            kernel = "gemm_f32_tc" if 11 <= code <= 15 else "attention_tree" if 21 <= code <= 23 else "gemm_tc or attention_prefill_tc"
             raise KernelError(f"{kernel}: a bounded wait ran out (code {code}); its results are not valid")
 
 
@@ -2186,30 +2186,31 @@ TREE_MAX_GROUP = 64         # query heads a kv head
 MAX_BEAMS, MAX_BEST = 32, 64
 
 
-def _same_device(what, *tensors):
-    """All on the device whose stream the launch goes to."""
-    for t in tensors:
-        if t is not None and t.is_cuda and t.device.index != torch.cuda.current_device():
-            raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+def _need_all(what, tensors):
+    """Each of ``tensors`` (tensor or None, name, dtype, shape): contiguous, of that type and shape, on the current device."""
+    device = torch.cuda.current_device() if tensors[0][0].is_cuda else None
+    for t, name, dtype, shape in tensors:
+        if t is None or (t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == device):
+            continue
+        _need(t, name, dtype, len(shape))
+        if t.shape != shape:
+            raise KernelError(f"{what}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+        raise KernelError(f"{what}: {name} on {t.device}, the current device is cuda:{device}")
 
 
-def _need_shape(t, name, shape):
-    if t is not None and tuple(t.shape) != tuple(shape):
-        raise KernelError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-
-
-def _need_tree(what, rows, n_seq, max_nodes, cu_q, row_pos):
-    if not 1 <= max_nodes <= TREE_MAX_NODES:
-        raise KernelError(f"{what}: max_nodes {max_nodes}, trees have 1 to {TREE_MAX_NODES} nodes")
-    _need(cu_q, "cu_q", torch.int32, 1), _need(row_pos, "row_pos", torch.int32, 1)
-    _need_shape(cu_q, "cu_q", (n_seq + 1,)), _need_shape(row_pos, "row_pos", (rows,))
-    if not 1 <= n_seq <= 65535:
-        raise KernelError(f"{what}: {n_seq} sequences, 1 to 65535 go in one call")
+def _need_counts(what, n_seq, max_nodes):
+    if not 1 <= max_nodes <= TREE_MAX_NODES or not 1 <= n_seq <= 65535:
+        raise KernelError(f"{what}: {n_seq} sequences (1 to 65535) of up to {max_nodes} nodes (1 to {TREE_MAX_NODES})")
 
 
 @functools.lru_cache(maxsize=None)
-def _tree_blocks(head_dim, f32, max_nodes, group):
-    return _lib("attention_tree.cu", {"HD": head_dim}).dk_attn_tree_blocks(f32, max_nodes, group)
+def _tree_plan(head_dim, f32, max_nodes, group):
+    """(whether the tensor-core kernel takes it, blocks of a launch, rows of a tile)."""
+    if not f32 and head_dim in TC_ATTENTION_HEAD_DIMS:
+        lib = _lib("attention_tree_tc.cu", {"HD": head_dim})
+        return True, lib.dk_tree_tc_blocks_per_sm() * sm_count(), lib.dk_tree_tc_tile_rows()
+    lib = _lib("attention_tree.cu", {"HD": head_dim})
+    return False, lib.dk_attn_tree_blocks(f32, max_nodes, group), lib.dk_tree_tile_rows(max_nodes, group)
 
 
 def attention_tree(q, out, k_store, v_store, cu_q, seq_pos0, row_pos, tree, page_table, n_heads, n_kv_heads, head_dim, window, scale,
@@ -2223,37 +2224,47 @@ def attention_tree(q, out, k_store, v_store, cu_q, seq_pos0, row_pos, tree, page
     it. A page id outside the store holds no keys. q and out [rows, heads * head_dim] (rows of wider matrices, 16-byte boundaries),
     float32 or bfloat16, head sizes in steps of 16 up to 256. The lengths are read on the device: a captured graph may be replayed
     with other ones, as long as ``max_nodes`` and the table's width hold."""
+    global _tc_err
     _need_rows(q, "q"), _need_rows(out, "out", q.dtype)
-    rows, n_seq = q.shape[0], seq_pos0.shape[0]
-    _need_tree("attention_tree", rows, n_seq, max_nodes, cu_q, row_pos)
-    _need(seq_pos0, "seq_pos0", torch.int32, 1), _need(tree, "tree", torch.int32, 2), _need(page_table, "page_table", torch.int32, 2)
-    _need(k_store, "k_store", q.dtype, 4), _need(v_store, "v_store", q.dtype, 4)
+    _dt(q)
+    n_seq, (rows, width) = seq_pos0.shape[0], q.shape
+    _need_counts("attention_tree", n_seq, max_nodes)
     if head_dim % 16 or not 16 <= head_dim <= 256 or n_kv_heads < 1 or n_heads % n_kv_heads or not 1 <= n_heads // n_kv_heads <= TREE_MAX_GROUP:
         raise KernelError(f"attention_tree: head size {head_dim} (multiples of 16 up to 256) / heads {n_heads}:{n_kv_heads} (up to "
                           f"{TREE_MAX_GROUP} a kv head) not supported")
-    _need_shape(q, "q", (rows, n_heads * head_dim)), _need_shape(out, "out", (rows, n_heads * head_dim))
-    _need_shape(k_store, "k_store", (k_store.shape[0], n_kv_heads, PAGE, head_dim)), _need_shape(v_store, "v_store", k_store.shape)
-    _need_shape(tree, "tree", (rows, tree.shape[1])), _need_shape(page_table, "page_table", (n_seq, page_table.shape[1]))
-    if k_store.shape[0] < 1 or page_table.shape[1] < 1 or tree.shape[1] < 1:
-        raise KernelError("attention_tree: an empty store, page table or row of tree bits")
-    if not scale > 0 or int(window or 0) < 0:
+    if width != n_heads * head_dim or out.shape != q.shape:
+        raise KernelError(f"attention_tree: q {tuple(q.shape)} and out {tuple(out.shape)} must be [rows, {n_heads} * {head_dim}]")
+    n_pages, words, table = k_store.shape[0], tree.shape[-1], page_table.shape[-1]
+    store = (n_pages, n_kv_heads, PAGE, head_dim)
+    _need_all("attention_tree", ((k_store, "k_store", q.dtype, store), (v_store, "v_store", q.dtype, store), (cu_q, "cu_q", torch.int32, (n_seq + 1,)),
+                                 (seq_pos0, "seq_pos0", torch.int32, (n_seq,)), (row_pos, "row_pos", torch.int32, (rows,)),
+                                 (tree, "tree", torch.int32, (rows, words)), (page_table, "page_table", torch.int32, (n_seq, table))))
+    if n_pages < 1 or n_pages * n_kv_heads * PAGE >= 1 << 31 or table < 1 or words < 1:
+        raise KernelError("attention_tree: a store, page table or row of tree bits that is empty, or a store of 2^31 rows")
+    if not scale > 0 or (window or 0) < 0:
         raise KernelError(f"attention_tree: scale {scale} must be positive, window {window} not negative")
-    size = q.element_size()
-    if any(t.data_ptr() % 16 or t.stride(0) * size % 16 for t in (q, out)):
+    if (q.data_ptr() | out.data_ptr() | q.stride(0) * q.element_size() | out.stride(0) * q.element_size()) % 16:
         raise KernelError("attention_tree: rows of q and out must lie on 16-byte boundaries")
-    _same_device("attention_tree", q, out, k_store, v_store, cu_q, seq_pos0, row_pos, tree, page_table)
+    if q.get_device() != cu_q.get_device() or out.get_device() != cu_q.get_device():
+        raise KernelError("attention_tree: q and out must be on the current device")
     if rows == 0:
         return
-    group, f32 = n_heads // n_kv_heads, int(q.dtype == torch.float32)
-    _dt(q)
-    lib = _lib("attention_tree.cu", {"HD": head_dim})
-    blocks = _tree_blocks(head_dim, f32, max_nodes, group)
-    n = 2 * blocks * lib.dk_tree_tile_rows(max_nodes, group)
-    ws = torch.empty(n * (head_dim + 2), dtype=torch.float32, device=q.device)
-    _check(lib, lib.dk_attn_tree(f32, _p(q), c_longlong(q.stride(0)), _p(out), c_longlong(out.stride(0)), _p(k_store), _p(v_store),
-                                 k_store.shape[0], _p(cu_q), _p(seq_pos0), _p(row_pos), _p(tree), tree.shape[1], _p(page_table),
-                                 page_table.shape[1], n_seq, n_heads, n_kv_heads, int(window or 0), c_float(scale), max_nodes,
-                                 _p(ws), _p(ws[n * head_dim:]), blocks, _stream()), "attention_tree", 2)
+    f32 = int(q.dtype == torch.float32)
+    tc, blocks, tile = _tree_plan(head_dim, f32, max_nodes, n_heads // n_kv_heads)
+    n = 2 * blocks * tile * head_dim
+    ws = torch.empty(n + 4 * blocks * tile, dtype=torch.float32, device=q.device)
+    head = (_p(q), c_longlong(q.stride(0)), _p(out), c_longlong(out.stride(0)))
+    body = (_p(k_store), _p(v_store), n_pages, _p(cu_q), _p(seq_pos0), _p(row_pos), _p(tree), words, _p(page_table), table, n_seq, n_heads,
+            n_kv_heads, int(window or 0), c_float(scale), max_nodes, _p(ws), c_void_p(ws.data_ptr() + 4 * n), blocks)
+    if tc:
+        if _tc_err is None:
+            _tc_err = torch.zeros(1, dtype=torch.int32, device=q.device)
+        lib = _lib("attention_tree_tc.cu", {"HD": head_dim})
+        err = lib.dk_attn_tree_tc(*head, c_longlong(rows), *body, _p(_tc_err), _stream())
+    else:
+        lib = _lib("attention_tree.cu", {"HD": head_dim})
+        err = lib.dk_attn_tree(f32, *head, *body, _stream())
+    _check(lib, err, "attention_tree", 2)
 
 
 def tree_accept(logits, tok, parent, cu_q, row_pos, temperature, seeds, path, n_path, next_tok):
@@ -2263,23 +2274,20 @@ def tree_accept(logits, tok, parent, cu_q, row_pos, temperature, seeds, path, n_
     ``sample`` chooses from its logits at row_pos; from node 0 on the path goes to the child that holds it (the lowest such child)
     until there is none. ``path`` [n_seq, max_nodes] becomes the nodes on the way, node 0 first, -1 behind them, ``n_path`` [n_seq]
     their number, ``next_tok`` [n_seq] the token chosen at the last of them. A sequence without nodes gets 0 nodes and token 0."""
-    _need(logits, "logits", torch.float32, 2), _need(tok, "tok", torch.int32, 1), _need(parent, "parent", torch.int32, 1)
-    _need(temperature, "temperature", torch.float32, 1), _need(seeds, "seeds", torch.int32, 2), _need(path, "path", torch.int32, 2)
-    _need(n_path, "n_path", torch.int32, 1), _need(next_tok, "next_tok", torch.int32, 1)
+    if logits.dim() != 2 or path.dim() != 2 or logits.shape[1] < 1:
+        raise KernelError(f"tree_accept: logits {tuple(logits.shape)} must be [rows, vocab], path {tuple(path.shape)} [sequences, nodes]")
     (rows, V), (n_seq, max_nodes) = logits.shape, path.shape
-    _need_tree("tree_accept", rows, n_seq, max_nodes, cu_q, row_pos)
-    for t, name, shape in ((tok, "tok", (rows,)), (parent, "parent", (rows,)), (temperature, "temperature", (n_seq,)),
-                           (seeds, "seeds", (n_seq, 2)), (n_path, "n_path", (n_seq,)), (next_tok, "next_tok", (n_seq,))):
-        _need_shape(t, name, shape)
-    if V < 1:
-        raise KernelError("tree_accept: logits without columns")
-    _same_device("tree_accept", logits, tok, parent, cu_q, row_pos, temperature, seeds, path, n_path, next_tok)
+    _need_counts("tree_accept", n_seq, max_nodes)
+    _need_all("tree_accept", ((logits, "logits", torch.float32, (rows, V)), (tok, "tok", torch.int32, (rows,)),
+                              (parent, "parent", torch.int32, (rows,)), (cu_q, "cu_q", torch.int32, (n_seq + 1,)),
+                              (row_pos, "row_pos", torch.int32, (rows,)), (temperature, "temperature", torch.float32, (n_seq,)),
+                              (seeds, "seeds", torch.int32, (n_seq, 2)), (path, "path", torch.int32, (n_seq, max_nodes)),
+                              (n_path, "n_path", torch.int32, (n_seq,)), (next_tok, "next_tok", torch.int32, (n_seq,))))
     lib = _lib("tree_accept.cu")
     n = max(1, rows * lib.dk_tree_accept_pieces(V))
-    ws_val = torch.empty(n, dtype=torch.float32, device=logits.device)
-    ws_idx = torch.empty(n, dtype=torch.int32, device=logits.device)
+    ws = torch.empty(2 * n, dtype=torch.int32, device=logits.device)
     _check(lib, lib.dk_tree_accept(_p(logits), V, _p(tok), _p(parent), _p(cu_q), _p(row_pos), _p(temperature), _p(seeds), n_seq, max_nodes,
-                                   _p(ws_val), _p(ws_idx), _p(path), _p(n_path), _p(next_tok), _stream()), "tree_accept", 2)
+                                   _p(ws), c_void_p(ws.data_ptr() + 4 * n), _p(path), _p(n_path), _p(next_tok), _stream()), "tree_accept", 2)
 
 
 def beam_select(logits, scores, ended, scores_out, beam_out, tok_out):
@@ -2289,24 +2297,24 @@ def beam_select(logits, scores, ended, scores_out, beam_out, tok_out):
     end and stands for itself alone, its own score with token 0. A logit that is not finite is no candidate and weighs nothing, a beam
     whose score is not finite brings no candidates; where there are fewer than asked for the rest is (-infinity, 0, 0). Up to 32 beams
     and 64 results, which may not lie in ``scores``."""
-    _need(logits, "logits", torch.float32, 2), _need(scores, "scores", torch.float32, 2), _need(ended, "ended", torch.int32, 2)
-    _need(scores_out, "scores_out", torch.float32, 2), _need(beam_out, "beam_out", torch.int32, 2), _need(tok_out, "tok_out", torch.int32, 2)
+    if scores.dim() != 2 or scores_out.dim() != 2 or logits.dim() != 2:
+        raise KernelError("beam_select: logits, scores and results have two dimensions each")
     (requests, beams), best, V = scores.shape, scores_out.shape[1], logits.shape[1]
     if requests < 1 or not 1 <= beams <= MAX_BEAMS or not 1 <= best <= MAX_BEST or V < 1:
         raise KernelError(f"beam_select: {requests} requests, {beams} beams (1 to {MAX_BEAMS}), {best} results (1 to {MAX_BEST}), {V} tokens")
     if requests * beams > 65535 or beams * V >= 1 << 31:
         raise KernelError(f"beam_select: {requests} requests of {beams} beams over {V} tokens are too many for one call")
-    _need_shape(logits, "logits", (requests * beams, V)), _need_shape(ended, "ended", (requests, beams))
-    for t, name in ((scores_out, "scores_out"), (beam_out, "beam_out"), (tok_out, "tok_out")):
-        _need_shape(t, name, (requests, best))
-    _same_device("beam_select", logits, scores, ended, scores_out, beam_out, tok_out)
+    one, out = (requests, beams), (requests, best)
+    _need_all("beam_select", ((logits, "logits", torch.float32, (requests * beams, V)), (scores, "scores", torch.float32, one),
+                              (ended, "ended", torch.int32, one), (scores_out, "scores_out", torch.float32, out),
+                              (beam_out, "beam_out", torch.int32, out), (tok_out, "tok_out", torch.int32, out)))
     lib = _lib("beam_select.cu")
     pieces = lib.dk_beam_pieces(V)
     if not lib.dk_beam_select_takes(V, beams, best):
         raise KernelError(f"beam_select: {best} of {beams} beams over {V} tokens need more shared memory than a block has")
-    ws_key = torch.empty(requests * beams * pieces * best, dtype=torch.int64, device=logits.device)
-    ws_sum = torch.empty(requests * beams * pieces * 2, dtype=torch.float64, device=logits.device)
-    _check(lib, lib.dk_beam_select(_p(logits), V, requests, beams, best, _p(scores), _p(ended), _p(ws_key), _p(ws_sum), _p(scores_out),
+    n = requests * beams * pieces
+    ws = torch.empty(n * (best + 2), dtype=torch.int64, device=logits.device)      # pairs of doubles first, then the keys
+    _check(lib, lib.dk_beam_select(_p(logits), V, requests, beams, best, _p(scores), _p(ended), c_void_p(ws.data_ptr() + 16 * n), _p(ws), _p(scores_out),
                                    _p(beam_out), _p(tok_out), _stream()), "beam_select", 2)
 
 
@@ -2317,7 +2325,8 @@ def _need_store(store, page_table, what):
     row = store.shape[-1] * store.element_size()
     if row % 2 or store.data_ptr() % 2:
         raise KernelError(f"{what}: rows of {row} bytes, which must be even")
-    _need(page_table, "page_table", torch.int32, 2)
+    if page_table.dim() != 2 or page_table.shape[1] < 1 or store.device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: a page table {tuple(page_table.shape)} that is not [sequences, pages], or a store on another device")
     pages, nkv = store.shape[-4], store.shape[-3]
     return store.numel() // (pages * nkv * PAGE * store.shape[-1]), pages, nkv, row
 
@@ -2328,24 +2337,21 @@ def kv_keep(store, page_table, seq_pos0, path, n_path):
     ``path`` [n_seq, up to 1024] rising, as ``tree_accept`` leaves it (a row whose path[s, k] <= k stays where it is). All other rows
     keep what they hold. Places outside the table and pages outside the store are left out."""
     outer, pages, nkv, row = _need_store(store, page_table, "kv_keep")
-    _need(seq_pos0, "seq_pos0", torch.int32, 1), _need(path, "path", torch.int32, 2), _need(n_path, "n_path", torch.int32, 1)
+    if path.dim() != 2:
+        raise KernelError(f"kv_keep: path {tuple(path.shape)} must be [sequences, nodes]")
     n_seq, width = path.shape
-    if not 1 <= width <= TREE_MAX_NODES or not 1 <= n_seq <= 65535 or page_table.shape[1] < 1:
-        raise KernelError(f"kv_keep: paths of {width} nodes (1 to {TREE_MAX_NODES}) of {n_seq} sequences")
-    for t, name, shape in ((seq_pos0, "seq_pos0", (n_seq,)), (n_path, "n_path", (n_seq,)), (page_table, "page_table", (n_seq, page_table.shape[1]))):
-        _need_shape(t, name, shape)
-    _same_device("kv_keep", store, page_table, seq_pos0, path, n_path)
+    _need_counts("kv_keep", n_seq, width)
+    _need_all("kv_keep", ((page_table, "page_table", torch.int32, (n_seq, page_table.shape[1])), (seq_pos0, "seq_pos0", torch.int32, (n_seq,)),
+                          (path, "path", torch.int32, (n_seq, width)), (n_path, "n_path", torch.int32, (n_seq,))))
     lib = _lib("cache_moves.cu")
     _check(lib, lib.dk_kv_keep(_p(store), outer, pages, nkv, c_longlong(row), _p(page_table), page_table.shape[1], n_seq, _p(seq_pos0),
                                _p(path), width, _p(n_path), _stream()), "kv_keep")
 
 
-def _need_parents(parent, what):
-    _need(parent, "parent", torch.int32, 2)
-    requests, beams = parent.shape
-    if not 1 <= requests <= 65535 or not 1 <= beams <= MAX_BEAMS:
-        raise KernelError(f"{what}: {requests} requests of {beams} beams (1 to {MAX_BEAMS})")
-    return requests, beams
+def _beams(parent, what):
+    if parent.dim() != 2 or not 1 <= parent.shape[0] <= 65535 or not 1 <= parent.shape[1] <= MAX_BEAMS:
+        raise KernelError(f"{what}: parent {tuple(parent.shape)} must be [requests, beams], 1 to {MAX_BEAMS} beams")
+    return parent.shape
 
 
 def kv_reorder(store, page_table, parent, first, last):
@@ -2354,14 +2360,11 @@ def kv_reorder(store, page_table, parent, first, last):
     any type. The sequences' pages are their own; rows outside [first, last), beams that are their own parents (or whose parent is
     none of the request's), places outside the table and pages outside the store are left as they were."""
     outer, pages, nkv, row = _need_store(store, page_table, "kv_reorder")
-    requests, beams = _need_parents(parent, "kv_reorder")
-    _need(first, "first", torch.int32, 1), _need(last, "last", torch.int32, 1)
-    if outer > 65535 or page_table.shape[1] < 1:
-        raise KernelError(f"kv_reorder: {outer} stores in one call, or a table without columns")
-    for t, name, shape in ((first, "first", (requests,)), (last, "last", (requests,)),
-                           (page_table, "page_table", (requests * beams, page_table.shape[1]))):
-        _need_shape(t, name, shape)
-    _same_device("kv_reorder", store, page_table, parent, first, last)
+    requests, beams = _beams(parent, "kv_reorder")
+    if outer > 65535:
+        raise KernelError(f"kv_reorder: {outer} stores in one call, 65535 at most")
+    _need_all("kv_reorder", ((page_table, "page_table", torch.int32, (requests * beams, page_table.shape[1])), (parent, "parent", torch.int32,
+              (requests, beams)), (first, "first", torch.int32, (requests,)), (last, "last", torch.int32, (requests,))))
     lib = _lib("cache_moves.cu")
     _check(lib, lib.dk_kv_reorder(_p(store), outer, pages, nkv, c_longlong(row), _p(page_table), page_table.shape[1], requests, beams,
                                   _p(parent), _p(first), _p(last), _stream()), "kv_reorder")
@@ -2371,14 +2374,13 @@ def state_reorder(store, seq_slot, parent):
     """Every beam takes its parent's state, in place: in each entry of ``store`` [entries, slots, ..] of any type, slot
     seq_slot[r * beams + b] gets what slot seq_slot[r * beams + parent[r, b]] held before the call. The slots are distinct; beams that
     are their own parents (or whose parent is none of the request's) and slots outside the store are left as they were."""
-    requests, beams = _need_parents(parent, "state_reorder")
-    _need(seq_slot, "seq_slot", torch.int32, 1), _need_shape(seq_slot, "seq_slot", (requests * beams,))
+    requests, beams = _beams(parent, "state_reorder")
+    _need_all("state_reorder", ((seq_slot, "seq_slot", torch.int32, (requests * beams,)), (parent, "parent", torch.int32, (requests, beams))))
     if not store.is_cuda or not store.is_contiguous() or store.dim() < 2 or store.numel() == 0 or store.shape[0] > 65535:
         raise KernelError(f"state_reorder: store must be a contiguous CUDA tensor [entries, slots, ..], got {tuple(store.shape)}")
     size = store.numel() // (store.shape[0] * store.shape[1]) * store.element_size()
-    if size % 2 or store.data_ptr() % 2:
-        raise KernelError(f"state_reorder: states of {size} bytes, which must be even")
-    _same_device("state_reorder", store, seq_slot, parent)
+    if size % 2 or store.data_ptr() % 2 or store.get_device() != torch.cuda.current_device():
+        raise KernelError(f"state_reorder: states of {size} bytes, which must be even, or a store on another device")
     lib = _lib("cache_moves.cu")
     _check(lib, lib.dk_state_reorder(_p(store), store.shape[0], store.shape[1], c_longlong(size), _p(seq_slot), requests, beams, _p(parent),
                                      _stream()), "state_reorder")
