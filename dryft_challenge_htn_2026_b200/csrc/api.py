@@ -2208,7 +2208,7 @@ def _tree_plan(head_dim, f32, max_nodes, group):
     """(whether the tensor-core kernel takes it, blocks of a launch, rows of a tile)."""
     if not f32 and head_dim in TC_ATTENTION_HEAD_DIMS:
         lib = _lib("attention_tree_tc.cu", {"HD": head_dim})
-        return True, lib.dk_tree_tc_blocks_per_sm() * sm_count(), lib.dk_tree_tc_tile_rows()
+        return True, sm_count(), lib.dk_tree_tc_tile_rows()
     lib = _lib("attention_tree.cu", {"HD": head_dim})
     return False, lib.dk_attn_tree_blocks(f32, max_nodes, group), lib.dk_tree_tile_rows(max_nodes, group)
 

@@ -35,12 +35,12 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
     pdl_wait();
     pdl_launch_dependents();
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, G = a.nh / a.nkv;
-    const long long total = tree_units(a, a.n_seq);
+    int before;
+    const int total = tree_units(a, 0, before);
     const int nb = share_count(total, gridDim.x);
     if ((int)blockIdx.x >= nb) return;
-    long long u = share_begin(total, blockIdx.x, nb);
-    const long long u_end = share_begin(total, blockIdx.x + 1, nb);
-    long long before;
+    int u = share_begin(total, blockIdx.x, nb);
+    const int u_end = share_begin(total, blockIdx.x + 1, nb);
     int s = tree_find(a, u, before);
     TreeSeq sq;
     sq.load(a, s);
@@ -49,8 +49,7 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
             before += sq.units(a.nkv);
             sq.load(a, ++s);
         }
-        const long long at = u - before;
-        const int item = (int)(at / sq.pages), p0 = (int)(at % sq.pages), p1 = (int)min((long long)sq.pages, p0 + (u_end - u));
+        const int at = u - before, item = at / sq.pages, p0 = at % sq.pages, p1 = min(sq.pages, p0 + (u_end - u));
         const int kvh = item / sq.tiles, node0 = (item % sq.tiles) * a.tile_nodes;
         const int rows = min(a.tile_nodes, sq.n - node0) * G, flat0 = sq.flat0 + node0;
         const int* pt = a.page_table + (size_t)s * a.pt_stride;
@@ -173,7 +172,7 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
             } else {
                 if (tx == 0) ws_ml[slot + r] = make_float2(m[i], l[i]);
 #pragma unroll
-                for (int c = 0; c < CV; c++) ws_acc[(slot + r) * HD + tx + 16 * c] = acc[i][c];
+                for (int c = 0; c < CV; c++) ws_acc[slot * HD + part_at(TM, r, tx + 16 * c)] = acc[i][c];
             }
         }
         u += p1 - p0;
@@ -196,8 +195,7 @@ int launch(const TreeArgs& a, const void* q, long long ldq, void* out, long long
     int r = dk_launch(tree_kernel<T, NI>, dim3(blocks), dim3(THREADS), tree_smem<NI>(), st, a, (const T*)q, ldq, (T*)out, ldo,
                       (const T*)k_store, (const T*)v_store, ws_acc, (float2*)ws_ml);
     if (r) return r;
-    return dk_launch(tree_merge_kernel<T, HD>, dim3((unsigned)(((long long)max_nodes * a.nh + 7) / 8), a.n_seq), dim3(256), 0, st, a,
-                     (const float*)ws_acc, (const float2*)ws_ml, (T*)out, ldo, 16 * NI, blocks);
+    return tree_merge<T, HD>(a, ws_acc, ws_ml, out, ldo, 16 * NI, max_nodes, blocks, st);
 }
 
 }  // namespace
@@ -232,8 +230,9 @@ DK_EXPORT int dk_attn_tree(int f32, const void* q, long long ldq, void* out, lon
     if (nkv < 1 || nh % nkv || nh / nkv > 64 || n_pages < 1 || pt_stride < 1 || words < 1 || blocks < 1 || max_nodes < 1 || n_seq > 65535)
         return (int)cudaErrorInvalidValue;
     const int G = nh / nkv, rows = dk_tree_tile_rows(max_nodes, G);
-    TreeArgs a = {cu_q, seq_pos0, row_pos, page_table, tree, n_seq, words, pt_stride, n_pages, nh, nkv, window, rows / G,
+    TreeArgs a = {cu_q, seq_pos0, row_pos, page_table, tree, n_seq, words, pt_stride, n_pages, nh, nkv, window, rows / G, rows / G, rows,
                   scale * 1.4426950408889634f};
+    if (!tree_units_fit(a, max_nodes) || nkv > 65535) return (int)cudaErrorInvalidValue;
 #define DK_TREE(T, NI) launch<T, NI>(a, q, ldq, out, ldo, k_store, v_store, ws_acc, ws_ml, max_nodes, blocks, st)
     if (f32) return rows == 16 ? DK_TREE(float, 1) : rows == 32 ? DK_TREE(float, 2) : DK_TREE(float, 4);
     return rows == 16 ? DK_TREE(bf16, 1) : rows == 32 ? DK_TREE(bf16, 2) : DK_TREE(bf16, 4);

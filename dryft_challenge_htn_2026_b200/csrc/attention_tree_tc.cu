@@ -1,18 +1,26 @@
 // bfloat16 attention of trees of drafted tokens over the paged cache on the 5th-generation tensor cores, for head sizes 64 and 128
 // (built per head size with -DHD=64 or -DHD=128). Which keys a node sees and how the work is dealt out: attention_tree.cuh.
 //
-// A tile is 128 rows, nodes x the query heads of one kv head (four heads a kv head: 32 nodes), so that a page of keys is read once for
-// all of them. A block walks the pages of its share:
-//   warp 5, one thread: TMA loads. Q once a tile, as boxes [tile nodes][heads of the kv head][64 columns]; K and V of each page as
-//       [64 keys x 64 columns], 128-byte swizzle, two stages each.
-//   warp 4, one thread: all tcgen05.mma. S[128 x 64] = Q.K^T into one of two buffers, O[128 x HD] += P.V with P from tensor memory. S
-//       runs two pages ahead of P.V.
-//   warps 0-3: softmax, a thread a row: its row of S from tensor memory, running maximum and sum in float32, P as bfloat16 (rounded
-//       once, to be the product's operand; the sum takes the unrounded weights) over its S buffer, and at the end the row of O.
+// A block, one an SM, has two streams A and B of softmax warps, score buffers and accumulators, which share the tensor core and the
+// pages that one thread loads:
+//   a tile of up to 256 rows (nodes x the query heads of one kv head; four heads a kv head: 64 nodes) goes with its first 128 rows to
+//   A and the rest to B, and every page is read once for both;
+//   a tile of up to 128 rows goes to both, A takes the even pages of the block's share and B the odd ones, and their results are put
+//   together from tensor memory (a row has the same lane in both accumulators).
+// Roles:
+//   warp 10, one thread: TMA loads. Q once a tile, as boxes [nodes][heads of the kv head][64 columns]; K and V of each page as [64 keys x
+//       64 columns], 128-byte swizzle, into rings of their own (a key page is free once S is computed, its values after P.V), K two
+//       pages ahead of V.
+//   warps 8 (A) and 9 (B), one thread each: the stream's tcgen05.mma. S[128 x 64] = Q.K^T into one of the stream's two buffers, O[128 x HD] += P.V with P from tensor
+//       memory. S runs two pages ahead of P.V.
+//   warps 0-3 (A), 4-7 (B): softmax, a thread a row: its row of S from tensor memory, running maximum and sum in float32, P as bfloat16
+//       (rounded once, to be the product's operand; the sum takes the unrounded weights) over its S buffer, at the end the row of O.
+// Nobody waits for a tile's end but for what it leaves: the loader runs on into the next tile's pages, S of the next tile starts while
+// the rows of the last one are written, only P.V into O waits until they are read.
 // Pages of cached tokens that every row sees need no mask. In the others (the tree's own, the first of a window) a row's 64 visible
 // places are one word of bits. P.V adds up 0 * v for what a row does not see: where such a page holds a value that is not finite it is
 // set to zero in shared memory, and at the end the rows that do see it take it up from the cache.
-// Tensor memory: S0 | S1 | O = 64 + 64 + 128 columns; two blocks an SM (96 KB of shared memory each at head size 128).
+// Tensor memory: S of A 0 | 1, S of B 0 | 1, O of A, O of B = 4 x 64 + 2 x 128 columns.
 // Every mbarrier wait is bounded; a wait that runs out stores a code in *err, and the block still frees its tensor memory and returns.
 #include <cuda.h>
 
@@ -25,16 +33,20 @@ static_assert(HD == 64 || HD == 128, "built for head sizes 64 and 128");
 
 namespace {
 
-constexpr int BM = 128, BN = DK_PAGE;             // rows a tile, keys a step (one page)
-constexpr int SOFT = 128;                         // softmax threads, one a row; then the mma warp, then the loader warp
-constexpr int THREADS = SOFT + 64;
-constexpr int BLOCKS_PER_SM = 2;
-constexpr int TMEM_ALLOC = 256;                   // S0 | S1 | O
-constexpr int OC = 32;                            // columns of O a thread handles at a time
+constexpr int BM = 128, BN = DK_PAGE;             // rows of a stream, keys a step (one page)
+constexpr int SOFT = 2 * BM;                      // softmax threads, one a row of each stream; then two mma warps, then the loader warp
+constexpr int THREADS = SOFT + 96, MMA_WARP = SOFT / 32, LOAD_WARP = MMA_WARP + 2;
+constexpr int TMEM_ALLOC = 512;
+constexpr int OC = 16;                            // columns of a row's result a thread handles at a time
 constexpr int HALVES = HD / 64;                   // 64-column swizzle atoms across the head
 constexpr int Q_BYTES = BM * HD * 2, KV_BYTES = BN * HD * 2;
 constexpr int Q_ATOM_BYTES = BM * 128, KV_ATOM_BYTES = BN * 128;
-constexpr size_t SMEM_BYTES = 1024 + Q_BYTES + 4 * KV_BYTES + 14 * sizeof(uint64_t);
+constexpr int NK = HD == 128 ? 5 : 9, NV = HD == 128 ? 4 : 8;          // pages in the rings
+constexpr int RING = 2 * Q_BYTES, V_RING = RING + NK * KV_BYTES, BARS = V_RING + NV * KV_BYTES;
+constexpr int N_BARS = 2 * NK + 2 * NV + 12 + 4;
+constexpr int ML = BARS + (N_BARS + 4) * 8;       // [2][2][BM] pairs (maximum, sum) that the streams exchange
+constexpr size_t SMEM_BYTES = 1024 + ML + 4 * BM * 8;
+static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of a block");
 #ifndef DK_WAIT_CYCLES
 #define DK_WAIT_CYCLES 2000000000LL               // about a second: a wait this long has failed
 #endif
@@ -129,6 +141,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
     asm volatile(
@@ -161,27 +179,63 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// grid min(units, 2 * SMs), 192 threads. q as [rows][heads][HD] (map_q), map_k / map_v over one layer's store as [pages * nkv * 64, HD].
-// The per-step barriers (K, V, S, P, O) complete once a step and bar_q once a tile: their phases run on over the tiles.
-__global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM)
+// Where a block stands in its share; every role walks it for itself.
+struct Walk {
+    TreeSeq sq;
+    int u, u_end, before, s;
+    // the tile at hand: its kv head, first node, nodes, pages [p0, p1) of the sequence's
+    int kvh, node0, nodes, p0, p1;
+    bool pair;                                             // two streams of rows; else two streams of pages
+    const int* pt;
+    __device__ __forceinline__ bool next(const TreeArgs& a) {
+        if (u >= u_end) return false;
+        while (u >= before + sq.units(a.nkv)) {
+            before += sq.units(a.nkv);
+            sq.load(a, ++s);
+        }
+        const int at = u - before, item = at / sq.pages;
+        p0 = at % sq.pages, p1 = min(sq.pages, p0 + (u_end - u));
+        kvh = item / sq.tiles, node0 = (item % sq.tiles) * a.tile_nodes;
+        nodes = min(a.tile_nodes, sq.n - node0);
+        pair = nodes > a.half_nodes;
+        pt = a.page_table + (size_t)s * a.pt_stride + sq.first_page;
+        u += p1 - p0;
+        return true;
+    }
+    __device__ __forceinline__ int pages() const { return p1 - p0; }
+    // steps of stream x, and the page of its step i, counted from p0
+    __device__ __forceinline__ int steps(int x) const { return pair ? pages() : (pages() + 1 - x) / 2; }
+    __device__ __forceinline__ int page_of(int x, int i) const { return pair ? i : 2 * i + x; }
+};
+
+// Uses of a ring of N barriers, in turn: the t-th is slot t % N in its (t / N)-th phase.
+template <int N> __device__ __forceinline__ uint32_t slot_of(uint32_t t) { return t % N; }
+template <int N> __device__ __forceinline__ uint32_t phase_of(uint32_t t) { return (t / N) & 1; }
+
+// grid SMs, 352 threads. q as [rows][heads][HD] (map_q), map_k / map_v over one layer's store as [pages * nkv * 64, HD].
+__global__ void __launch_bounds__(THREADS, 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                const __grid_constant__ TreeArgs a, bf16* out, long long ldo, const bf16* v_store, float* ws_acc, float2* ws_ml, int* err) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-    const uint32_t q_s = smem_u32(smem), k_s = q_s + Q_BYTES, v_s = k_s + 2 * KV_BYTES;   // Q, K stages 0 1, V stages 0 1
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Q_BYTES + 4 * KV_BYTES);
-    uint64_t *bar_q = bars, *bar_k = bars + 1, *bar_v = bars + 3, *bar_s = bars + 5, *bar_p = bars + 7, *bar_o = bars + 9;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 11);
-    volatile int* failed = reinterpret_cast<volatile int*>(bars + 12);     // [0] a wait ran out; [1] the last tile with a value that is not finite
+    const uint32_t q_s = smem_u32(smem), k_s = q_s + RING, v_s = q_s + V_RING;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + BARS);
+    uint64_t *k_full = bars, *k_free = k_full + NK, *v_full = k_free + NK, *v_free = v_full + NV;
+    uint64_t *s_full = v_free + NV, *p_full = s_full + 4, *o_full = p_full + 4;              // [stream][step & 1]
+    uint64_t *q_full = o_full + 4, *q_free = q_full + 1, *o_free = q_full + 2, *both = q_full + 3;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
+    volatile int* odd_tile = reinterpret_cast<volatile int*>(bars + N_BARS + 1);       // the last tile with a value that is not finite
+    float2* ml_s = reinterpret_cast<float2*>(smem + ML);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.nh / a.nkv;
-    constexpr int MMA_WARP = SOFT / 32, LOAD_WARP = MMA_WARP + 1;
 
     pdl_wait();
     if (threadIdx.x == 0) {
-        mbar_init(bar_q, 1);
-        for (int b = 0; b < 2; b++)
-            mbar_init(bar_k + b, 1), mbar_init(bar_v + b, 1), mbar_init(bar_s + b, 1), mbar_init(bar_o + b, 1), mbar_init(bar_p + b, SOFT);
-        failed[0] = 0, failed[1] = 0;
+        for (int i = 0; i < N_BARS; i++) {
+            uint64_t* b = bars + i;
+            const bool two = (b >= k_free && b < v_full) || (b >= v_free && b < s_full) || b == q_free;     // both streams say so
+            mbar_init(b, b >= p_full && b < o_full ? BM : b == o_free || b == both ? SOFT : two ? 2 : 1);
+        }
+        *odd_tile = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -190,150 +244,162 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // where the block's share begins; every warp finds it for itself
-    const long long total = tree_units(a, a.n_seq);
-    const int nb = share_count(total, gridDim.x);
-    const bool busy = (int)blockIdx.x < nb;
-    long long u = busy ? share_begin(total, blockIdx.x, nb) : 0, before = 0;
-    const long long u_end = busy ? share_begin(total, blockIdx.x + 1, nb) : 0;
-    int s = busy ? tree_find(a, u, before) : 0;
+    Walk w;
+    w.before = w.u = w.u_end = 0;
+    {
+        const int total = tree_units(a, 0, w.before);
+        const int nb = share_count(total, gridDim.x);
+        if ((int)blockIdx.x < nb) {
+            w.u = share_begin(total, blockIdx.x, nb), w.u_end = share_begin(total, blockIdx.x + 1, nb);
+            w.s = tree_find(a, w.u, w.before);
+            w.sq.load(a, w.s);
+        }
+    }
     fence_before();
     __syncthreads();
     fence_after();
     pdl_launch_dependents();       // not before every block holds its tensor memory: the next kernel's blocks may want some too
     const uint32_t tmem = *tmem_slot;
-    const uint32_t t_s = tmem, t_o = tmem + 2 * BN;        // S buffers (and P over them) of BN columns each, then O of HD columns
+    const uint32_t t_s = tmem, t_o = tmem + 4 * BN;        // S (and P over it) of [stream][step & 1], BN columns each; O of [stream], 128 each
 
-    TreeSeq sq;
-    if (busy) sq.load(a, s);
-    uint32_t step = 0;
-    int tiles_done = 0;
-    while (u < u_end && !failed[0]) {
-        while (u >= before + sq.units(a.nkv)) {
-            before += sq.units(a.nkv);
-            sq.load(a, ++s);
-        }
-        const long long at = u - before;
-        const int item = (int)(at / sq.pages), p0 = (int)(at % sq.pages), p1 = (int)min((long long)sq.pages, p0 + (u_end - u));
-        const int kvh = item / sq.tiles, node0 = (item % sq.tiles) * a.tile_nodes;
-        const int rows = min(a.tile_nodes, sq.n - node0) * G, flat0 = sq.flat0 + node0;
-        const int* pt = a.page_table + (size_t)s * a.pt_stride + sq.first_page;
-        const int n_blk = p1 - p0;
-
-        // Step j of the tile is step t = step + j of the block; it uses stage / buffer / barrier t & 1, whose barriers are then in
-        // their phase (t >> 1) & 1.
-        if (warp == LOAD_WARP) {
-            if (lane == 0 && DK_STALLED) failed[0] = 1;
-            if (lane == 0 && !DK_STALLED) {  // --------------------------------------------------- every TMA
-                auto load_kv = [&](const CUtensorMap* map, uint32_t stages, uint64_t* bar, int j) {
-                    const uint32_t b = (step + j) & 1;
-                    mbar_expect_tx(bar + b, KV_BYTES);
-                    int page = pt[p0 + j];
-                    if (page < 0 || page >= a.n_pages) page = 0;       // any page will do: its keys are masked
-                    const int row = (page * a.nkv + kvh) * DK_PAGE;
+    if (warp == LOAD_WARP) {
+        if (lane == 0 && !DK_STALLED) {  // --------------------------------------------------- every TMA
+            uint32_t t0 = 0, tile = 0;                     // pages and tiles before
+            bool ok = true;
+            auto load = [&](const CUtensorMap* map, uint32_t dst, uint64_t* bar, int j) {
+                mbar_expect_tx(bar, KV_BYTES);
+                int page = w.pt[w.p0 + j];
+                if (page < 0 || page >= a.n_pages) page = 0;           // any page will do: its keys are masked
+                const int row = (page * a.nkv + w.kvh) * DK_PAGE;
+                for (int hh = 0; hh < HALVES; hh++) tma_load_2d(dst + hh * KV_ATOM_BYTES, map, hh * 64, row, bar);
+            };
+            for (; ok && w.next(a); tile++) {
+                const int n = w.pages(), boxes = w.pair ? 2 : 1;
+                if (tile > 0 && !mbar_wait(q_free, (tile - 1) & 1)) { ok = false; break; }
+                mbar_expect_tx(q_full, boxes * HALVES * a.half_nodes * G * 128);
+                for (int x = 0; x < boxes; x++)
                     for (int hh = 0; hh < HALVES; hh++)
-                        tma_load_2d(stages + b * KV_BYTES + hh * KV_ATOM_BYTES, map, hh * 64, row, bar + b);
-                };
-                mbar_expect_tx(bar_q, HALVES * a.tile_nodes * G * 128);
-                for (int hh = 0; hh < HALVES; hh++) tma_load_3d(q_s + hh * Q_ATOM_BYTES, &map_q, hh * 64, kvh * G, flat0, bar_q);
-                load_kv(&map_k, k_s, bar_k, 0);
-                load_kv(&map_v, v_s, bar_v, 0);
-                if (n_blk > 1) load_kv(&map_k, k_s, bar_k, 1), load_kv(&map_v, v_s, bar_v, 1);
-                bool ok = true;
-                // in the order in which the stages come free: S(j) is done with K(j), then P.V(j-1) with V(j-1)
-                for (int j = 0; j + 2 < n_blk && ok; j++) {
-                    const uint32_t t = step + j;
-                    if (!mbar_wait(bar_s + (t & 1), (t >> 1) & 1)) { ok = false; break; }
-                    load_kv(&map_k, k_s, bar_k, j + 2);
-                    if (j >= 1) {
-                        if (!mbar_wait(bar_o + ((t - 1) & 1), ((t - 1) >> 1) & 1)) { ok = false; break; }
-                        load_kv(&map_v, v_s, bar_v, j + 1);
+                        tma_load_3d(q_s + x * Q_BYTES + hh * Q_ATOM_BYTES, &map_q, hh * 64, w.kvh * G, w.sq.flat0 + w.node0 + x * a.half_nodes, q_full);
+                for (int j = 0; j < n + 2 && ok; j++) {
+                    if (j < n) {
+                        const uint32_t t = t0 + j;
+                        if (t >= NK && !mbar_wait(k_free + slot_of<NK>(t), phase_of<NK>(t - NK))) { ok = false; break; }
+                        load(&map_k, k_s + slot_of<NK>(t) * KV_BYTES, k_full + slot_of<NK>(t), j);
+                    }
+                    if (j >= 2) {
+                        const uint32_t t = t0 + j - 2;
+                        if (t >= NV && !mbar_wait(v_free + slot_of<NV>(t), phase_of<NV>(t - NV))) { ok = false; break; }
+                        load(&map_v, v_s + slot_of<NV>(t) * KV_BYTES, v_full + slot_of<NV>(t), j - 2);
                     }
                 }
-                if (ok && n_blk > 2) {                                 // the last page's values: after P.V(n - 3)
-                    const uint32_t t = step + n_blk - 3;
-                    ok = mbar_wait(bar_o + (t & 1), (t >> 1) & 1);
-                    if (ok) load_kv(&map_v, v_s, bar_v, n_blk - 1);
-                }
-                if (!ok) atomicExch(err, 23), failed[0] = 1;
+                t0 += n;
             }
-        } else if (warp == MMA_WARP) {
-            if (lane == 0) {  // ------------------------------------------------------------ every tcgen05.mma
-                const uint64_t dq = desc_k_major(q_s), dk = desc_k_major(k_s), dv = desc_n_major(v_s);
-                auto issue_s = [&](int j) {
-                    const uint32_t b = (step + j) & 1;
-                    const uint64_t dkb = dk + (uint64_t)((b * KV_BYTES) >> 4);
+            if (!ok) atomicExch(err, 23);
+        }
+    } else if (warp >= MMA_WARP) {
+        if (lane == 0) {  // ------------------------------------------------------------ a stream's tcgen05.mma
+            // (One thread for both streams: a step of the two took 3,300 clocks, of which it was busy issuing for 2,100.)
+            const int x = warp - MMA_WARP;
+            const uint64_t dq = desc_k_major(q_s), dk = desc_k_major(k_s), dv = desc_n_major(v_s);
+            uint64_t *bar_s = s_full + 2 * x, *bar_p = p_full + 2 * x, *bar_o = o_full + 2 * x;
+            const uint32_t t_sx = t_s + 2 * x * BN, t_ox = t_o + x * 128;
+            uint32_t t0 = 0, tile = 0, done = 0;           // pages, tiles and steps before
+            bool ok = true;
+            for (; ok && w.next(a); tile++) {
+                const int n = w.steps(x);
+                // a page that both streams read is free when both say so; one that this stream alone reads it gives back for both
+                auto give_back = [&](uint64_t* bar) {
+                    umma_commit(bar);
+                    if (!w.pair) umma_commit(bar);
+                };
+                const uint64_t dqx = dq + (uint64_t)((w.pair ? x * Q_BYTES : 0) >> 4);
+                auto issue_s = [&](int i) {
+                    const uint32_t t = t0 + w.page_of(x, i), b = (done + i) & 1;
+                    if (!mbar_wait(k_full + slot_of<NK>(t), phase_of<NK>(t))) return false;
+                    fence_after();
+                    const uint64_t dkt = dk + (uint64_t)((slot_of<NK>(t) * KV_BYTES) >> 4);
 #pragma unroll
                     for (int hh = 0; hh < HALVES; hh++)
 #pragma unroll
                         for (int k = 0; k < 4; k++)
-                            umma_ss(t_s + b * BN, dq + (uint64_t)((hh * Q_ATOM_BYTES + k * 32) >> 4),
-                                    dkb + (uint64_t)((hh * KV_ATOM_BYTES + k * 32) >> 4), IDESC_S, (hh | k) != 0);
+                            umma_ss(t_sx + b * BN, dqx + (uint64_t)((hh * Q_ATOM_BYTES + k * 32) >> 4),
+                                    dkt + (uint64_t)((hh * KV_ATOM_BYTES + k * 32) >> 4), IDESC_S, (hh | k) != 0);
                     umma_commit(bar_s + b);
+                    give_back(k_free + slot_of<NK>(t));
+                    if (i + 1 == n) umma_commit(q_free);
+                    return true;
                 };
-                bool ok = mbar_wait(bar_q, tiles_done & 1);
-                for (int j = 0; j < 2 && j < n_blk && ok; j++) {
-                    const uint32_t t = step + j;
-                    ok = mbar_wait(bar_k + (t & 1), (t >> 1) & 1);
-                    if (ok) fence_after(), issue_s(j);
-                }
-                for (int i = 0; i < n_blk && ok; i++) {
-                    const uint32_t t = step + i, b = t & 1, ph = (t >> 1) & 1;
-                    if (!mbar_wait(bar_p + b, ph)) { ok = false; break; }
-                    if (!mbar_wait(bar_v + b, ph)) { ok = false; break; }
+                ok = mbar_wait(q_full, tile & 1);
+                if (ok && n == 0) umma_commit(q_free);     // one page only: nothing for B
+                if (ok && n > 0) ok = issue_s(0);
+                if (ok && n > 1) ok = issue_s(1);
+                // the rows of the tile before have been read out of O
+                if (ok && tile > 0) ok = mbar_wait(o_free, (tile - 1) & 1);
+                for (int i = 0; i < n && ok; i++) {
+                    const uint32_t t = t0 + w.page_of(x, i), step = done + i, b = step & 1;
+                    if (!mbar_wait(v_full + slot_of<NV>(t), phase_of<NV>(t))) { ok = false; break; }
+                    if (!mbar_wait(bar_p + b, (step >> 1) & 1)) { ok = false; break; }
                     fence_after();
+                    const uint64_t dvt = dv + (uint64_t)((slot_of<NV>(t) * KV_BYTES) >> 4);
 #pragma unroll
                     for (int k = 0; k < BN / 16; k++)
-                        umma_ts(t_o, t_s + b * BN + k * 8, dv + (uint64_t)((b * KV_BYTES + k * 16 * 128) >> 4), IDESC_PV, (i | k) != 0);
+                        umma_ts(t_ox, t_sx + b * BN + k * 8, dvt + (uint64_t)((k * 16 * 128) >> 4), IDESC_PV, (i | k) != 0);   // the first overwrites O
                     umma_commit(bar_o + b);
-                    if (i + 2 < n_blk) {       // into the buffer whose P was just used: products of one thread run in order
-                        const uint32_t t2 = t + 2;
-                        if (!mbar_wait(bar_k + (t2 & 1), (t2 >> 1) & 1)) { ok = false; break; }
-                        fence_after();
-                        issue_s(i + 2);
-                    }
+                    give_back(v_free + slot_of<NV>(t));
+                    // into the buffer whose P was just used: products of one thread run in order
+                    if (i + 2 < n) ok = issue_s(i + 2);
                 }
-                if (!ok) atomicExch(err, 21), failed[0] = 1;
+                t0 += w.pages(), done += n;
             }
-        } else {  // ------------------------------------------------------------------ softmax, a thread a row
-            const int r = threadIdx.x, node = flat0 + r / G, mark = tiles_done + 1;
+            if (!ok) atomicExch(err, 21);
+        }
+    } else {  // ------------------------------------------------------------------ softmax, a thread a row of a stream
+        const int x = warp >> 2, r = threadIdx.x & (BM - 1);
+        const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16, t_sx = t_s + lane_off + 2 * x * BN, t_ox = t_o + lane_off + x * 128;
+        uint64_t *bar_s = s_full + 2 * x, *bar_p = p_full + 2 * x, *bar_o = o_full + 2 * x;
+        uint32_t t0 = 0, tile = 0, done = 0, shared_tiles = 0;
+        bool ok = true;
+        for (; ok && w.next(a); tile++) {
+            const TreeSeq& sq = w.sq;
+            const int n = w.steps(x), first = w.node0 + (w.pair && x ? a.half_nodes : 0);
+            const int rows = min(w.node0 + w.nodes - first, a.half_nodes) * G, node = sq.flat0 + first + r / G, mark = (int)tile + 1;
             const int qpos = r < rows ? a.row_pos[node] : -1;
             const bool valid = qpos >= 0;
-            const uint32_t* words = a.tree + (size_t)(r < rows ? node : flat0) * a.words;
-            const bool any_row = warp * 32 < rows;                     // else the warp has no row of the tile
-            const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+            const uint32_t* words = a.tree + (size_t)(r < rows ? node : sq.flat0) * a.words;
+            const bool any_row = (warp & 3) * 32 < rows;               // else the warp has no row of the tile
             // pages that every row sees: the cached tokens' and, with a window, none that the last node's begins in
             const int open_lo = a.window > 0 ? max(0, sq.pos0 + sq.n - a.window) : 0;
             float m = -INFINITY, l = 0.f;
-            bool ok = true;
-            for (int i = 0; i < n_blk && ok; i++) {
-                const uint32_t t = step + i, b = t & 1, ph = (t >> 1) & 1;
-                const int key0 = (sq.first_page + p0 + i) * BN, page = pt[p0 + i];
+            for (int i = 0; i < n && ok; i++) {
+                const uint32_t step = done + i, b = step & 1, ph = (step >> 1) & 1;
+                const int j = w.p0 + w.page_of(x, i), key0 = (sq.first_page + j) * BN, page = w.pt[j];
                 const bool held = page >= 0 && page < a.n_pages;
                 const bool open = held && key0 + BN <= sq.pos0 && key0 >= open_lo;
                 uint64_t seen = ~0ull;
                 if (!open) {
+                    const uint32_t t = t0 + j - w.p0;
                     seen = held && valid ? tree_mask(a, sq, words, qpos, key0) : 0ull;
-                    if (!mbar_wait(bar_v + b, ph)) { ok = false; break; }
+                    if (!mbar_wait(v_full + slot_of<NV>(t), phase_of<NV>(t))) { ok = false; break; }
                     // 16 bytes each of the page's values at a time
-                    uint4* vs = reinterpret_cast<uint4*>(smem + Q_BYTES + 2 * KV_BYTES + b * KV_BYTES);
+                    uint4* vs = reinterpret_cast<uint4*>(smem + V_RING + slot_of<NV>(t) * KV_BYTES);
                     bool odd = false;
 #pragma unroll
-                    for (int k = 0; k < KV_BYTES / 16 / SOFT; k++) {
-                        uint4 x = vs[k * SOFT + r];
-                        uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+                    for (int k = 0; k < KV_BYTES / 16 / BM; k++) {
+                        uint4 val = vs[k * BM + r];
+                        uint32_t* e = reinterpret_cast<uint32_t*>(&val);
                         bool mine = false;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u, mine = true;
-                            if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0xffffu, mine = true;
+                        for (int q = 0; q < 4; q++) {
+                            if ((e[q] & 0x7f80u) == 0x7f80u) e[q] &= 0xffff0000u, mine = true;
+                            if ((e[q] & 0x7f800000u) == 0x7f800000u) e[q] &= 0xffffu, mine = true;
                         }
-                        if (mine) vs[k * SOFT + r] = x, odd = true;
+                        if (mine) {                                    // said before it is done: the other stream may look at the page too
+                            *odd_tile = mark;
+                            __threadfence_block();
+                            vs[k * BM + r] = val, odd = true;
+                        }
                     }
-                    if (odd) {
-                        failed[1] = mark;
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    }
+                    if (odd) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 if (!mbar_wait(bar_s + b, ph)) { ok = false; break; }
                 if (any_row) {
@@ -341,17 +407,17 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     fence_after();
                     uint32_t v[BN];
 #pragma unroll
-                    for (int c = 0; c < BN; c += 32) tmem_ld32(t_s + lane_off + b * BN + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
+                    for (int c = 0; c < BN; c += 32) tmem_ld32(t_sx + b * BN + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
                     tmem_wait_ld();
                     float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     if (!open) {
                         const uint32_t half[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
 #pragma unroll
-                        for (int j = 0; j < BN; j++)
-                            if (!(half[j / 32] >> (j % 32) & 1)) v[j] = 0xff800000u;           // -infinity
+                        for (int k = 0; k < BN; k++)
+                            if (!(half[k / 32] >> (k % 32) & 1)) v[k] = 0xff800000u;           // -infinity
                     }
 #pragma unroll
-                    for (int j = 0; j < BN; j += 2) mx4[(j >> 1) & 3] = max3(mx4[(j >> 1) & 3], __uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+                    for (int k = 0; k < BN; k += 2) mx4[(k >> 1) & 3] = max3(mx4[(k >> 1) & 3], __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
                     const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.sl2;   // sl2 > 0: scaling keeps the order
                     float m_new = fmaxf(m, mx);
                     // a maximum that moved by less than 8 (a factor 256) keeps the old reference: O need not be rescaled
@@ -359,28 +425,29 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     const float ms = m_new == -INFINITY ? 0.f : m_new;
                     const float alpha = m_new == m ? 1.f : ex2(m - ms);
                     if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-                        if (!mbar_wait(bar_o + (b ^ 1), ((t - 1) >> 1) & 1)) { ok = false; break; }
+                        if (!mbar_wait(bar_o + (b ^ 1), ((step - 1) >> 1) & 1)) { ok = false; break; }
+                        __syncwarp();
                         fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < HD; c += OC) {
-                            uint32_t o[OC];
-                            tmem_ld32(t_o + lane_off + c, o);
+                        for (int c = 0; c < HD; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(t_ox + c, o);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int j = 0; j < OC; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-                            tmem_st32(t_o + lane_off + c, o);
+                            for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                            tmem_st32(t_ox + c, o);
                         }
                     }
                     float sum4[4] = {0.f, 0.f, 0.f, 0.f};
                     uint32_t p[BN / 2];
 #pragma unroll
-                    for (int j = 0; j < BN; j += 2) {
-                        const float e0 = ex2(fmaf(__uint_as_float(v[j]), a.sl2, -ms)), e1 = ex2(fmaf(__uint_as_float(v[j + 1]), a.sl2, -ms));
-                        sum4[(j >> 1) & 3] += e0 + e1;
+                    for (int k = 0; k < BN; k += 2) {
+                        const float e0 = ex2(fmaf(__uint_as_float(v[k]), a.sl2, -ms)), e1 = ex2(fmaf(__uint_as_float(v[k + 1]), a.sl2, -ms));
+                        sum4[(k >> 1) & 3] += e0 + e1;
                         __nv_bfloat162 pk = __floats2bfloat162_rn(e0, e1);
-                        p[j / 2] = *reinterpret_cast<uint32_t*>(&pk);
+                        p[k / 2] = *reinterpret_cast<uint32_t*>(&pk);
                     }
-                    tmem_st32(t_s + lane_off + b * BN, p);
+                    tmem_st32(t_sx + b * BN, p);
                     l = l * alpha + (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
                     m = m_new;
                     tmem_wait_st();
@@ -388,64 +455,87 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 }
                 mbar_arrive(bar_p + b);
             }
-            if (ok) ok = mbar_wait(bar_o + ((step + n_blk - 1) & 1), ((step + n_blk - 1) >> 1) & 1);
-            if (ok && any_row) {
+            if (ok && n > 0) ok = mbar_wait(bar_o + ((done + n - 1) & 1), ((done + n - 1) >> 1) & 1);
+            if (!ok) break;
+            if (!valid) m = -INFINITY, l = 0.f;
+            // the factors of the two streams' rows: with rows in both, the own one alone
+            float mine = 1.f, other = 0.f;
+            int c0 = 0, c1 = HD;
+            if (!w.pair) {
+                float2* ml = ml_s + (shared_tiles & 1) * 2 * BM;
+                ml[x * BM + r] = make_float2(m, l);
+                mbar_arrive(both);
+                if (!mbar_wait(both, shared_tiles & 1)) { ok = false; break; }
+                shared_tiles++;
+                const float2 o = ml[(1 - x) * BM + r];
+                const float mn = fmaxf(m, o.x), ms = mn == -INFINITY ? 0.f : mn;
+                mine = ex2(m - ms), other = ex2(o.x - ms);
+                l = l * mine + o.y * other, m = mn;
+                c0 = x * (HD / 2), c1 = c0 + HD / 2;                   // each stream's thread writes half the row
+            }
+            if (any_row) {
+                __syncwarp();
                 fence_after();
-                const bool whole = n_blk == sq.pages, mend = failed[1] == mark;
-                if (!valid) m = -INFINITY, l = 0.f;
+                const bool whole = w.pages() == sq.pages, mend = *odd_tile == mark, has = n > 0, has_other = !w.pair && w.steps(1 - x) > 0;
                 const float inv = l == 0.f ? 0.f : 1.f / l;
-                const size_t slot = (size_t)(2 * blockIdx.x + (p0 == 0 ? 1 : 0)) * BM + r;
-                bf16* dst = out + (size_t)(flat0 + r / G) * ldo + (size_t)(kvh * G + r % G) * HD;
-                if (!whole && r < rows) ws_ml[slot] = make_float2(m, l);
+                const size_t slot = (size_t)(2 * blockIdx.x + (w.p0 == 0 ? 1 : 0)) * 2 * BM;
+                const int row = (w.pair ? x * BM : 0) + r;
+                bf16* dst = out + (size_t)node * ldo + (size_t)(w.kvh * G + r % G) * HD;
+                if (!whole && r < rows && c0 == 0) ws_ml[slot + row] = make_float2(m, l);
 #pragma unroll 1
-                for (int c = 0; c < HD; c += OC) {
-                    uint32_t o[OC];
+                for (int c = c0; c < c1; c += OC) {
+                    uint32_t o[OC], o2[OC];
                     __syncwarp();
-                    tmem_ld32(t_o + lane_off + c, o);
+                    if (has) tmem_ld16(t_ox + c, o);
+                    if (has_other) tmem_ld16(t_o + lane_off + (1 - x) * 128 + c, o2);
                     tmem_wait_ld();
-                    if (r >= rows) continue;
-                    if (!valid || l == 0.f) {
 #pragma unroll
-                        for (int j = 0; j < OC; j++) o[j] = 0;
-                    } else if (mend) {         // values that are not finite, for the rows that see them
-                        for (int i = 0; i < n_blk; i++) {
-                            const int key0 = (sq.first_page + p0 + i) * BN, page = pt[p0 + i];
-                            if (page < 0 || page >= a.n_pages || (key0 + BN <= sq.pos0 && key0 >= open_lo)) continue;
-                            for (uint64_t left = tree_mask(a, sq, words, qpos, key0); left; left &= left - 1) {
-                                const bf16* val = v_store + kv_offset(page, a.nkv, kvh, __ffsll((long long)left) - 1, HD) + c;
+                    for (int k = 0; k < OC; k++)
+                        o[k] = __float_as_uint((has ? __uint_as_float(o[k]) * mine : 0.f) + (has_other ? __uint_as_float(o2[k]) * other : 0.f));
+                    if (r < rows) {
+                        if (!valid || l == 0.f) {
 #pragma unroll
-                                for (int j = 0; j < OC; j++) {
-                                    const float x = __bfloat162float(val[j]);
-                                    if (!isfinite(x)) o[j] = __float_as_uint(__uint_as_float(o[j]) + x);
+                            for (int k = 0; k < OC; k++) o[k] = 0;
+                        } else if (mend) {     // values that are not finite, for the rows that see them
+                            for (int j = w.p0; j < w.p1; j++) {
+                                const int key0 = (sq.first_page + j) * BN, page = w.pt[j];
+                                if (page < 0 || page >= a.n_pages || (key0 + BN <= sq.pos0 && key0 >= open_lo)) continue;
+                                for (uint64_t left = tree_mask(a, sq, words, qpos, key0); left; left &= left - 1) {
+                                    const bf16* val = v_store + kv_offset(page, a.nkv, w.kvh, __ffsll((long long)left) - 1, HD) + c;
+#pragma unroll
+                                    for (int k = 0; k < OC; k++) {
+                                        const float y = __bfloat162float(val[k]);
+                                        if (!isfinite(y)) o[k] = __float_as_uint(__uint_as_float(o[k]) + y);
+                                    }
                                 }
                             }
                         }
-                    }
-                    if (whole) {
+                        if (whole) {
 #pragma unroll
-                        for (int j = 0; j < OC; j += 8) {
-                            uint4 pk;
-                            __nv_bfloat162* pp = reinterpret_cast<__nv_bfloat162*>(&pk);
+                            for (int k = 0; k < OC; k += 8) {
+                                uint4 pk;
+                                __nv_bfloat162* pp = reinterpret_cast<__nv_bfloat162*>(&pk);
 #pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                pp[e] = __floats2bfloat162_rn(__uint_as_float(o[j + 2 * e]) * inv, __uint_as_float(o[j + 2 * e + 1]) * inv);
-                            *reinterpret_cast<uint4*>(dst + c + j) = pk;
+                                for (int e = 0; e < 4; e++)
+                                    pp[e] = __floats2bfloat162_rn(__uint_as_float(o[k + 2 * e]) * inv, __uint_as_float(o[k + 2 * e + 1]) * inv);
+                                *reinterpret_cast<uint4*>(dst + c + k) = pk;
+                            }
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < OC; k += 4)
+                                *reinterpret_cast<uint4*>(ws_acc + slot * HD + part_at(2 * BM, row, c + k)) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
                         }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < OC; j += 4) *reinterpret_cast<uint4*>(ws_acc + slot * HD + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
                     }
                 }
-            } else if (!ok && lane == 0) {
-                atomicExch(err, 22), failed[0] = 1;
+                fence_before();
             }
+            mbar_arrive(o_free);
+            t0 += w.pages(), done += n;
         }
-        // everyone is done with the tile: O has been read out of tensor memory
-        step += n_blk, tiles_done++, u += n_blk;
-        fence_before();
-        __syncthreads();
-        fence_after();
+        if (!ok && lane == 0) atomicExch(err, 22);
     }
+    fence_before();
+    __syncthreads();
     if (warp == MMA_WARP) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_ALLOC) : "memory");
@@ -481,11 +571,10 @@ int make_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dim
 
 }  // namespace
 
-DK_EXPORT int dk_tree_tc_tile_rows() { return BM; }
-DK_EXPORT int dk_tree_tc_blocks_per_sm() { return BLOCKS_PER_SM; }
+DK_EXPORT int dk_tree_tc_tile_rows() { return 2 * BM; }
 
 // q [n_rows, nh*HD] and out, bf16, rows ldq / ldo elements apart (multiples of 8, 16-byte boundaries); k_store, v_store [n_pages, nkv, 64,
-// HD]; ws_acc: 2 * blocks * 128 * HD floats, ws_ml: 2 * blocks * 128 * 2 floats; err: device int for a wait that ran out.
+// HD]; ws_acc: 2 * blocks * 256 * HD floats, ws_ml: 2 * blocks * 256 * 2 floats; err: device int for a wait that ran out.
 DK_EXPORT int dk_attn_tree_tc(const void* q, long long ldq, void* out, long long ldo, long long n_rows, const void* k_store,
                               const void* v_store, int n_pages, const int* cu_q, const int* seq_pos0, const int* row_pos,
                               const uint32_t* tree, int words, const int* page_table, int pt_stride, int n_seq, int nh, int nkv, int window,
@@ -494,8 +583,9 @@ DK_EXPORT int dk_attn_tree_tc(const void* q, long long ldq, void* out, long long
         err == nullptr || ldq % 8 || ldo % 8 || ((uintptr_t)q | (uintptr_t)out) % 16 || (long long)n_pages * nkv * DK_PAGE > 0x7fffffffLL)
         return (int)cudaErrorInvalidValue;
     const int G = nh / nkv;
-    TreeArgs a = {cu_q, seq_pos0, row_pos, page_table, tree, n_seq, words, pt_stride, n_pages, nh, nkv, window, BM / G,
+    TreeArgs a = {cu_q, seq_pos0, row_pos, page_table, tree, n_seq, words, pt_stride, n_pages, nh, nkv, window, 2 * (BM / G), BM / G, BM,
                   scale * 1.4426950408889634f};
+    if (!tree_units_fit(a, max_nodes) || nkv > 65535) return (int)cudaErrorInvalidValue;
     cudaError_t ce = cudaFuncSetAttribute(tree_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
     if (ce != cudaSuccess) {
         cudaGetLastError();
@@ -513,6 +603,5 @@ DK_EXPORT int dk_attn_tree_tc(const void* q, long long ldq, void* out, long long
     e = dk_launch(tree_tc_kernel, dim3(blocks), dim3(THREADS), SMEM_BYTES, st, mq, mk, mv, a, (bf16*)out, ldo, (const bf16*)v_store, ws_acc,
                   (float2*)ws_ml, err);
     if (e) return e;
-    return dk_launch(tree_merge_kernel<bf16, HD>, dim3((unsigned)(((long long)max_nodes * nh + 7) / 8), n_seq), dim3(256), 0, st, a,
-                     (const float*)ws_acc, (const float2*)ws_ml, (bf16*)out, ldo, BM, blocks);
+    return tree_merge<bf16, HD>(a, ws_acc, ws_ml, out, ldo, 2 * BM, max_nodes, blocks, st);
 }
