@@ -35,24 +35,12 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
     pdl_wait();
     pdl_launch_dependents();
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, G = a.nh / a.nkv;
-    int before;
-    const int total = tree_units(a, 0, before);
-    const int nb = share_count(total, gridDim.x);
-    if ((int)blockIdx.x >= nb) return;
-    int u = share_begin(total, blockIdx.x, nb);
-    const int u_end = share_begin(total, blockIdx.x + 1, nb);
-    int s = tree_find(a, u, before);
-    TreeSeq sq;
-    sq.load(a, s);
-    while (u < u_end) {
-        while (u >= before + sq.units(a.nkv)) {
-            before += sq.units(a.nkv);
-            sq.load(a, ++s);
-        }
-        const int at = u - before, item = at / sq.pages, p0 = at % sq.pages, p1 = min(sq.pages, p0 + (u_end - u));
-        const int kvh = item / sq.tiles, node0 = (item % sq.tiles) * a.tile_nodes;
-        const int rows = min(a.tile_nodes, sq.n - node0) * G, flat0 = sq.flat0 + node0;
-        const int* pt = a.page_table + (size_t)s * a.pt_stride;
+    TreeWalk w;
+    w.begin(a);
+    const TreeSeq& sq = w.sq;
+    while (w.next(a)) {
+        const int p0 = w.p0, p1 = w.p1, kvh = w.kvh, rows = w.nodes * G, flat0 = sq.flat0 + w.node0;
+        const int* pt = w.pt;
         for (int i = threadIdx.x; i < TM * (HD / 4); i += THREADS) {
             const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
             if (r < rows) load4(q_s + r * HD + c, q + (size_t)(flat0 + r / G) * ldq + (kvh * G + r % G) * HD + c);
@@ -67,7 +55,7 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
         }
         for (int p = p0; p < p1; p++) {
             const int key0 = (sq.first_page + p) * DK_PAGE;
-            int page = pt[sq.first_page + p];
+            int page = pt[p];
             const bool held = page >= 0 && page < a.n_pages;           // a page that is none holds no keys
             if (!held) page = 0;
             const size_t off = kv_offset(page, a.nkv, kvh, 0, HD);
@@ -122,9 +110,9 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
                 float sum = 0.f;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const float w = exp2f(fmaf(sc[i][j], a.sl2, -ms));
-                    sum += w;
-                    p_s[(ty + 16 * i) * LDP + tx + 16 * j] = w;
+                    const float pw = exp2f(fmaf(sc[i][j], a.sl2, -ms));
+                    sum += pw;
+                    p_s[(ty + 16 * i) * LDP + tx + 16 * j] = pw;
                 }
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -136,14 +124,14 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
             if (!odd) {
 #pragma unroll 4
                 for (int k = 0; k < DK_PAGE; k++) {
-                    float w[NI];
+                    float pw[NI];
 #pragma unroll
-                    for (int i = 0; i < NI; i++) w[i] = p_s[(ty + 16 * i) * LDP + k];
+                    for (int i = 0; i < NI; i++) pw[i] = p_s[(ty + 16 * i) * LDP + k];
 #pragma unroll
                     for (int c = 0; c < CV; c++) {
                         const float v = v_s[k * HD + tx + 16 * c];
 #pragma unroll
-                        for (int i = 0; i < NI; i++) acc[i][c] = fmaf(w[i], v, acc[i][c]);
+                        for (int i = 0; i < NI; i++) acc[i][c] = fmaf(pw[i], v, acc[i][c]);
                     }
                 }
             } else {
@@ -151,15 +139,15 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
 #pragma unroll
                     for (int i = 0; i < NI; i++)
                         if (mask_s[ty + 16 * i] >> k & 1) {
-                            const float w = p_s[(ty + 16 * i) * LDP + k];
+                            const float pw = p_s[(ty + 16 * i) * LDP + k];
 #pragma unroll
-                            for (int c = 0; c < CV; c++) acc[i][c] = fmaf(w, v_s[k * HD + tx + 16 * c], acc[i][c]);
+                            for (int c = 0; c < CV; c++) acc[i][c] = fmaf(pw, v_s[k * HD + tx + 16 * c], acc[i][c]);
                         }
             }
             __syncthreads();
         }
-        const bool whole = p0 == 0 && p1 == sq.pages;
-        const size_t slot = (size_t)(2 * blockIdx.x + (p0 == 0 ? 1 : 0)) * TM;
+        const bool whole = w.all();
+        const size_t slot = (size_t)w.slot() * TM;
 #pragma unroll
         for (int i = 0; i < NI; i++) {
             const int r = ty + 16 * i;
@@ -175,7 +163,6 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
                 for (int c = 0; c < CV; c++) ws_acc[slot * HD + part_at(TM, r, tx + 16 * c)] = acc[i][c];
             }
         }
-        u += p1 - p0;
     }
 }
 
@@ -231,7 +218,7 @@ DK_EXPORT int dk_attn_tree(int f32, const void* q, long long ldq, void* out, lon
         return (int)cudaErrorInvalidValue;
     const int G = nh / nkv, rows = dk_tree_tile_rows(max_nodes, G);
     TreeArgs a = {cu_q, seq_pos0, row_pos, page_table, tree, n_seq, words, pt_stride, n_pages, nh, nkv, window, rows / G, rows / G, rows,
-                  scale * 1.4426950408889634f};
+                  pt_stride <= 1, 0, scale * 1.4426950408889634f};
     if (!tree_units_fit(a, max_nodes) || nkv > 65535) return (int)cudaErrorInvalidValue;
 #define DK_TREE(T, NI) launch<T, NI>(a, q, ldq, out, ldo, k_store, v_store, ws_acc, ws_ml, max_nodes, blocks, st)
     if (f32) return rows == 16 ? DK_TREE(float, 1) : rows == 32 ? DK_TREE(float, 2) : DK_TREE(float, 4);

@@ -8,14 +8,16 @@
 // head (laid out as halves of half_nodes nodes, each half_rows rows apart in a slot). The units of all sequences stand in one run (sequence, kv head, tile, page), and block b of nb takes the b-th of nb equal
 // shares, so lengths that differ leave no block idle, and the lengths may change under a captured graph: only device arrays say them.
 // A block that holds all pages of a tile writes the tile's rows; else it leaves a part (maximum, sum, sum of P.V) in one of its two
-// slots: 2 b + 1 for the tile its share begins (and does not end), 2 b for one that began in an earlier block.
+// slots: 2 b + 1 for the tile whose first page it has, 2 b for one that began in an earlier block. Taking up a tile and writing its
+// rows costs a block as much as some pages do: `extra` units that stand before a tile's pages and ask for no work.
+// With tables of a few pages (`whole`) a tile is one unit: there are no parts and there is no merge.
 #pragma once
 #include "common.cuh"
 
 struct TreeArgs {
     const int *cu_q, *seq_pos0, *row_pos, *page_table;
     const uint32_t* tree;                  // [rows, words]
-    int n_seq, words, pt_stride, n_pages, nh, nkv, window, tile_nodes, half_nodes, half_rows;
+    int n_seq, words, pt_stride, n_pages, nh, nkv, window, tile_nodes, half_nodes, half_rows, whole, extra;
     float sl2;                             // scale * log2(e)
 };
 
@@ -32,7 +34,8 @@ struct TreeSeq {
         first_page = min((a.window > 0 ? max(0, pos0 - a.window + 1) : 0) / DK_PAGE, a.pt_stride - 1);
         pages = max(1, end - first_page);
     }
-    __device__ __forceinline__ int units(int nkv) const { return tiles * nkv * pages; }
+    __device__ __forceinline__ int length(const TreeArgs& a) const { return a.whole ? 1 : pages + a.extra; }      // units of a tile
+    __device__ __forceinline__ int units(const TreeArgs& a) const { return tiles * a.nkv * length(a); }
 };
 
 __device__ __forceinline__ int warp_scan(int v) {          // inclusive
@@ -45,53 +48,107 @@ __device__ __forceinline__ int warp_scan(int v) {          // inclusive
     return v;
 }
 
-// Units of all sequences (the launch has seen to it that they stay below 2^31), and of those before sequence `upto`. A whole warp
-// calls it.
-__device__ __forceinline__ int tree_units(const TreeArgs& a, int upto, int& before) {
-    int sum = 0, first = 0;
-    for (int s = threadIdx.x & 31; s < a.n_seq; s += 32) {
+// The run of units as a warp sees it: the total, and sequence by sequence where it begins. Up to 32 sequences are read once and kept,
+// one a lane; more are read again where they are asked for. A whole warp calls all of this.
+struct TreeRun {
+    TreeSeq mine;                          // of sequence `lane`
+    int upto, total;                       // units of the sequences up to and including `lane`'s; of all
+    __device__ __forceinline__ int load(const TreeArgs& a, int s0) {
+        const int s = s0 + (threadIdx.x & 31);
+        if (s < a.n_seq) mine.load(a, s);
+        else mine.tiles = 0, mine.pages = 0;
+        upto = warp_scan(mine.units(a));
+        return __shfl_sync(0xffffffffu, upto, 31);
+    }
+    __device__ __forceinline__ void read(const TreeArgs& a) {
+        total = 0;
+        for (int s0 = 0; s0 < a.n_seq; s0 += 32) total += load(a, s0);
+    }
+    __device__ __forceinline__ TreeSeq seq_of_lane(int l) const {
         TreeSeq q;
-        q.load(a, s);
-        sum += q.units(a.nkv);
-        if (s < upto) first += q.units(a.nkv);
+        q.n = __shfl_sync(0xffffffffu, mine.n, l), q.pos0 = __shfl_sync(0xffffffffu, mine.pos0, l);
+        q.first_page = __shfl_sync(0xffffffffu, mine.first_page, l), q.pages = __shfl_sync(0xffffffffu, mine.pages, l);
+        q.tiles = __shfl_sync(0xffffffffu, mine.tiles, l), q.flat0 = __shfl_sync(0xffffffffu, mine.flat0, l);
+        return q;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        first += __shfl_xor_sync(0xffffffffu, first, o);
-    }
-    before = first;
-    return sum;
-}
-
-// The sequence that unit u (below the total) belongs to, and the units before it. A whole warp calls it.
-__device__ __forceinline__ int tree_find(const TreeArgs& a, int u, int& before) {
-    const int lane = threadIdx.x & 31;
-    before = 0;
-    for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
-        int mine = 0;
-        if (s0 + lane < a.n_seq) {
-            TreeSeq q;
-            q.load(a, s0 + lane);
-            mine = q.units(a.nkv);
+    // The sequence that unit u (below the total) belongs to, and the units before it.
+    __device__ __forceinline__ TreeSeq find(const TreeArgs& a, int u, int& s, int& before) {
+        before = 0;
+        for (int s0 = 0;; s0 += 32) {
+            const int here = a.n_seq <= 32 ? total : load(a, s0);
+            if (before + here > u || s0 + 32 >= a.n_seq) {
+                const int l = __ffs(__ballot_sync(0xffffffffu, before + upto > u)) - 1;
+                before += __shfl_sync(0xffffffffu, upto - mine.units(a), l);
+                s = s0 + l;
+                return seq_of_lane(l);
+            }
+            before += here;
         }
-        const int upto = warp_scan(mine);
-        const unsigned past = __ballot_sync(0xffffffffu, before + upto > u);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            before += __shfl_sync(0xffffffffu, upto - mine, l);
-            return s0 + l;
-        }
-        before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    return a.n_seq;
-}
+    // Sequence s, and the units before it.
+    __device__ __forceinline__ TreeSeq at(const TreeArgs& a, int s, int& before) {
+        before = 0;
+        if (a.n_seq > 32)
+            for (int s0 = 0; s0 <= s; s0 += 32) {
+                const int here = load(a, s0);
+                if (s0 + 32 <= s) before += here;
+            }
+        before += __shfl_sync(0xffffffffu, upto - mine.units(a), s & 31);
+        return seq_of_lane(s & 31);
+    }
+};
 
 // Shares of a launch of `blocks`.
 __device__ __forceinline__ int share_count(int total, int blocks) { return min(total, blocks); }
 // Block b's share begins at this unit; the share that unit u lies in.
-__device__ __forceinline__ int share_begin(int total, int b, int nb) { return (int)((long long)total * b / nb); }
-__device__ __forceinline__ int share_of(int total, int u, int nb) { return (int)(((long long)(u + 1) * nb - 1) / total); }
+__device__ __forceinline__ int scaled(int x, int y, int by) {             // x * y / by; a 64-bit division only where it has to be
+    const unsigned long long xy = (unsigned long long)x * (unsigned)y;
+    return xy >> 32 ? (int)(xy / (unsigned)by) : (int)((unsigned)xy / (unsigned)by);
+}
+__device__ __forceinline__ int share_begin(int total, int b, int nb) { return scaled(total, b, nb); }
+__device__ __forceinline__ int share_of(int total, int u, int nb) {
+    const unsigned long long x = (unsigned long long)(u + 1) * (unsigned)nb - 1;
+    return x >> 32 ? (int)(x / (unsigned)total) : (int)((unsigned)x / (unsigned)total);
+}
+
+// Where a block stands in its share; every role walks it for itself. A whole warp calls begin().
+struct TreeWalk {
+    TreeSeq sq;
+    int u, u_end, before, s;
+    // the tile at hand: its kv head, first node, nodes, pages [p0, p1) of the sequence's
+    int kvh, node0, nodes, p0, p1;
+    const int* pt;
+    __device__ __forceinline__ void begin(const TreeArgs& a) {
+        u = u_end = 0;
+        TreeRun run;
+        run.read(a);
+        const int nb = share_count(run.total, gridDim.x);
+        if ((int)blockIdx.x < nb) {
+            u = share_begin(run.total, blockIdx.x, nb), u_end = share_begin(run.total, blockIdx.x + 1, nb);
+            sq = run.find(a, u, s, before);
+        }
+    }
+    __device__ __forceinline__ bool next(const TreeArgs& a) {
+        for (;;) {
+            if (u >= u_end) return false;
+            while (u >= before + sq.units(a)) {
+                before += sq.units(a);
+                sq.load(a, ++s);
+            }
+            const int len = sq.length(a), at = u - before, item = at / len, v0 = at % len, v1 = min(len, v0 + u_end - u);
+            u += v1 - v0;
+            p0 = a.whole ? 0 : max(0, v0 - a.extra), p1 = a.whole ? sq.pages : max(0, v1 - a.extra);
+            if (p0 >= p1) continue;
+            kvh = item / sq.tiles, node0 = (item % sq.tiles) * a.tile_nodes;
+            nodes = min(a.tile_nodes, sq.n - node0);
+            pt = a.page_table + (size_t)s * a.pt_stride + sq.first_page;
+            return true;
+        }
+    }
+    __device__ __forceinline__ int pages() const { return p1 - p0; }
+    __device__ __forceinline__ bool all() const { return p1 - p0 == sq.pages; }       // the tile's rows are complete here
+    __device__ __forceinline__ int slot() const { return 2 * blockIdx.x + (p0 == 0 ? 1 : 0); }
+};
 
 // Where column d of row `row` of a slot lies among its tile_rows * D numbers: four columns of a row side by side, then the next row's,
 // so that threads with a row each write and read whole lines.
@@ -135,48 +192,56 @@ tree_merge_kernel(TreeArgs a, const float* ws_acc, const float2* ws_ml, T* out, 
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, s = blockIdx.z, kvh = blockIdx.y, G = a.nh / a.nkv;
     const int groups = (tile_rows + 31) / 32, tile = blockIdx.x / groups, row = blockIdx.x % groups * 32 + lane;
-    TreeSeq q;
-    q.load(a, s);
-    if (tile >= q.tiles) return;
+    TreeRun run;
+    run.read(a);
     int u0;
-    const int total = tree_units(a, s, u0), nb = share_count(total, blocks);
-    u0 += (kvh * q.tiles + tile) * q.pages;
-    const int b0 = share_of(total, u0, nb), b1 = share_of(total, u0 + q.pages - 1, nb);
-    if (b0 == b1) return;
+    const TreeSeq q = run.at(a, s, u0);
+    const int total = run.total, nb = share_count(total, blocks);
     // the node of a row; -1: a row that is none, which has no parts
     auto node_of = [&](int r) {
         const int half = r / a.half_rows * a.half_nodes, in = r % a.half_rows, node = tile * a.tile_nodes + half + in / G;
         return in < a.half_nodes * G && half < a.tile_nodes && node < q.n ? node : -1;
     };
     const bool mine = node_of(row) >= 0;
+    if (tile >= q.tiles || !__any_sync(0xffffffffu, mine)) return;     // the same for all warps
+    u0 += (kvh * q.tiles + tile) * q.length(a);
+    const int b0 = share_of(total, u0 + a.extra, nb), b1 = share_of(total, u0 + q.length(a) - 1, nb);
+    if (b0 == b1) return;
     auto slot = [&](int b) { return (size_t)(2 * b + (b == b0 ? 1 : 0)) * tile_rows; };
     float m = -INFINITY, l = 0.f, acc[C][4] = {};
+    constexpr int AT_ONCE = C <= 4 ? 4 : 2;                            // parts that are asked for together
     if (mine)
-        for (int b = b0; b <= b1; b += 2) {                            // two parts at a time
-            const bool two = b < b1;
-            const float2 none = make_float2(-INFINITY, 0.f), p = ws_ml[slot(b) + row], p2 = two ? ws_ml[slot(b + 1) + row] : none;
-            float4 v[2][C];
+        for (int b = b0; b <= b1; b += AT_ONCE) {
+            float2 p[AT_ONCE];
+            float4 v[AT_ONCE][C];
 #pragma unroll
-            for (int c = 0; c < C; c++) {
-                const int d = (c * WARPS + w) * 4;
-                if (d < D) {
-                    v[0][c] = *reinterpret_cast<const float4*>(ws_acc + slot(b) * D + part_at(tile_rows, row, d));
-                    if (two) v[1][c] = *reinterpret_cast<const float4*>(ws_acc + slot(b + 1) * D + part_at(tile_rows, row, d));
+            for (int k = 0; k < AT_ONCE; k++) {
+                p[k] = b + k <= b1 ? ws_ml[slot(b + k) + row] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    const int d = (c * WARPS + w) * 4;
+                    v[k][c] = d < D && b + k <= b1 ? *reinterpret_cast<const float4*>(ws_acc + slot(b + k) * D + part_at(tile_rows, row, d))
+                                                   : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
             }
-            const float mn = fmaxf(m, fmaxf(p.x, p2.x)), ms = mn == -INFINITY ? 0.f : mn;
-            const float old = exp2f(m - ms), f = exp2f(p.x - ms), f2 = exp2f(p2.x - ms);
-            l = l * old + p.y * f + p2.y * f2;
-            m = mn;
+            float mn = m;
 #pragma unroll
-            for (int c = 0; c < C; c++) {
-                const float* x = reinterpret_cast<const float*>(&v[0][c]);
-                const float* x2 = reinterpret_cast<const float*>(&v[1][c]);
+            for (int k = 0; k < AT_ONCE; k++) mn = fmaxf(mn, p[k].x);
+            const float ms = mn == -INFINITY ? 0.f : mn, old = exp2f(m - ms);
+            l *= old, m = mn;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    acc[c][e] = acc[c][e] * old + x[e] * f;
-                    if (two) acc[c][e] += x2[e] * f2;
-                }
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[c][e] *= old;
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; k++) {
+                if (b + k > b1) break;
+                const float f = exp2f(p[k].x - ms);
+                l = fmaf(p[k].y, f, l);
+#pragma unroll
+                for (int c = 0; c < C; c++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[c][e] = fmaf(reinterpret_cast<const float*>(&v[k][c])[e], f, acc[c][e]);
             }
         }
     const float inv = l == 0.f ? 0.f : 1.f / l;                        // no key at all: a row of zeros
@@ -202,6 +267,7 @@ tree_merge_kernel(TreeArgs a, const float* ws_acc, const float2* ws_ml, T* out, 
 template <typename T, int D>
 static int tree_merge(const TreeArgs& a, const float* ws_acc, const float* ws_ml, void* out, long long ldo, int tile_rows, int max_nodes,
                       int blocks, cudaStream_t st) {
+    if (a.whole) return 0;
     const int tiles = (max_nodes + a.tile_nodes - 1) / a.tile_nodes;
     return dk_launch_as(true, tree_merge_kernel<T, D>, dim3((tile_rows + 31) / 32 * tiles, a.nkv, a.n_seq), dim3(256), 0, st, a, ws_acc,
                         (const float2*)ws_ml, (T*)out, ldo, tile_rows, blocks);
@@ -209,5 +275,5 @@ static int tree_merge(const TreeArgs& a, const float* ws_acc, const float* ws_ml
 
 // Whether the largest launch of these sizes has fewer than 2^31 units.
 static inline bool tree_units_fit(const TreeArgs& a, int max_nodes) {
-    return (double)a.n_seq * ((max_nodes + a.tile_nodes - 1) / a.tile_nodes) * a.nkv * a.pt_stride < 2147483647.0;
+    return (double)a.n_seq * ((max_nodes + a.tile_nodes - 1) / a.tile_nodes) * a.nkv * (a.pt_stride + a.extra) < 2147483647.0;
 }

@@ -41,9 +41,11 @@ constexpr int OC = 16;                            // columns of a row's result a
 constexpr int HALVES = HD / 64;                   // 64-column swizzle atoms across the head
 constexpr int Q_BYTES = BM * HD * 2, KV_BYTES = BN * HD * 2;
 constexpr int Q_ATOM_BYTES = BM * 128, KV_ATOM_BYTES = BN * 128;
+constexpr int WHOLE_PAGES = 8;                    // tables up to here are not split (see attention_tree.cuh)
+constexpr int EXTRA = 5;                          // pages that a tile's beginning and end take as long as
 constexpr int NK = HD == 128 ? 5 : 9, NV = HD == 128 ? 4 : 8;          // pages in the rings
 constexpr int RING = 2 * Q_BYTES, V_RING = RING + NK * KV_BYTES, BARS = V_RING + NV * KV_BYTES;
-constexpr int N_BARS = 2 * NK + 2 * NV + 12 + 4;
+constexpr int N_BARS = 2 * NK + 2 * NV + 16 + 5;
 constexpr int ML = BARS + (N_BARS + 4) * 8;       // [2][2][BM] pairs (maximum, sum) that the streams exchange
 constexpr size_t SMEM_BYTES = 1024 + ML + 4 * BM * 8;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of a block");
@@ -175,34 +177,30 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+// two numbers at a time: a * b + c, a + b
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; fma.rn.f32x2 x, x, y, z; mov.b64 {%0, %1}, x; }"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// Where a block stands in its share; every role walks it for itself.
-struct Walk {
-    TreeSeq sq;
-    int u, u_end, before, s;
-    // the tile at hand: its kv head, first node, nodes, pages [p0, p1) of the sequence's
-    int kvh, node0, nodes, p0, p1;
+struct Walk : TreeWalk {
     bool pair;                                             // two streams of rows; else two streams of pages
-    const int* pt;
     __device__ __forceinline__ bool next(const TreeArgs& a) {
-        if (u >= u_end) return false;
-        while (u >= before + sq.units(a.nkv)) {
-            before += sq.units(a.nkv);
-            sq.load(a, ++s);
-        }
-        const int at = u - before, item = at / sq.pages;
-        p0 = at % sq.pages, p1 = min(sq.pages, p0 + (u_end - u));
-        kvh = item / sq.tiles, node0 = (item % sq.tiles) * a.tile_nodes;
-        nodes = min(a.tile_nodes, sq.n - node0);
+        if (!TreeWalk::next(a)) return false;
         pair = nodes > a.half_nodes;
-        pt = a.page_table + (size_t)s * a.pt_stride + sq.first_page;
-        u += p1 - p0;
         return true;
     }
-    __device__ __forceinline__ int pages() const { return p1 - p0; }
     // steps of stream x, and the page of its step i, counted from p0
     __device__ __forceinline__ int steps(int x) const { return pair ? pages() : (pages() + 1 - x) / 2; }
     __device__ __forceinline__ int page_of(int x, int i) const { return pair ? i : 2 * i + x; }
@@ -221,8 +219,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const uint32_t q_s = smem_u32(smem), k_s = q_s + RING, v_s = q_s + V_RING;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + BARS);
     uint64_t *k_full = bars, *k_free = k_full + NK, *v_full = k_free + NK, *v_free = v_full + NV;
-    uint64_t *s_full = v_free + NV, *p_full = s_full + 4, *o_full = p_full + 4;              // [stream][step & 1]
-    uint64_t *q_full = o_full + 4, *q_free = q_full + 1, *o_free = q_full + 2, *both = q_full + 3;
+    uint64_t *s_full = v_free + NV, *p_full = s_full + 4, *o_full = p_full + 4, *v_here = o_full + 4;          // [stream][step & 1]
+    uint64_t *q_full = v_here + 4, *q_free = q_full + 1, *o_free = q_full + 2, *both = q_full + 3, *behind = q_full + 4;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
     volatile int* odd_tile = reinterpret_cast<volatile int*>(bars + N_BARS + 1);       // the last tile with a value that is not finite
     float2* ml_s = reinterpret_cast<float2*>(smem + ML);
@@ -233,7 +231,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         for (int i = 0; i < N_BARS; i++) {
             uint64_t* b = bars + i;
             const bool two = (b >= k_free && b < v_full) || (b >= v_free && b < s_full) || b == q_free;     // both streams say so
-            mbar_init(b, b >= p_full && b < o_full ? BM : b == o_free || b == both ? SOFT : two ? 2 : 1);
+            mbar_init(b, b >= p_full && b < o_full ? BM : b == o_free ? SOFT + 2 : b == both ? SOFT : two ? 2 : 1);
         }
         *odd_tile = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -245,16 +243,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     Walk w;
-    w.before = w.u = w.u_end = 0;
-    {
-        const int total = tree_units(a, 0, w.before);
-        const int nb = share_count(total, gridDim.x);
-        if ((int)blockIdx.x < nb) {
-            w.u = share_begin(total, blockIdx.x, nb), w.u_end = share_begin(total, blockIdx.x + 1, nb);
-            w.s = tree_find(a, w.u, w.before);
-            w.sq.load(a, w.s);
-        }
-    }
+    w.begin(a);
     fence_before();
     __syncthreads();
     fence_after();
@@ -307,17 +296,25 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             bool ok = true;
             for (; ok && w.next(a); tile++) {
                 const int n = w.steps(x);
-                // a page that both streams read is free when both say so; one that this stream alone reads it gives back for both
-                auto give_back = [&](uint64_t* bar) {
-                    umma_commit(bar);
-                    if (!w.pair) umma_commit(bar);
-                };
                 const uint64_t dqx = dq + (uint64_t)((w.pair ? x * Q_BYTES : 0) >> 4);
+                // Both streams see every page come in, one after the other, and give it back: a page that only the other one reads as
+                // soon as it has come. (A wait tells its phase from the one before by a bit alone, so no phase may be left out.)
+                int k_next = 0, v_next = 0;
+                auto see = [&](uint64_t* full, uint64_t* free, int& next, int j, auto slot, auto phase) {
+                    for (; next <= j; next++) {
+                        const uint32_t t = t0 + next;
+                        if (!mbar_wait(full + slot(t), phase(t))) return false;
+                        if (next < j) mbar_arrive(free + slot(t));
+                    }
+                    return true;
+                };
+                auto see_k = [&](int j) { return see(k_full, k_free, k_next, j, slot_of<NK>, phase_of<NK>); };
+                auto see_v = [&](int j) { return see(v_full, v_free, v_next, j, slot_of<NV>, phase_of<NV>); };
                 auto issue_s = [&](int i) {
-                    const uint32_t t = t0 + w.page_of(x, i), b = (done + i) & 1;
-                    if (!mbar_wait(k_full + slot_of<NK>(t), phase_of<NK>(t))) return false;
+                    const uint32_t j = w.page_of(x, i), slot = slot_of<NK>(t0 + j), b = (done + i) & 1;
+                    if (!see_k(j)) return false;
                     fence_after();
-                    const uint64_t dkt = dk + (uint64_t)((slot_of<NK>(t) * KV_BYTES) >> 4);
+                    const uint64_t dkt = dk + (uint64_t)((slot * KV_BYTES) >> 4);
 #pragma unroll
                     for (int hh = 0; hh < HALVES; hh++)
 #pragma unroll
@@ -325,30 +322,36 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                             umma_ss(t_sx + b * BN, dqx + (uint64_t)((hh * Q_ATOM_BYTES + k * 32) >> 4),
                                     dkt + (uint64_t)((hh * KV_ATOM_BYTES + k * 32) >> 4), IDESC_S, (hh | k) != 0);
                     umma_commit(bar_s + b);
-                    give_back(k_free + slot_of<NK>(t));
+                    umma_commit(k_free + slot);
                     if (i + 1 == n) umma_commit(q_free);
                     return true;
                 };
                 ok = mbar_wait(q_full, tile & 1);
+                // B begins a tile half a step behind A: side by side their warps all reach the exponentials at the same time
+                if (ok && x == 1) ok = mbar_wait(behind, tile & 1);
                 if (ok && n == 0) umma_commit(q_free);     // one page only: nothing for B
                 if (ok && n > 0) ok = issue_s(0);
                 if (ok && n > 1) ok = issue_s(1);
                 // the rows of the tile before have been read out of O
                 if (ok && tile > 0) ok = mbar_wait(o_free, (tile - 1) & 1);
                 for (int i = 0; i < n && ok; i++) {
-                    const uint32_t t = t0 + w.page_of(x, i), step = done + i, b = step & 1;
-                    if (!mbar_wait(v_full + slot_of<NV>(t), phase_of<NV>(t))) { ok = false; break; }
+                    const uint32_t j = w.page_of(x, i), slot = slot_of<NV>(t0 + j), step = done + i, b = step & 1;
+                    if (!see_v(j)) { ok = false; break; }
+                    mbar_arrive(v_here + 2 * x + b);       // softmax warps that look at the values wait for this
                     if (!mbar_wait(bar_p + b, (step >> 1) & 1)) { ok = false; break; }
                     fence_after();
-                    const uint64_t dvt = dv + (uint64_t)((slot_of<NV>(t) * KV_BYTES) >> 4);
+                    const uint64_t dvt = dv + (uint64_t)((slot * KV_BYTES) >> 4);
 #pragma unroll
                     for (int k = 0; k < BN / 16; k++)
                         umma_ts(t_ox, t_sx + b * BN + k * 8, dvt + (uint64_t)((k * 16 * 128) >> 4), IDESC_PV, (i | k) != 0);   // the first overwrites O
                     umma_commit(bar_o + b);
-                    give_back(v_free + slot_of<NV>(t));
+                    umma_commit(v_free + slot);
                     // into the buffer whose P was just used: products of one thread run in order
                     if (i + 2 < n) ok = issue_s(i + 2);
                 }
+                if (ok && k_next < w.pages()) ok = see_k(w.pages() - 1), mbar_arrive(k_free + slot_of<NK>(t0 + w.pages() - 1));
+                if (ok && v_next < w.pages()) ok = see_v(w.pages() - 1), mbar_arrive(v_free + slot_of<NV>(t0 + w.pages() - 1));
+                mbar_arrive(o_free);                       // the tile is not over before this thread has seen the last one's end
                 t0 += w.pages(), done += n;
             }
             if (!ok) atomicExch(err, 21);
@@ -369,17 +372,25 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             const bool any_row = (warp & 3) * 32 < rows;               // else the warp has no row of the tile
             // pages that every row sees: the cached tokens' and, with a window, none that the last node's begins in
             const int open_lo = a.window > 0 ? max(0, sq.pos0 + sq.n - a.window) : 0;
+            // the places that the row sees in its sequence's last two pages, worked out while the first scores are on their way
+            const int tail = max(w.p0, min(w.p1, sq.pages - 2));
+            uint64_t seen_tail[2] = {0, 0};
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                if (valid && tail + k < w.p1) seen_tail[k] = tree_mask(a, sq, words, qpos, (sq.first_page + tail + k) * BN);
             float m = -INFINITY, l = 0.f;
+            int next_page = n > 0 ? w.pt[w.p0 + w.page_of(x, 0)] : 0;
             for (int i = 0; i < n && ok; i++) {
                 const uint32_t step = done + i, b = step & 1, ph = (step >> 1) & 1;
-                const int j = w.p0 + w.page_of(x, i), key0 = (sq.first_page + j) * BN, page = w.pt[j];
+                const int j = w.p0 + w.page_of(x, i), key0 = (sq.first_page + j) * BN, page = next_page;
+                if (i + 1 < n) next_page = w.pt[w.p0 + w.page_of(x, i + 1)];
                 const bool held = page >= 0 && page < a.n_pages;
                 const bool open = held && key0 + BN <= sq.pos0 && key0 >= open_lo;
                 uint64_t seen = ~0ull;
                 if (!open) {
                     const uint32_t t = t0 + j - w.p0;
-                    seen = held && valid ? tree_mask(a, sq, words, qpos, key0) : 0ull;
-                    if (!mbar_wait(v_full + slot_of<NV>(t), phase_of<NV>(t))) { ok = false; break; }
+                    seen = !held || !valid ? 0ull : j >= tail ? seen_tail[j - tail ? 1 : 0] : tree_mask(a, sq, words, qpos, key0);
+                    if (!mbar_wait(v_here + 2 * x + b, ph)) { ok = false; break; }
                     // 16 bytes each of the page's values at a time
                     uint4* vs = reinterpret_cast<uint4*>(smem + V_RING + slot_of<NV>(t) * KV_BYTES);
                     bool odd = false;
@@ -409,6 +420,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 #pragma unroll
                     for (int c = 0; c < BN; c += 32) tmem_ld32(t_sx + b * BN + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
                     tmem_wait_ld();
+                    if (i == 0 && x == 0 && r == 0) mbar_arrive(behind);
                     float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     if (!open) {
                         const uint32_t half[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
@@ -438,17 +450,19 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                             tmem_st32(t_ox + c, o);
                         }
                     }
-                    float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+                    float2 sum2[2] = {};
                     uint32_t p[BN / 2];
+                    const float2 scale2 = make_float2(a.sl2, a.sl2), minus = make_float2(-ms, -ms);
 #pragma unroll
                     for (int k = 0; k < BN; k += 2) {
-                        const float e0 = ex2(fmaf(__uint_as_float(v[k]), a.sl2, -ms)), e1 = ex2(fmaf(__uint_as_float(v[k + 1]), a.sl2, -ms));
-                        sum4[(k >> 1) & 3] += e0 + e1;
-                        __nv_bfloat162 pk = __floats2bfloat162_rn(e0, e1);
+                        float2 e = fma2(make_float2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), scale2, minus);
+                        e.x = ex2(e.x), e.y = ex2(e.y);
+                        sum2[(k >> 1) & 1] = add2(sum2[(k >> 1) & 1], e);
+                        __nv_bfloat162 pk = __floats2bfloat162_rn(e.x, e.y);
                         p[k / 2] = *reinterpret_cast<uint32_t*>(&pk);
                     }
                     tmem_st32(t_sx + b * BN, p);
-                    l = l * alpha + (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+                    l = l * alpha + (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
                     m = m_new;
                     tmem_wait_st();
                     fence_before();
@@ -476,9 +490,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             if (any_row) {
                 __syncwarp();
                 fence_after();
-                const bool whole = w.pages() == sq.pages, mend = *odd_tile == mark, has = n > 0, has_other = !w.pair && w.steps(1 - x) > 0;
+                const bool whole = w.all(), mend = *odd_tile == mark, has = n > 0, has_other = !w.pair && w.steps(1 - x) > 0;
                 const float inv = l == 0.f ? 0.f : 1.f / l;
-                const size_t slot = (size_t)(2 * blockIdx.x + (w.p0 == 0 ? 1 : 0)) * 2 * BM;
+                const size_t slot = (size_t)w.slot() * 2 * BM;
                 const int row = (w.pair ? x * BM : 0) + r;
                 bf16* dst = out + (size_t)node * ldo + (size_t)(w.kvh * G + r % G) * HD;
                 if (!whole && r < rows && c0 == 0) ws_ml[slot + row] = make_float2(m, l);
@@ -584,7 +598,7 @@ DK_EXPORT int dk_attn_tree_tc(const void* q, long long ldq, void* out, long long
         return (int)cudaErrorInvalidValue;
     const int G = nh / nkv;
     TreeArgs a = {cu_q, seq_pos0, row_pos, page_table, tree, n_seq, words, pt_stride, n_pages, nh, nkv, window, 2 * (BM / G), BM / G, BM,
-                  scale * 1.4426950408889634f};
+                  pt_stride <= WHOLE_PAGES, EXTRA, scale * 1.4426950408889634f};
     if (!tree_units_fit(a, max_nodes) || nkv > 65535) return (int)cudaErrorInvalidValue;
     cudaError_t ce = cudaFuncSetAttribute(tree_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
     if (ce != cudaSuccess) {
