@@ -155,7 +155,8 @@ struct TreeWalk {
 __device__ __forceinline__ size_t part_at(int tile_rows, int row, int d) { return ((size_t)(d >> 2) * tile_rows + row) * 4 + (d & 3); }
 
 // Bits of the places [key0, key0 + 64) that a node sees; `words`: its row of the tree's bits; `pos`: its position, < 0 for none.
-__device__ __forceinline__ uint64_t tree_mask(const TreeArgs& a, const TreeSeq& q, const uint32_t* words, int pos, int key0) {
+// (Not inlined: the kernels are short, and code that runs once costs them more for being fetched than for being run.)
+static __device__ __noinline__ uint64_t tree_mask(const TreeArgs& a, TreeSeq q, const uint32_t* words, int pos, int key0) {
     if (pos < 0) return 0;
     auto low = [](int k) { return k <= 0 ? 0ull : k >= 64 ? ~0ull : (1ull << k) - 1; };   // the first k bits
     uint64_t m = low(q.pos0 - key0);

@@ -206,9 +206,16 @@ struct Walk : TreeWalk {
     __device__ __forceinline__ int page_of(int x, int i) const { return pair ? i : 2 * i + x; }
 };
 
-// Uses of a ring of N barriers, in turn: the t-th is slot t % N in its (t / N)-th phase.
-template <int N> __device__ __forceinline__ uint32_t slot_of(uint32_t t) { return t % N; }
-template <int N> __device__ __forceinline__ uint32_t phase_of(uint32_t t) { return (t / N) & 1; }
+// A place in a ring of N barriers, whose slots complete a phase at every turn.
+template <int N>
+struct Ring {
+    uint32_t slot = 0, phase = 0;
+    __device__ __forceinline__ void advance(uint32_t by = 1) {
+        slot += by;
+        while (slot >= N) slot -= N, phase ^= 1;
+    }
+    __device__ __forceinline__ uint32_t ahead(uint32_t by) const { return (slot + by) % N; }
+};
 
 // grid SMs, 352 threads. q as [rows][heads][HD] (map_q), map_k / map_v over one layer's store as [pages * nkv * 64, HD].
 __global__ void __launch_bounds__(THREADS, 1)
@@ -253,7 +260,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 
     if (warp == LOAD_WARP) {
         if (lane == 0 && !DK_STALLED) {  // --------------------------------------------------- every TMA
-            uint32_t t0 = 0, tile = 0;                     // pages and tiles before
+            uint32_t tile = 0, laps_k = 0, laps_v = 0;     // tiles before; pages asked for, up to a ring's length
+            Ring<NK> rk;
+            Ring<NV> rv;
             bool ok = true;
             auto load = [&](const CUtensorMap* map, uint32_t dst, uint64_t* bar, int j) {
                 mbar_expect_tx(bar, KV_BYTES);
@@ -271,17 +280,18 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                         tma_load_3d(q_s + x * Q_BYTES + hh * Q_ATOM_BYTES, &map_q, hh * 64, w.kvh * G, w.sq.flat0 + w.node0 + x * a.half_nodes, q_full);
                 for (int j = 0; j < n + 2 && ok; j++) {
                     if (j < n) {
-                        const uint32_t t = t0 + j;
-                        if (t >= NK && !mbar_wait(k_free + slot_of<NK>(t), phase_of<NK>(t - NK))) { ok = false; break; }
-                        load(&map_k, k_s + slot_of<NK>(t) * KV_BYTES, k_full + slot_of<NK>(t), j);
+                        if (laps_k == NK && !mbar_wait(k_free + rk.slot, rk.phase ^ 1)) { ok = false; break; }
+                        laps_k = min(laps_k + 1, (uint32_t)NK);
+                        load(&map_k, k_s + rk.slot * KV_BYTES, k_full + rk.slot, j);
+                        rk.advance();
                     }
                     if (j >= 2) {
-                        const uint32_t t = t0 + j - 2;
-                        if (t >= NV && !mbar_wait(v_free + slot_of<NV>(t), phase_of<NV>(t - NV))) { ok = false; break; }
-                        load(&map_v, v_s + slot_of<NV>(t) * KV_BYTES, v_full + slot_of<NV>(t), j - 2);
+                        if (laps_v == NV && !mbar_wait(v_free + rv.slot, rv.phase ^ 1)) { ok = false; break; }
+                        laps_v = min(laps_v + 1, (uint32_t)NV);
+                        load(&map_v, v_s + rv.slot * KV_BYTES, v_full + rv.slot, j - 2);
+                        rv.advance();
                     }
                 }
-                t0 += n;
             }
             if (!ok) atomicExch(err, 23);
         }
@@ -292,29 +302,30 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             const uint64_t dq = desc_k_major(q_s), dk = desc_k_major(k_s), dv = desc_n_major(v_s);
             uint64_t *bar_s = s_full + 2 * x, *bar_p = p_full + 2 * x, *bar_o = o_full + 2 * x;
             const uint32_t t_sx = t_s + 2 * x * BN, t_ox = t_o + x * 128;
-            uint32_t t0 = 0, tile = 0, done = 0;           // pages, tiles and steps before
+            uint32_t tile = 0, done = 0;                   // tiles and steps before
+            Ring<NK> rk;                                   // the next page to be seen
+            Ring<NV> rv;
             bool ok = true;
             for (; ok && w.next(a); tile++) {
                 const int n = w.steps(x);
                 const uint64_t dqx = dq + (uint64_t)((w.pair ? x * Q_BYTES : 0) >> 4);
-                // Both streams see every page come in, one after the other, and give it back: a page that only the other one reads as
-                // soon as it has come. (A wait tells its phase from the one before by a bit alone, so no phase may be left out.)
+                // Both streams see every page come in, one after the other: a wait tells its phase from the one before by a bit alone,
+                // so no phase may be left out. A page that only the other stream reads is given back as soon as it has come.
                 int k_next = 0, v_next = 0;
-                auto see = [&](uint64_t* full, uint64_t* free, int& next, int j, auto slot, auto phase) {
-                    for (; next <= j; next++) {
-                        const uint32_t t = t0 + next;
-                        if (!mbar_wait(full + slot(t), phase(t))) return false;
-                        if (next < j) mbar_arrive(free + slot(t));
+                auto see = [&](uint64_t* full, uint64_t* free, auto& ring, int& next, int upto) {
+                    for (; next < upto; next++) {
+                        if (!mbar_wait(full + ring.slot, ring.phase)) return false;
+                        mbar_arrive(free + ring.slot);
+                        ring.advance();
                     }
                     return true;
                 };
-                auto see_k = [&](int j) { return see(k_full, k_free, k_next, j, slot_of<NK>, phase_of<NK>); };
-                auto see_v = [&](int j) { return see(v_full, v_free, v_next, j, slot_of<NV>, phase_of<NV>); };
+                auto have_k = [&](int i) {                 // the keys of step i are here
+                    return see(k_full, k_free, rk, k_next, w.page_of(x, i)) && mbar_wait(k_full + rk.slot, rk.phase);
+                };
                 auto issue_s = [&](int i) {
-                    const uint32_t j = w.page_of(x, i), slot = slot_of<NK>(t0 + j), b = (done + i) & 1;
-                    if (!see_k(j)) return false;
-                    fence_after();
-                    const uint64_t dkt = dk + (uint64_t)((slot * KV_BYTES) >> 4);
+                    const uint32_t b = (done + i) & 1;
+                    const uint64_t dkt = dk + (uint64_t)((rk.slot * KV_BYTES) >> 4);
 #pragma unroll
                     for (int hh = 0; hh < HALVES; hh++)
 #pragma unroll
@@ -322,37 +333,39 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                             umma_ss(t_sx + b * BN, dqx + (uint64_t)((hh * Q_ATOM_BYTES + k * 32) >> 4),
                                     dkt + (uint64_t)((hh * KV_ATOM_BYTES + k * 32) >> 4), IDESC_S, (hh | k) != 0);
                     umma_commit(bar_s + b);
-                    umma_commit(k_free + slot);
                     if (i + 1 == n) umma_commit(q_free);
-                    return true;
+                    rk.advance(), k_next++;
                 };
                 ok = mbar_wait(q_full, tile & 1);
                 // B begins a tile half a step behind A: side by side their warps all reach the exponentials at the same time
                 if (ok && x == 1) ok = mbar_wait(behind, tile & 1);
                 if (ok && n == 0) umma_commit(q_free);     // one page only: nothing for B
-                if (ok && n > 0) ok = issue_s(0);
-                if (ok && n > 1) ok = issue_s(1);
+                for (int i = 0; i < min(n, 2) && ok; i++) {
+                    ok = have_k(i);
+                    if (ok) fence_after(), issue_s(i);
+                }
                 // the rows of the tile before have been read out of O
                 if (ok && tile > 0) ok = mbar_wait(o_free, (tile - 1) & 1);
                 for (int i = 0; i < n && ok; i++) {
-                    const uint32_t j = w.page_of(x, i), slot = slot_of<NV>(t0 + j), step = done + i, b = step & 1;
-                    if (!see_v(j)) { ok = false; break; }
+                    const uint32_t step = done + i, b = step & 1;
+                    if (!see(v_full, v_free, rv, v_next, w.page_of(x, i)) || !mbar_wait(v_full + rv.slot, rv.phase)) { ok = false; break; }
                     mbar_arrive(v_here + 2 * x + b);       // softmax warps that look at the values wait for this
+                    // all that both products wait for, so that they go out in one run
+                    if (i + 2 < n && !have_k(i + 2)) { ok = false; break; }
                     if (!mbar_wait(bar_p + b, (step >> 1) & 1)) { ok = false; break; }
                     fence_after();
-                    const uint64_t dvt = dv + (uint64_t)((slot * KV_BYTES) >> 4);
+                    const uint64_t dvt = dv + (uint64_t)((rv.slot * KV_BYTES) >> 4);
 #pragma unroll
                     for (int k = 0; k < BN / 16; k++)
                         umma_ts(t_ox, t_sx + b * BN + k * 8, dvt + (uint64_t)((k * 16 * 128) >> 4), IDESC_PV, (i | k) != 0);   // the first overwrites O
                     umma_commit(bar_o + b);
-                    umma_commit(v_free + slot);
+                    rv.advance(), v_next++;
                     // into the buffer whose P was just used: products of one thread run in order
-                    if (i + 2 < n) ok = issue_s(i + 2);
+                    if (i + 2 < n) issue_s(i + 2);
                 }
-                if (ok && k_next < w.pages()) ok = see_k(w.pages() - 1), mbar_arrive(k_free + slot_of<NK>(t0 + w.pages() - 1));
-                if (ok && v_next < w.pages()) ok = see_v(w.pages() - 1), mbar_arrive(v_free + slot_of<NV>(t0 + w.pages() - 1));
+                if (ok) ok = see(k_full, k_free, rk, k_next, w.pages()) && see(v_full, v_free, rv, v_next, w.pages());
                 mbar_arrive(o_free);                       // the tile is not over before this thread has seen the last one's end
-                t0 += w.pages(), done += n;
+                done += n;
             }
             if (!ok) atomicExch(err, 21);
         }
@@ -360,7 +373,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         const int x = warp >> 2, r = threadIdx.x & (BM - 1);
         const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16, t_sx = t_s + lane_off + 2 * x * BN, t_ox = t_o + lane_off + x * 128;
         uint64_t *bar_s = s_full + 2 * x, *bar_p = p_full + 2 * x, *bar_o = o_full + 2 * x;
-        uint32_t t0 = 0, tile = 0, done = 0, shared_tiles = 0;
+        uint32_t tile = 0, done = 0, shared_tiles = 0;
+        Ring<NK> rk;                                       // the tile's first page
+        Ring<NV> rv;
         bool ok = true;
         for (; ok && w.next(a); tile++) {
             const TreeSeq& sq = w.sq;
@@ -386,13 +401,18 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 if (i + 1 < n) next_page = w.pt[w.p0 + w.page_of(x, i + 1)];
                 const bool held = page >= 0 && page < a.n_pages;
                 const bool open = held && key0 + BN <= sq.pos0 && key0 >= open_lo;
+                if (!mbar_wait(bar_s + b, ph)) { ok = false; break; }
+                if (r == 0) {                              // S is here, so its keys are free, and P.V of two steps before, which stood ahead of it, is done
+                    mbar_arrive(k_free + rk.ahead(j - w.p0));
+                    // (said before this step's values are waited for: their page may come to lie where those did)
+                    if (i > 1) mbar_arrive(v_free + rv.ahead(w.page_of(x, i - 2)));
+                }
                 uint64_t seen = ~0ull;
                 if (!open) {
-                    const uint32_t t = t0 + j - w.p0;
                     seen = !held || !valid ? 0ull : j >= tail ? seen_tail[j - tail ? 1 : 0] : tree_mask(a, sq, words, qpos, key0);
                     if (!mbar_wait(v_here + 2 * x + b, ph)) { ok = false; break; }
                     // 16 bytes each of the page's values at a time
-                    uint4* vs = reinterpret_cast<uint4*>(smem + V_RING + slot_of<NV>(t) * KV_BYTES);
+                    uint4* vs = reinterpret_cast<uint4*>(smem + V_RING + rv.ahead(j - w.p0) * KV_BYTES);
                     bool odd = false;
 #pragma unroll
                     for (int k = 0; k < KV_BYTES / 16 / BM; k++) {
@@ -412,7 +432,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     }
                     if (odd) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
-                if (!mbar_wait(bar_s + b, ph)) { ok = false; break; }
                 if (any_row) {
                     __syncwarp();
                     fence_after();
@@ -471,6 +490,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             }
             if (ok && n > 0) ok = mbar_wait(bar_o + ((done + n - 1) & 1), ((done + n - 1) >> 1) & 1);
             if (!ok) break;
+            if (r == 0)
+                for (int i = max(0, n - 2); i < n; i++) mbar_arrive(v_free + rv.ahead(w.page_of(x, i)));
             if (!valid) m = -INFINITY, l = 0.f;
             // the factors of the two streams' rows: with rows in both, the own one alone
             float mine = 1.f, other = 0.f;
@@ -544,7 +565,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 fence_before();
             }
             mbar_arrive(o_free);
-            t0 += w.pages(), done += n;
+            rk.advance(w.pages() % NK), rv.advance(w.pages() % NV), done += n;
         }
         if (!ok && lane == 0) atomicExch(err, 22);
     }
