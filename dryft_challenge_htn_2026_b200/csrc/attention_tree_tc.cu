@@ -194,6 +194,13 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+// Whether one of two bfloat16 numbers is infinite or none; the two with 0 in the place of such a one.
+__device__ __forceinline__ bool no_number(uint32_t x) { return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u; }
+__device__ __forceinline__ uint32_t numbers_of(uint32_t x) {
+    if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
+    return (x & 0x7f800000u) == 0x7f800000u ? x & 0xffffu : x;
+}
+
 struct Walk : TreeWalk {
     bool pair;                                             // two streams of rows; else two streams of pages
     __device__ __forceinline__ bool next(const TreeArgs& a) {
@@ -205,6 +212,26 @@ struct Walk : TreeWalk {
     __device__ __forceinline__ int steps(int x) const { return pair ? pages() : (pages() + 1 - x) / 2; }
     __device__ __forceinline__ int page_of(int x, int i) const { return pair ? i : 2 * i + x; }
 };
+
+// Values that are not finite were left out of the products: the columns [c0, c1) of a row that sees some become their sum, which the
+// rest of the row's sum does not change. To dst (the row's result) or, if that is null, to its part.
+__device__ __noinline__ void mend_row(const TreeArgs& a, const Walk& w, const uint32_t* words, int pos, int open_lo, const bf16* v_store,
+                                      int c0, int c1, bf16* dst, float* part, int row) {
+    for (int c = c0; c < c1; c++) {
+        float sum = 0.f;
+        for (int j = w.p0; j < w.p1; j++) {
+            const int key0 = (w.sq.first_page + j) * BN, page = w.pt[j];
+            if (page < 0 || page >= a.n_pages || (key0 + BN <= w.sq.pos0 && key0 >= open_lo)) continue;
+            for (uint64_t left = tree_mask(a, w.sq, words, pos, key0); left; left &= left - 1) {
+                const float x = __bfloat162float(v_store[kv_offset(page, a.nkv, w.kvh, __ffsll((long long)left) - 1, HD) + c]);
+                if (!isfinite(x)) sum += x;
+            }
+        }
+        if (sum == 0.f) continue;
+        if (dst != nullptr) dst[c] = __float2bfloat16_rn(sum);
+        else part[part_at(2 * BM, row, c)] = sum;
+    }
+}
 
 // A place in a ring of N barriers, whose slots complete a phase at every turn.
 template <int N>
@@ -234,12 +261,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.nh / a.nkv;
 
     pdl_wait();
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < N_BARS; i++) {
-            uint64_t* b = bars + i;
-            const bool two = (b >= k_free && b < v_full) || (b >= v_free && b < s_full) || b == q_free;     // both streams say so
-            mbar_init(b, b >= p_full && b < o_full ? BM : b == o_free ? SOFT + 2 : b == both ? SOFT : two ? 2 : 1);
-        }
+    if (threadIdx.x < N_BARS) {
+        uint64_t* b = bars + threadIdx.x;
+        const bool two = (b >= k_free && b < v_full) || (b >= v_free && b < s_full) || b == q_free;     // both streams say so
+        mbar_init(b, b >= p_full && b < o_full ? BM : b == o_free ? SOFT + 2 : b == both ? SOFT : two ? 2 : 1);
         *odd_tile = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -414,19 +439,14 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     // 16 bytes each of the page's values at a time
                     uint4* vs = reinterpret_cast<uint4*>(smem + V_RING + rv.ahead(j - w.p0) * KV_BYTES);
                     bool odd = false;
-#pragma unroll
+#pragma unroll 2
                     for (int k = 0; k < KV_BYTES / 16 / BM; k++) {
                         uint4 val = vs[k * BM + r];
-                        uint32_t* e = reinterpret_cast<uint32_t*>(&val);
-                        bool mine = false;
-#pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            if ((e[q] & 0x7f80u) == 0x7f80u) e[q] &= 0xffff0000u, mine = true;
-                            if ((e[q] & 0x7f800000u) == 0x7f800000u) e[q] &= 0xffffu, mine = true;
-                        }
-                        if (mine) {                                    // said before it is done: the other stream may look at the page too
+                        if (no_number(val.x) | no_number(val.y) | no_number(val.z) | no_number(val.w)) {
+                            // said before it is done: the other stream may look at the page too
                             *odd_tile = mark;
                             __threadfence_block();
+                            val = make_uint4(numbers_of(val.x), numbers_of(val.y), numbers_of(val.z), numbers_of(val.w));
                             vs[k * BM + r] = val, odd = true;
                         }
                     }
@@ -528,23 +548,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     for (int k = 0; k < OC; k++)
                         o[k] = __float_as_uint((has ? __uint_as_float(o[k]) * mine : 0.f) + (has_other ? __uint_as_float(o2[k]) * other : 0.f));
                     if (r < rows) {
-                        if (!valid || l == 0.f) {
+                        if (!valid || l == 0.f)
 #pragma unroll
                             for (int k = 0; k < OC; k++) o[k] = 0;
-                        } else if (mend) {     // values that are not finite, for the rows that see them
-                            for (int j = w.p0; j < w.p1; j++) {
-                                const int key0 = (sq.first_page + j) * BN, page = w.pt[j];
-                                if (page < 0 || page >= a.n_pages || (key0 + BN <= sq.pos0 && key0 >= open_lo)) continue;
-                                for (uint64_t left = tree_mask(a, sq, words, qpos, key0); left; left &= left - 1) {
-                                    const bf16* val = v_store + kv_offset(page, a.nkv, w.kvh, __ffsll((long long)left) - 1, HD) + c;
-#pragma unroll
-                                    for (int k = 0; k < OC; k++) {
-                                        const float y = __bfloat162float(val[k]);
-                                        if (!isfinite(y)) o[k] = __float_as_uint(__uint_as_float(o[k]) + y);
-                                    }
-                                }
-                            }
-                        }
                         if (whole) {
 #pragma unroll
                             for (int k = 0; k < OC; k += 8) {
@@ -563,6 +569,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     }
                 }
                 fence_before();
+                if (mend && valid && l != 0.f)
+                    mend_row(a, w, words, qpos, open_lo, v_store, c0, c1, whole ? dst : nullptr, ws_acc + slot * HD, row);
             }
             mbar_arrive(o_free);
             rk.advance(w.pages() % NK), rv.advance(w.pages() % NV), done += n;
