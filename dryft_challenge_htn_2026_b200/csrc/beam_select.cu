@@ -11,22 +11,26 @@
 // against the piece's maximum, added up in float32 within a thread and in double from there on, values compared in double, so that a
 // rank does not hang on the rounding of the scores (float32 scores around -30 are 2^-19 apart).
 //
-// First launch, a block a piece of a row: the logits stay in registers; the block's `best`-th largest of the threads' own maxima is
-// a floor under the `best`-th largest logit, few logits beside the ones looked for reach it, and these are ranked by counting. Second
-// launch, a block a request: the same over what the pieces left. Bound by reading the logits where there are many rows, by the two
-// launches' latency where there are few.
-#include "common.cuh"
+// First launch, a block a piece of 8,192 logits of a row, which stay in registers. A floor under the `best`-th largest: of each warp
+// the best / 8-th largest of its threads' own maxima, the least of these; few logits beside the ones looked for reach it, and these
+// are ranked by counting. Where many do (a warp without large ones), the exact `best`-th largest of the threads' maxima takes its
+// place, above which `best` threads have all there is. (That one alone, 256 comparisons a thread, took two thirds of the kernel's
+// time: 47 us for 128 rows of 100,003.) Second launch, a block a request: the same over the pieces' lists, which are in order. Bound
+// by reading the logits where there are many rows, by the two launches' latency where there are few.
+#include "logit_rows.cuh"
 
 namespace {
 
-constexpr int THREADS = 256, MAX_BEST = 64, MAX_BEAMS = 32;
+constexpr int THREADS = 256, WARPS = THREADS / 32, EACH = 32, MAX_BEST = 64, MAX_BEAMS = 32;
+constexpr int ROOM = 512;                                               // logits that are ranked at once under the quick floor
+typedef LogitPiece<THREADS, EACH> Piece;
 
 // Larger key: larger logit, then lower index. 0: none.
-__device__ __forceinline__ uint64_t key_of(float v, int i) {
-    if (!isfinite(v)) return 0;
+__device__ __forceinline__ uint32_t order_of(float v) {
     const uint32_t b = __float_as_uint(v + 0.f);                         // -0 counts as 0
-    return (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (uint32_t)~i;
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ uint64_t key_of(float v, int i) { return isfinite(v) ? (uint64_t)order_of(v) << 32 | (uint32_t)~i : 0; }
 __device__ __forceinline__ float logit_of(uint64_t key) {
     const uint32_t b = (uint32_t)(key >> 32);
     return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
@@ -34,57 +38,63 @@ __device__ __forceinline__ float logit_of(uint64_t key) {
 __device__ __forceinline__ int index_of(uint64_t key) { return (int)~(uint32_t)key; }
 
 // grid (pieces, rows). ws_key [rows][pieces][best] in falling order (0: none), ws_sum [rows][pieces] = (maximum, sum).
-template <int EACH, bool WIDE>
 __global__ void __launch_bounds__(THREADS)
 beam_pieces_kernel(const float* logits, int V, int best, uint64_t* ws_key, double2* ws_sum) {
-    __shared__ uint64_t tops[THREADS], floor_key;
+    __shared__ uint64_t tops[THREADS], floors[WARPS], exact_floor;
     __shared__ uint64_t found[MAX_BEST * EACH];
-    __shared__ float red_m[THREADS / 32];
-    __shared__ double red_s[THREADS / 32];
+    __shared__ float red_m[WARPS];
+    __shared__ double red_s[WARPS];
     __shared__ int count;
     pdl_wait();
     pdl_launch_dependents();
     const int t = threadIdx.x, lane = t & 31, w = t >> 5;
     const float* z = logits + (size_t)blockIdx.y * V;
-    const int begin = blockIdx.x * (THREADS * EACH), end = min(V, begin + THREADS * EACH);
-    auto index = [&](int k) { return WIDE ? begin + ((k / 4) * THREADS + t) * 4 + k % 4 : begin + k * THREADS + t; };
+    const Piece piece(z, blockIdx.x);
     float v[EACH];
-    if (WIDE) {
-#pragma unroll
-        for (int k = 0; k < EACH; k += 4)
-            *reinterpret_cast<float4*>(v + k) = index(k) < end ? *reinterpret_cast<const float4*>(z + index(k))
-                                                              : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    } else {
-#pragma unroll
-        for (int k = 0; k < EACH; k++) v[k] = index(k) < end ? z[index(k)] : -INFINITY;
-    }
-    if (t == 0) count = 0, floor_key = 1;
-    uint64_t top = 0;
+    piece.load(z, V, v);
+    if (t == 0) count = 0, exact_floor = 1;
     float m = -INFINITY;
 #pragma unroll
     for (int k = 0; k < EACH; k++) {
         if (!isfinite(v[k])) v[k] = -INFINITY;
         m = fmaxf(m, v[k]);
     }
+    int at = 0;
 #pragma unroll
     for (int k = EACH - 1; k >= 0; k--)
-        if (v[k] == m) top = key_of(v[k], index(k));                    // the lowest index of the thread's maximum
+        if (v[k] == m) at = piece.index(k);                              // the lowest index of the thread's maximum
+    const uint64_t top = key_of(m, at);
     tops[t] = top;
+    // the warp's floor: its threads' maxima, largest first
+    uint64_t least = ~0ull;
+    uint32_t left = (uint32_t)(top >> 32);
+    for (int r = 0; r < (best + WARPS - 1) / WARPS; r++) {
+        const uint32_t high = __reduce_max_sync(0xffffffffu, left);
+        const int who = __ffs(__ballot_sync(0xffffffffu, left == high)) - 1;
+        const uint64_t key = high ? __shfl_sync(0xffffffffu, top, who) : 0;
+        least = key < least ? key : least;
+        if (lane == who) left = 0;
+    }
+    float wm = m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) red_m[w] = m;
+    for (int o = 16; o > 0; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
+    if (lane == 0) red_m[w] = wm, floors[w] = least;
     __syncthreads();
-    m = red_m[0];
+    float bm = red_m[0];
+    uint64_t floor_key = floors[0];
 #pragma unroll
-    for (int i = 1; i < THREADS / 32; i++) m = fmaxf(m, red_m[i]);
-    // the best-th largest of the threads' maxima
-    int above = 0;
-#pragma unroll 8
-    for (int i = 0; i < THREADS; i++) above += tops[i] > top;
-    if (top != 0 && above == best - 1) floor_key = top;
+    for (int i = 1; i < WARPS; i++) bm = fmaxf(bm, red_m[i]), floor_key = floors[i] < floor_key ? floors[i] : floor_key;
+    floor_key = floor_key ? floor_key : 1;
+    int mine = 0;
+    if (top >= floor_key) {
+        const float low = logit_of(floor_key);
+#pragma unroll
+        for (int k = 0; k < EACH; k++) mine += floor_key == 1 ? v[k] != -INFINITY : v[k] >= low;
+    }
+    if (mine) atomicAdd(&count, mine);                                   // an upper bound of what is to be ranked
     float sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < EACH; k++) sum += v[k] == -INFINITY ? 0.f : expf(v[k] - m);
+    for (int k = 0; k < EACH; k++) sum += v[k] == -INFINITY ? 0.f : expf(v[k] - bm);
     double total = sum;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -92,16 +102,28 @@ beam_pieces_kernel(const float* logits, int V, int best, uint64_t* ws_key, doubl
     __syncthreads();
     if (t == 0) {
         total = 0.;
-        for (int i = 0; i < THREADS / 32; i++) total += red_s[i];
-        ws_sum[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = make_double2((double)m, total);
+        for (int i = 0; i < WARPS; i++) total += red_s[i];
+        ws_sum[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = make_double2((double)bm, total);
     }
-    const uint64_t least = floor_key;
-    if (top >= least) {
+    if (count > ROOM) {
+        int above = 0;
+#pragma unroll 4
+        for (int i = 0; i < THREADS; i++) above += tops[i] > top;
+        if (top != 0 && above == best - 1) exact_floor = top;
+        __syncthreads();
+        floor_key = exact_floor;
+    }
+    __syncthreads();
+    if (t == 0) count = 0;
+    __syncthreads();
+    if (top >= floor_key) {
+        const float low = floor_key == 1 ? -INFINITY : logit_of(floor_key);
 #pragma unroll
-        for (int k = 0; k < EACH; k++) {
-            const uint64_t key = key_of(v[k], index(k));
-            if (key >= least) found[atomicAdd(&count, 1)] = key;        // `best` threads at most have any
-        }
+        for (int k = 0; k < EACH; k++)
+            if (v[k] >= low) {
+                const uint64_t key = key_of(v[k], piece.index(k));
+                if (key >= floor_key) found[atomicAdd(&count, 1)] = key;
+            }
     }
     __syncthreads();
     const int n = count;
@@ -115,15 +137,21 @@ beam_pieces_kernel(const float* logits, int V, int best, uint64_t* ws_key, doubl
     for (int i = n + t; i < best; i += THREADS) out[i] = 0;
 }
 
+// A value in double, in the order of its bits, and its place among all beams' tokens; place -1: none.
 struct Candidate {
-    double value;
-    int flat;                                                            // beam * V + token; -1: none
-    __device__ __forceinline__ bool before(const Candidate& o) const {
-        return flat >= 0 && (o.flat < 0 || value > o.value || (value == o.value && flat < o.flat));
-    }
+    uint64_t order;
+    int flat;
+    __device__ __forceinline__ bool before(const Candidate& o) const { return order > o.order || (order == o.order && (unsigned)flat < (unsigned)o.flat); }
 };
+__device__ __forceinline__ Candidate candidate(double value, int flat) {
+    const uint64_t b = (uint64_t)__double_as_longlong(value + 0.);
+    return Candidate{b >> 63 ? ~b : b | 1ull << 63, flat};
+}
+__device__ __forceinline__ double value_of(const Candidate& c) {
+    return __longlong_as_double((long long)(c.order >> 63 ? c.order & ~(1ull << 63) : ~c.order));
+}
 
-// grid (requests). Dynamic shared memory: best * ceil(beams * pieces * best / THREADS) candidates.
+// grid (requests). Dynamic shared memory: best * best * ceil(lists / THREADS) candidates.
 __global__ void __launch_bounds__(THREADS)
 beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, int V, int beams, int best, const float* scores,
                    const int* ended, float* scores_out, int* beam_out, int* tok_out) {
@@ -133,11 +161,14 @@ beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, in
     __shared__ double offset[MAX_BEAMS];
     __shared__ int kind[MAX_BEAMS];                                      // 0: not live, 1: live, 2: at its end
     __shared__ int count;
+    const Candidate none = {0, -1};
     pdl_wait();
     pdl_launch_dependents();
     const int r = blockIdx.x, t = threadIdx.x, lane = t & 31, w = t >> 5;
-    for (int b = w; b < beams; b += THREADS / 32) {
+    for (int b = w; b < beams; b += WARPS) {
         const double2* part = ws_sum + (size_t)(r * beams + b) * pieces;
+        const float score = scores[r * beams + b];
+        const bool done = ended != nullptr && ended[r * beams + b] != 0;
         double m = -INFINITY, sum = 0.;
         for (int c = lane; c < pieces; c += 32) m = fmax(m, part[c].x);
 #pragma unroll
@@ -146,44 +177,41 @@ beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, in
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {
-            const float score = scores[r * beams + b];
-            const bool done = ended != nullptr && ended[r * beams + b] != 0;
             kind[b] = !isfinite(score) ? 0 : done ? 2 : sum > 0. ? 1 : 0;
             offset[b] = kind[b] == 1 ? (double)score - (m + log(sum)) : (double)score;
         }
     }
-    if (t == 0) count = 0, least = Candidate{-INFINITY, -1};
+    if (t == 0) count = 0, least = none;
     __syncthreads();
-    // item i: the (i / lists)-th of list i % lists, so that the threads' first items are the lists' first
-    const int lists = beams * pieces, items = lists * best;
-    auto item = [&](int i) {
-        const int list = i % lists, rank = i / lists, b = list / pieces;
-        Candidate c = {-INFINITY, -1};
-        if (kind[b] == 2) {
-            if (rank == 0 && list == b * pieces) c = Candidate{offset[b], b * V};
-        } else if (kind[b] == 1) {
-            const uint64_t key = ws_key[((size_t)r * lists + list) * best + rank];
-            if (key) c = Candidate{(double)logit_of(key) + offset[b], b * V + index_of(key)};
-        }
-        return c;
+    // list l: piece l % pieces of beam l / pieces, in falling order; a beam at its end has one candidate, in its first list
+    const int lists = beams * pieces;
+    auto item = [&](int l, int rank) {
+        const int b = l / pieces;
+        if (kind[b] == 2) return rank == 0 && l == b * pieces ? candidate(offset[b], b * V) : none;
+        const uint64_t key = kind[b] == 1 ? ws_key[((size_t)r * lists + l) * best + rank] : 0;
+        return key ? candidate((double)logit_of(key) + offset[b], b * V + index_of(key)) : none;
     };
-    Candidate top = {-INFINITY, -1};
-    for (int i = t; i < items; i += THREADS) {
-        const Candidate c = item(i);
+    Candidate top = none;
+    for (int l = t; l < lists; l += THREADS) {
+        const Candidate c = item(l, 0);
         if (c.before(top)) top = c;
     }
     tops[t] = top;
     __syncthreads();
     int above = 0;
-#pragma unroll 8
-    for (int i = 0; i < THREADS; i++) above += tops[i].before(top);
-    if (top.flat >= 0 && above == best - 1) least = top;
+    const int n_tops = min(THREADS, lists);
+#pragma unroll 4
+    for (int i = 0; i < n_tops; i++) above += tops[i].before(top);
+    if (top.flat >= 0 && above == best - 1) least = top;                 // the best-th largest of the threads' largest
     __syncthreads();
-    if (top.flat >= 0 && !least.before(top))
-        for (int i = t; i < items; i += THREADS) {
-            const Candidate c = item(i);
-            if (c.flat >= 0 && !least.before(c)) found[atomicAdd(&count, 1)] = c;
-        }
+    const Candidate low = least;
+    if (top.flat >= 0 && !low.before(top))
+        for (int l = t; l < lists; l += THREADS)
+            for (int rank = 0; rank < best; rank++) {
+                const Candidate c = item(l, rank);
+                if (c.flat < 0 || low.before(c)) break;
+                found[atomicAdd(&count, 1)] = c;
+            }
     __syncthreads();
     const int n = count;
     for (int i = t; i < n; i += THREADS) {
@@ -191,7 +219,7 @@ beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, in
         int rank = 0;
         for (int j = 0; j < n; j++) rank += found[j].before(c);
         if (rank < best) {
-            scores_out[(size_t)r * best + rank] = (float)c.value;
+            scores_out[(size_t)r * best + rank] = (float)value_of(c);
             beam_out[(size_t)r * best + rank] = c.flat / V;
             tok_out[(size_t)r * best + rank] = c.flat % V;
         }
@@ -200,17 +228,13 @@ beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, in
         scores_out[(size_t)r * best + i] = -INFINITY, beam_out[(size_t)r * best + i] = 0, tok_out[(size_t)r * best + i] = 0;
 }
 
-// Logits a block of the first launch takes
-constexpr int EACH = 32;
-
 size_t select_smem(int beams, int pieces, int best) {
-    return (size_t)best * ((beams * pieces * best + THREADS - 1) / THREADS) * sizeof(Candidate);
+    return (size_t)best * best * ((beams * pieces + THREADS - 1) / THREADS) * sizeof(Candidate);
 }
 
 }  // namespace
 
-DK_EXPORT int dk_beam_pieces(int V) { return (V + THREADS * EACH - 1) / (THREADS * EACH); }
-
+DK_EXPORT int dk_beam_pieces(int V) { return logit_pieces(V, Piece::SIZE); }
 DK_EXPORT int dk_beam_select_takes(int V, int beams, int best) { return select_smem(beams, dk_beam_pieces(V), best) <= 200 * 1024; }
 
 // logits [requests * beams, V] float32, scores [requests, beams], ended [requests, beams] or null; ws_key: requests * beams * pieces *
@@ -223,15 +247,16 @@ DK_EXPORT int dk_beam_select(const float* logits, int V, int requests, int beams
     const int pieces = dk_beam_pieces(V);
     const size_t smem = select_smem(beams, pieces, best);
     if (smem > 200 * 1024) return (int)cudaErrorInvalidValue;
-    cudaError_t ce = cudaFuncSetAttribute(beam_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-    if (ce != cudaSuccess) {
-        cudaGetLastError();
-        return (int)ce;
+    if (smem > 32 * 1024) {
+        cudaError_t ce = cudaFuncSetAttribute(beam_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+        if (ce != cudaSuccess) {
+            cudaGetLastError();
+            return (int)ce;
+        }
     }
-    const bool wide = V % 4 == 0 && ((uintptr_t)logits & 15) == 0;      // rows on 16-byte boundaries: 16 bytes a load
-    int e = dk_launch(wide ? beam_pieces_kernel<EACH, true> : beam_pieces_kernel<EACH, false>, dim3(pieces, requests * beams), dim3(THREADS),
-                      0, st, logits, V, best, ws_key, (double2*)ws_sum);
+    int e = dk_launch(beam_pieces_kernel, dim3(pieces, requests * beams), dim3(THREADS), 0, st, logits, V, best, ws_key, (double2*)ws_sum);
     if (e) return e;
-    return dk_launch(beam_select_kernel, dim3(requests), dim3(THREADS), smem, st, (const uint64_t*)ws_key, (const double2*)ws_sum, pieces, V,
-                     beams, best, scores, ended, scores_out, beam_out, tok_out);
+    // (may start under the end of the first: it reads nothing before)
+    return dk_launch_as(true, beam_select_kernel, dim3(requests), dim3(THREADS), smem, st, (const uint64_t*)ws_key, (const double2*)ws_sum, pieces,
+                        V, beams, best, scores, ended, scores_out, beam_out, tok_out);
 }

@@ -7,16 +7,29 @@
 // how many steps they take, not which they are. From node 0 on the path goes to the child that holds the chosen token (the lowest
 // one, if several do) until there is none; the token chosen there is the sequence's next.
 //
-// Two launches: the best token of each piece of 4,096 logits, over all nodes and pieces side by side (one pass over the logits: bound
-// by reading them); then a block a sequence puts the pieces together and walks the path.
+// Two launches: the best token of each piece of 8,192 logits, over all nodes and pieces side by side (one pass over the logits: bound
+// by reading them where the choice is greedy); then a block a sequence puts the pieces together and walks the path. Drawing costs a
+// hash and two logarithms a logit. Most logits are spared the logarithms: -log(u) >= 1 - u, so the noise is at most -log(1 - u), and
+// what does not reach the thread's best so far with that much cannot win.
+#include "logit_rows.cuh"
 #include "sampling_kernels.cuh"
 
 namespace {
 
-constexpr int THREADS = 256, EACH = 16, CHUNK = THREADS * EACH, MAX_NODES = 1024;
+constexpr int THREADS = 256, EACH = 32, MAX_NODES = 1024, PATH_THREADS = 1024;
+typedef LogitPiece<THREADS, EACH> Piece;
+
+template <int WIDTH>
+__device__ __forceinline__ void best_of(float& bv, int& bi) {
+#pragma unroll
+    for (int o = WIDTH / 2; o > 0; o >>= 1) {
+        const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
+        const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
+        better(bv, bi, ov, oi);
+    }
+}
 
 // grid (pieces, max_nodes, sequences)
-template <bool WIDE>
 __global__ void __launch_bounds__(THREADS)
 accept_pieces_kernel(const float* logits, int V, const int* cu_q, const int* row_pos, const float* temperature, const uint32_t* seeds,
                      float* ws_val, int* ws_idx) {
@@ -27,46 +40,43 @@ accept_pieces_kernel(const float* logits, int V, const int* cu_q, const int* row
     const int s = blockIdx.z, row = cu_q[s] + blockIdx.y;
     if (row >= cu_q[s + 1]) return;
     const float* z = logits + (size_t)row * V;
-    const int begin = blockIdx.x * CHUNK, end = min(V, begin + CHUNK);
-    auto index = [&](int k) { return WIDE ? begin + ((k / 4) * THREADS + (int)threadIdx.x) * 4 + k % 4 : begin + k * THREADS + (int)threadIdx.x; };
-    float v[EACH];
-    if (WIDE) {
-#pragma unroll
-        for (int k = 0; k < EACH; k += 4)
-            *reinterpret_cast<float4*>(v + k) = index(k) < end ? *reinterpret_cast<const float4*>(z + index(k))
-                                                              : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    } else {
-#pragma unroll
-        for (int k = 0; k < EACH; k++) v[k] = index(k) < end ? z[index(k)] : -INFINITY;
-    }
+    const Piece piece(z, blockIdx.x);
     const int pos = row_pos[row];
     const float temp = temperature[s];
     float bv = -INFINITY;
     int bi = 0x7fffffff;
-    if (pos >= 0) {
-        const float inv_t = temp > 0.f ? 1.f / temp : 1.f;
-        const uint32_t lo = seeds[2 * s], hi = seeds[2 * s + 1];
+    if (!(temp > 0.f)) {
+        float v[EACH];
+        piece.load(z, V, v);
 #pragma unroll
-        for (int k = 0; k < EACH; k++) {
-            const int i = index(k);
-            if (i < end) better(bv, bi, temp > 0.f ? v[k] * inv_t + gumbel(lo, hi, (uint32_t)(pos + 1), (uint32_t)i) : v[k], i);
+        for (int k = 0; k < EACH; k++)
+            if (v[k] > bv) bv = v[k], bi = piece.index(k);             // a thread's own numbers come with rising index
+    } else {
+        const float inv_t = 1.f / temp;
+        const uint32_t lo = seeds[2 * s], hi = seeds[2 * s + 1], mid = lo + (uint32_t)(pos + 1) * 0x85EBCA6Bu;
+#pragma unroll 2
+        for (int q = 0; q < EACH / 4; q++) {
+            const float4 four = piece.four(z, V, q);
+            const float v[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = piece.at(q) + e;
+                const uint32_t x = mix32(mix32(mix32((uint32_t)i ^ 0x9E3779B9u) + mid) ^ hi) >> 8, d = 0xffffffu - x;   // as gumbel() makes them
+                // u is (x + 0.5) / 2^24 to the nearest float32, so 1 - u is d / 2^24 at least; where d is 0, u is 1 and the noise infinite
+                const float most = 0.6931472f * (24.f - __log2f((float)d)) + 1e-3f;
+                if (d == 0 || v[e] * inv_t + most >= bv) better(bv, bi, v[e] * inv_t + gumbel(lo, hi, (uint32_t)(pos + 1), (uint32_t)i), i);
+            }
         }
     }
-    auto reduce = [&](int lanes) {
-        for (int o = lanes / 2; o > 0; o >>= 1) {
-            const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-            const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-            better(bv, bi, ov, oi);
-        }
-    };
+    if (pos < 0) bv = -INFINITY;                                       // a padding row
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    reduce(32);
+    best_of<32>(bv, bi);
     if (lane == 0) sv[w] = bv, si[w] = bi;
     __syncthreads();
     if (w == 0) {
         bv = lane < THREADS / 32 ? sv[lane] : -INFINITY;
         bi = lane < THREADS / 32 ? si[lane] : 0x7fffffff;
-        reduce(THREADS / 32);
+        best_of<THREADS / 32>(bv, bi);
         if (lane == 0) {
             const size_t at = (size_t)row * gridDim.x + blockIdx.x;
             ws_val[at] = bv, ws_idx[at] = bi;
@@ -75,7 +85,7 @@ accept_pieces_kernel(const float* logits, int V, const int* cu_q, const int* row
 }
 
 // grid (sequences)
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(PATH_THREADS)
 accept_path_kernel(const float* ws_val, const int* ws_idx, int pieces, const int* cu_q, const int* tok, const int* parent, int max_nodes,
                    int* path, int* n_path, int* next_tok) {
     __shared__ int choice[MAX_NODES], toks[MAX_NODES], up[MAX_NODES];
@@ -83,19 +93,14 @@ accept_path_kernel(const float* ws_val, const int* ws_idx, int pieces, const int
     pdl_launch_dependents();
     const int s = blockIdx.x, row0 = cu_q[s], n = min(max_nodes, cu_q[s + 1] - row0);
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    for (int i = threadIdx.x; i < n; i += THREADS) toks[i] = tok[row0 + i], up[i] = parent[row0 + i];
-    for (int i = w; i < n; i += THREADS / 32) {
+    for (int i = threadIdx.x; i < n; i += PATH_THREADS) toks[i] = tok[row0 + i], up[i] = parent[row0 + i];
+    for (int i = w; i < n; i += PATH_THREADS / 32) {
         float bv = -INFINITY;
         int bi = 0x7fffffff;
         const size_t at = (size_t)(row0 + i) * pieces;
         for (int c = lane; c < pieces; c += 32) better(bv, bi, ws_val[at + c], ws_idx[at + c]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-            const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-            better(bv, bi, ov, oi);
-        }
-        if (lane == 0) choice[i] = bi == 0x7fffffff ? 0 : bi;
+        best_of<32>(bv, bi);
+        if (lane == 0) choice[i] = bv == -INFINITY ? 0 : bi;
     }
     __syncthreads();
     if (w != 0) return;
@@ -123,7 +128,7 @@ accept_path_kernel(const float* ws_val, const int* ws_idx, int pieces, const int
 
 }  // namespace
 
-DK_EXPORT int dk_tree_accept_pieces(int V) { return (V + CHUNK - 1) / CHUNK; }
+DK_EXPORT int dk_tree_accept_pieces(int V) { return logit_pieces(V, Piece::SIZE); }
 
 // logits [rows, V] float32; temperature [n_seq], seeds [n_seq][2]; ws_val, ws_idx: rows * dk_tree_accept_pieces(V) elements;
 // path [n_seq, max_nodes], n_path [n_seq], next_tok [n_seq].
@@ -132,10 +137,10 @@ DK_EXPORT int dk_tree_accept(const float* logits, int V, const int* tok, const i
                              int* path, int* n_path, int* next_tok, cudaStream_t st) {
     if (V < 1 || max_nodes < 1 || max_nodes > MAX_NODES || n_seq < 1 || n_seq > 65535) return (int)cudaErrorInvalidValue;
     const int pieces = dk_tree_accept_pieces(V);
-    const bool wide = V % 4 == 0 && ((uintptr_t)logits & 15) == 0;      // rows on 16-byte boundaries: 16 bytes a load
-    int e = dk_launch(wide ? accept_pieces_kernel<true> : accept_pieces_kernel<false>, dim3(pieces, max_nodes, n_seq), dim3(THREADS), 0, st,
-                      logits, V, cu_q, row_pos, temperature, seeds, ws_val, ws_idx);
+    int e = dk_launch(accept_pieces_kernel, dim3(pieces, max_nodes, n_seq), dim3(THREADS), 0, st, logits, V, cu_q, row_pos, temperature, seeds,
+                      ws_val, ws_idx);
     if (e) return e;
-    return dk_launch(accept_path_kernel, dim3(n_seq), dim3(THREADS), 0, st, (const float*)ws_val, (const int*)ws_idx, pieces, cu_q, tok,
-                     parent, max_nodes, path, n_path, next_tok);
+    // (may start under the end of the first: it reads nothing before)
+    return dk_launch_as(true, accept_path_kernel, dim3(n_seq), dim3(PATH_THREADS), 0, st, (const float*)ws_val, (const int*)ws_idx, pieces, cu_q,
+                        tok, parent, max_nodes, path, n_path, next_tok);
 }
