@@ -2284,7 +2284,7 @@ def tree_accept(logits, tok, parent, cu_q, row_pos, temperature, seeds, path, n_
                               (seeds, "seeds", torch.int32, (n_seq, 2)), (path, "path", torch.int32, (n_seq, max_nodes)),
                               (n_path, "n_path", torch.int32, (n_seq,)), (next_tok, "next_tok", torch.int32, (n_seq,))))
     lib = _lib("tree_accept.cu")
-    n = max(1, rows * lib.dk_tree_accept_pieces(V))
+    n = max(1, rows * lib.dk_tree_accept_pieces(V, n_seq, max_nodes))
     ws = torch.empty(2 * n, dtype=torch.int32, device=logits.device)
     _check(lib, lib.dk_tree_accept(_p(logits), V, _p(tok), _p(parent), _p(cu_q), _p(row_pos), _p(temperature), _p(seeds), n_seq, max_nodes,
                                    _p(ws), c_void_p(ws.data_ptr() + 4 * n), _p(path), _p(n_path), _p(next_tok), _stream()), "tree_accept", 2)

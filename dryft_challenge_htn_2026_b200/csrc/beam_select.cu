@@ -13,9 +13,9 @@
 //
 // First launch, a block a piece of 8,192 logits of a row, which stay in registers. A floor under the `best`-th largest: of each warp
 // the best / 8-th largest of its threads' own maxima, the least of these; few logits beside the ones looked for reach it, and these
-// are ranked by counting. Where many do (a warp without large ones), the exact `best`-th largest of the threads' maxima takes its
-// place, above which `best` threads have all there is. (That one alone, 256 comparisons a thread, took two thirds of the kernel's
-// time: 47 us for 128 rows of 100,003.) Second launch, a block a request: the same over the pieces' lists, which are in order. Bound
+// are ranked by counting. Where many do (equal logits, a warp without large ones), the exact `best`-th largest of the threads' maxima
+// takes its place, above which `best` threads have all there is. (That one alone, 256 comparisons a thread, took two thirds of the
+// kernel's time: 47 us for 128 rows of 100,003.) Second launch, a block a request: the same over the pieces' lists, which are in order. Bound
 // by reading the logits where there are many rows, by the two launches' latency where there are few.
 #include "logit_rows.cuh"
 
@@ -31,18 +31,24 @@ __device__ __forceinline__ uint32_t order_of(float v) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ uint64_t key_of(float v, int i) { return isfinite(v) ? (uint64_t)order_of(v) << 32 | (uint32_t)~i : 0; }
-__device__ __forceinline__ float logit_of(uint64_t key) {
-    const uint32_t b = (uint32_t)(key >> 32);
-    return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
-}
+__device__ __forceinline__ float value_of_order(uint32_t b) { return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b); }
+__device__ __forceinline__ float logit_of(uint64_t key) { return value_of_order((uint32_t)(key >> 32)); }
 __device__ __forceinline__ int index_of(uint64_t key) { return (int)~(uint32_t)key; }
+
+constexpr float LOG2E = 1.4426950408889634f;
+// 2^x, one instruction (-infinity gives 0)
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // grid (pieces, rows). ws_key [rows][pieces][best] in falling order (0: none), ws_sum [rows][pieces] = (maximum, sum).
 __global__ void __launch_bounds__(THREADS)
 beam_pieces_kernel(const float* logits, int V, int best, uint64_t* ws_key, double2* ws_sum) {
-    __shared__ uint64_t tops[THREADS], floors[WARPS], exact_floor;
+    __shared__ uint64_t tops[THREADS], exact_floor;
     __shared__ uint64_t found[MAX_BEST * EACH];
-    __shared__ float red_m[WARPS];
+    __shared__ float red_m[WARPS], floors[WARPS];
     __shared__ double red_s[WARPS];
     __shared__ int count;
     pdl_wait();
@@ -52,78 +58,82 @@ beam_pieces_kernel(const float* logits, int V, int best, uint64_t* ws_key, doubl
     const Piece piece(z, blockIdx.x);
     float v[EACH];
     piece.load(z, V, v);
-    if (t == 0) count = 0, exact_floor = 1;
-    float m = -INFINITY;
+    uint32_t bits = 0;                                                   // the thread's logits that reach the floor
+    for (bool again = false;; again = true) {
+        if (t == 0) count = 0, exact_floor = 1;
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int k = 0; k < EACH; k++) {
-        if (!isfinite(v[k])) v[k] = -INFINITY;
-        m = fmaxf(m, v[k]);
-    }
-    int at = 0;
-#pragma unroll
-    for (int k = EACH - 1; k >= 0; k--)
-        if (v[k] == m) at = piece.index(k);                              // the lowest index of the thread's maximum
-    const uint64_t top = key_of(m, at);
-    tops[t] = top;
-    // the warp's floor: its threads' maxima, largest first
-    uint64_t least = ~0ull;
-    uint32_t left = (uint32_t)(top >> 32);
-    for (int r = 0; r < (best + WARPS - 1) / WARPS; r++) {
-        const uint32_t high = __reduce_max_sync(0xffffffffu, left);
-        const int who = __ffs(__ballot_sync(0xffffffffu, left == high)) - 1;
-        const uint64_t key = high ? __shfl_sync(0xffffffffu, top, who) : 0;
-        least = key < least ? key : least;
-        if (lane == who) left = 0;
-    }
-    float wm = m;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
-    if (lane == 0) red_m[w] = wm, floors[w] = least;
-    __syncthreads();
-    float bm = red_m[0];
-    uint64_t floor_key = floors[0];
-#pragma unroll
-    for (int i = 1; i < WARPS; i++) bm = fmaxf(bm, red_m[i]), floor_key = floors[i] < floor_key ? floors[i] : floor_key;
-    floor_key = floor_key ? floor_key : 1;
-    int mine = 0;
-    if (top >= floor_key) {
-        const float low = logit_of(floor_key);
-#pragma unroll
-        for (int k = 0; k < EACH; k++) mine += floor_key == 1 ? v[k] != -INFINITY : v[k] >= low;
-    }
-    if (mine) atomicAdd(&count, mine);                                   // an upper bound of what is to be ranked
-    float sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < EACH; k++) sum += v[k] == -INFINITY ? 0.f : expf(v[k] - bm);
-    double total = sum;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (lane == 0) red_s[w] = total;
-    __syncthreads();
-    if (t == 0) {
-        total = 0.;
-        for (int i = 0; i < WARPS; i++) total += red_s[i];
-        ws_sum[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = make_double2((double)bm, total);
-    }
-    if (count > ROOM) {
-        int above = 0;
-#pragma unroll 4
-        for (int i = 0; i < THREADS; i++) above += tops[i] > top;
-        if (top != 0 && above == best - 1) exact_floor = top;
+        for (int k = 0; k < EACH; k++) m4[k & 3] = fmaxf(m4[k & 3], v[k]);
+        const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        // the warp's largest, and its floor: its threads' largest ones, one after the other
+        uint32_t left = order_of(top), high = 0;
+        float wm = 0.f;
+        for (int r = 0; r < (best + WARPS - 1) / WARPS; r++) {
+            high = __reduce_max_sync(0xffffffffu, left);
+            if (r == 0) wm = value_of_order(high);
+            if (lane == __ffs(__ballot_sync(0xffffffffu, left == high)) - 1) left = 0;
+        }
+        if (lane == 0) red_m[w] = wm, floors[w] = high ? value_of_order(high) : -INFINITY;
         __syncthreads();
-        floor_key = exact_floor;
+        float bm = red_m[0], low = floors[0];
+#pragma unroll
+        for (int i = 1; i < WARPS; i++) bm = fmaxf(bm, red_m[i]), low = fminf(low, floors[i]);
+        low = fmaxf(low, -3.402823466e38f);                             // -infinity is no candidate
+        auto reach = [&](float least) {
+            uint32_t b = 0;
+#pragma unroll
+            for (int k = 0; k < EACH; k++) b |= v[k] >= least ? 1u << k : 0u;
+            return b;
+        };
+        bits = top >= low ? reach(low) : 0;
+        if (bits) atomicAdd(&count, __popc(bits));
+        float sum = 0.f;
+        const float shift = -bm * LOG2E;
+        if (bm > -INFINITY)
+#pragma unroll
+            for (int k = 0; k < EACH; k++) sum += ex2(fmaf(v[k], LOG2E, shift));
+        double total = sum;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        if (lane == 0) red_s[w] = total;
+        __syncthreads();
+        total = 0.;
+#pragma unroll
+        for (int i = 0; i < WARPS; i++) total += red_s[i];
+        // an infinite logit, or one that is none, shows in the sum: once more without it
+        if (!again && !(total < INFINITY)) {
+#pragma unroll
+            for (int k = 0; k < EACH; k++)
+                if (!(fabsf(v[k]) < INFINITY)) v[k] = -INFINITY;
+            __syncthreads();
+            continue;
+        }
+        if (t == 0) ws_sum[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = make_double2((double)bm, total);
+        if (count > ROOM) {                                              // the best-th largest of the threads' largest, each the first of its kind
+            int at = 0;
+#pragma unroll
+            for (int k = EACH - 1; k >= 0; k--)
+                if (v[k] == top) at = k;
+            const uint64_t key = key_of(top, piece.index(at));
+            tops[t] = key;
+            __syncthreads();
+            int above = 0;
+#pragma unroll 4
+            for (int i = 0; i < THREADS; i++) above += tops[i] > key;
+            if (key != 0 && above == best - 1) exact_floor = key;
+            __syncthreads();
+            bits = key >= exact_floor ? reach(exact_floor == 1 ? low : logit_of(exact_floor)) : 0;
+        }
+        break;
     }
+    const uint64_t floor_key = exact_floor;                              // 1 without the exact one: all that `bits` says
     __syncthreads();
     if (t == 0) count = 0;
     __syncthreads();
-    if (top >= floor_key) {
-        const float low = floor_key == 1 ? -INFINITY : logit_of(floor_key);
-#pragma unroll
-        for (int k = 0; k < EACH; k++)
-            if (v[k] >= low) {
-                const uint64_t key = key_of(v[k], piece.index(k));
-                if (key >= floor_key) found[atomicAdd(&count, 1)] = key;
-            }
+    for (; bits; bits &= bits - 1) {                                     // few have any: they are read again
+        const int i = piece.index(__ffs(bits) - 1);
+        const uint64_t key = key_of(z[i], i);
+        if (key >= floor_key) found[atomicAdd(&count, 1)] = key;
     }
     __syncthreads();
     const int n = count;
@@ -131,6 +141,7 @@ beam_pieces_kernel(const float* logits, int V, int best, uint64_t* ws_key, doubl
     for (int i = t; i < n; i += THREADS) {
         const uint64_t key = found[i];
         int rank = 0;
+#pragma unroll 4
         for (int j = 0; j < n; j++) rank += found[j] > key;
         if (rank < best) out[rank] = key;
     }
@@ -151,7 +162,9 @@ __device__ __forceinline__ double value_of(const Candidate& c) {
     return __longlong_as_double((long long)(c.order >> 63 ? c.order & ~(1ull << 63) : ~c.order));
 }
 
-// grid (requests). Dynamic shared memory: best * best * ceil(lists / THREADS) candidates.
+constexpr int KEYS = 4096;                                              // keys that are brought into shared memory at once, if there are no more
+
+// grid (requests). Dynamic shared memory: best * best * ceil(lists / THREADS) candidates, then the keys where they are KEYS at most.
 __global__ void __launch_bounds__(THREADS)
 beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, int V, int beams, int best, const float* scores,
                    const int* ended, float* scores_out, int* beam_out, int* tok_out) {
@@ -165,17 +178,30 @@ beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, in
     pdl_wait();
     pdl_launch_dependents();
     const int r = blockIdx.x, t = threadIdx.x, lane = t & 31, w = t >> 5;
+    const int lists = beams * pieces;
+    const uint64_t* keys = ws_key + (size_t)r * lists * best;
+    if (lists * best <= KEYS) {
+        uint64_t* here = reinterpret_cast<uint64_t*>(found + best * best * ((lists + THREADS - 1) / THREADS));
+#pragma unroll 8
+        for (int i = t; i < lists * best; i += THREADS) here[i] = keys[i];
+        keys = here;
+    }
     for (int b = w; b < beams; b += WARPS) {
         const double2* part = ws_sum + (size_t)(r * beams + b) * pieces;
         const float score = scores[r * beams + b];
         const bool done = ended != nullptr && ended[r * beams + b] != 0;
         double m = -INFINITY, sum = 0.;
-        for (int c = lane; c < pieces; c += 32) m = fmax(m, part[c].x);
+        for (int c0 = 0; c0 < pieces; c0 += 32) {                        // 32 pieces at a time, one after the other into (m, sum)
+            const double2 p = c0 + lane < pieces ? part[c0 + lane] : make_double2(-INFINITY, 0.);
+            double top = p.x;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-        for (int c = lane; c < pieces; c += 32) sum += part[c].y > 0. ? part[c].y * exp(part[c].x - m) : 0.;
+            for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const double mn = fmax(m, top);
+            double add = p.y > 0. ? p.y * exp(p.x - mn) : 0.;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            for (int o = 16; o > 0; o >>= 1) add += __shfl_xor_sync(0xffffffffu, add, o);
+            sum = (sum > 0. ? sum * exp(m - mn) : 0.) + add, m = mn;
+        }
         if (lane == 0) {
             kind[b] = !isfinite(score) ? 0 : done ? 2 : sum > 0. ? 1 : 0;
             offset[b] = kind[b] == 1 ? (double)score - (m + log(sum)) : (double)score;
@@ -184,11 +210,10 @@ beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, in
     if (t == 0) count = 0, least = none;
     __syncthreads();
     // list l: piece l % pieces of beam l / pieces, in falling order; a beam at its end has one candidate, in its first list
-    const int lists = beams * pieces;
     auto item = [&](int l, int rank) {
         const int b = l / pieces;
         if (kind[b] == 2) return rank == 0 && l == b * pieces ? candidate(offset[b], b * V) : none;
-        const uint64_t key = kind[b] == 1 ? ws_key[((size_t)r * lists + l) * best + rank] : 0;
+        const uint64_t key = kind[b] == 1 ? keys[l * best + rank] : 0;
         return key ? candidate((double)logit_of(key) + offset[b], b * V + index_of(key)) : none;
     };
     Candidate top = none;
@@ -229,7 +254,8 @@ beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, in
 }
 
 size_t select_smem(int beams, int pieces, int best) {
-    return (size_t)best * best * ((beams * pieces + THREADS - 1) / THREADS) * sizeof(Candidate);
+    const long long lists = (long long)beams * pieces;
+    return (size_t)(best * best * ((lists + THREADS - 1) / THREADS)) * sizeof(Candidate) + (lists * best <= KEYS ? (size_t)(lists * best) * 8 : 0);
 }
 
 }  // namespace

@@ -14,19 +14,27 @@ struct LogitPiece {
     }
     __device__ __forceinline__ int at(int q) const { return first + q * THREADS * 4; }
     __device__ __forceinline__ int index(int k) const { return at(k / 4) + k % 4; }
+    // whether all of the block's piece is the row's
+    __device__ __forceinline__ bool inside(int V) const {
+        const int begin = first - (int)threadIdx.x * 4;
+        return begin >= 0 && begin + SIZE <= V;
+    }
+    __device__ __forceinline__ float one(const float* z, int V, int i) const { return i >= 0 && i < V ? z[i] : -INFINITY; }
     __device__ __forceinline__ float4 four(const float* z, int V, int q) const {
         const int i = at(q);
         if (i >= 0 && i + 4 <= V) return *reinterpret_cast<const float4*>(z + i);
-        float4 x;
-        x.x = i >= 0 && i < V ? z[i] : -INFINITY, x.y = i + 1 >= 0 && i + 1 < V ? z[i + 1] : -INFINITY;
-        x.z = i + 2 >= 0 && i + 2 < V ? z[i + 2] : -INFINITY, x.w = i + 3 >= 0 && i + 3 < V ? z[i + 3] : -INFINITY;
-        return x;
+        return make_float4(one(z, V, i), one(z, V, i + 1), one(z, V, i + 2), one(z, V, i + 3));
     }
     __device__ __forceinline__ void load(const float* z, int V, float (&v)[EACH]) const {
+        if (inside(V)) {
 #pragma unroll
-        for (int q = 0; q < EACH / 4; q++) {
-            const float4 x = four(z, V, q);
-            v[4 * q] = x.x, v[4 * q + 1] = x.y, v[4 * q + 2] = x.z, v[4 * q + 3] = x.w;
+            for (int q = 0; q < EACH / 4; q++) {
+                const float4 x = *reinterpret_cast<const float4*>(z + at(q));
+                v[4 * q] = x.x, v[4 * q + 1] = x.y, v[4 * q + 2] = x.z, v[4 * q + 3] = x.w;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < EACH; k++) v[k] = one(z, V, index(k));
         }
     }
 };

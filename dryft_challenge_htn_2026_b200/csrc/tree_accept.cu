@@ -7,7 +7,7 @@
 // how many steps they take, not which they are. From node 0 on the path goes to the child that holds the chosen token (the lowest
 // one, if several do) until there is none; the token chosen there is the sequence's next.
 //
-// Two launches: the best token of each piece of 8,192 logits, over all nodes and pieces side by side (one pass over the logits: bound
+// Two launches: the best token of each piece of 8,192 (or 2,048) logits, over all nodes and pieces side by side (one pass over the logits: bound
 // by reading them where the choice is greedy); then a block a sequence puts the pieces together and walks the path. Drawing costs a
 // hash and two logarithms a logit. Most logits are spared the logarithms: -log(u) >= 1 - u, so the noise is at most -log(1 - u), and
 // what does not reach the thread's best so far with that much cannot win.
@@ -16,8 +16,7 @@
 
 namespace {
 
-constexpr int THREADS = 256, EACH = 32, MAX_NODES = 1024, PATH_THREADS = 1024;
-typedef LogitPiece<THREADS, EACH> Piece;
+constexpr int THREADS = 256, MAX_NODES = 1024, PATH_THREADS = 1024;
 
 template <int WIDTH>
 __device__ __forceinline__ void best_of(float& bv, int& bi) {
@@ -29,7 +28,8 @@ __device__ __forceinline__ void best_of(float& bv, int& bi) {
     }
 }
 
-// grid (pieces, max_nodes, sequences)
+// grid (pieces, max_nodes, sequences); EACH: logits a thread
+template <int EACH>
 __global__ void __launch_bounds__(THREADS)
 accept_pieces_kernel(const float* logits, int V, const int* cu_q, const int* row_pos, const float* temperature, const uint32_t* seeds,
                      float* ws_val, int* ws_idx) {
@@ -40,7 +40,7 @@ accept_pieces_kernel(const float* logits, int V, const int* cu_q, const int* row
     const int s = blockIdx.z, row = cu_q[s] + blockIdx.y;
     if (row >= cu_q[s + 1]) return;
     const float* z = logits + (size_t)row * V;
-    const Piece piece(z, blockIdx.x);
+    const LogitPiece<THREADS, EACH> piece(z, blockIdx.x);
     const int pos = row_pos[row];
     const float temp = temperature[s];
     float bv = -INFINITY;
@@ -128,17 +128,29 @@ accept_path_kernel(const float* ws_val, const int* ws_idx, int pieces, const int
 
 }  // namespace
 
-DK_EXPORT int dk_tree_accept_pieces(int V) { return logit_pieces(V, Piece::SIZE); }
+// Logits a thread of the first launch takes: 32, or 8 where that leaves SMs without a block, as with a handful of nodes (5 nodes of
+// 151,936, drawn: 13.5 us with 32, 8.5 with 16).
+static int each_for(int V, long long rows) {
+    static int sms = 0;
+    if (sms == 0) {
+        int dev = 0;
+        cudaGetDevice(&dev);
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    }
+    return rows * logit_pieces(V, 32 * THREADS) >= 4 * sms ? 32 : 8;
+}
 
-// logits [rows, V] float32; temperature [n_seq], seeds [n_seq][2]; ws_val, ws_idx: rows * dk_tree_accept_pieces(V) elements;
+DK_EXPORT int dk_tree_accept_pieces(int V, int n_seq, int max_nodes) { return logit_pieces(V, each_for(V, (long long)n_seq * max_nodes) * THREADS); }
+
+// logits [rows, V] float32; temperature [n_seq], seeds [n_seq][2]; ws_val, ws_idx: rows * dk_tree_accept_pieces elements;
 // path [n_seq, max_nodes], n_path [n_seq], next_tok [n_seq].
 DK_EXPORT int dk_tree_accept(const float* logits, int V, const int* tok, const int* parent, const int* cu_q, const int* row_pos,
                              const float* temperature, const uint32_t* seeds, int n_seq, int max_nodes, float* ws_val, int* ws_idx,
                              int* path, int* n_path, int* next_tok, cudaStream_t st) {
     if (V < 1 || max_nodes < 1 || max_nodes > MAX_NODES || n_seq < 1 || n_seq > 65535) return (int)cudaErrorInvalidValue;
-    const int pieces = dk_tree_accept_pieces(V);
-    int e = dk_launch(accept_pieces_kernel, dim3(pieces, max_nodes, n_seq), dim3(THREADS), 0, st, logits, V, cu_q, row_pos, temperature, seeds,
-                      ws_val, ws_idx);
+    const int each = each_for(V, (long long)n_seq * max_nodes), pieces = logit_pieces(V, each * THREADS);
+    int e = dk_launch(each == 8 ? accept_pieces_kernel<8> : accept_pieces_kernel<32>, dim3(pieces, max_nodes, n_seq), dim3(THREADS), 0, st, logits,
+                      V, cu_q, row_pos, temperature, seeds, ws_val, ws_idx);
     if (e) return e;
     // (may start under the end of the first: it reads nothing before)
     return dk_launch_as(true, accept_path_kernel, dim3(n_seq), dim3(PATH_THREADS), 0, st, (const float*)ws_val, (const int*)ws_idx, pieces, cu_q,
