@@ -152,7 +152,8 @@ beam_pieces_kernel(const float* logits, int V, int best, uint64_t* ws_key, doubl
 struct Candidate {
     uint64_t order;
     int flat;
-    __device__ __forceinline__ bool before(const Candidate& o) const { return order > o.order || (order == o.order && (unsigned)flat < (unsigned)o.flat); }
+    // (without a branch: with two of them a comparison in the loops below took a hundred clocks)
+    __device__ __forceinline__ bool before(const Candidate& o) const { return (order > o.order) | ((order == o.order) & ((unsigned)flat < (unsigned)o.flat)); }
 };
 __device__ __forceinline__ Candidate candidate(double value, int flat) {
     const uint64_t b = (uint64_t)__double_as_longlong(value + 0.);
@@ -225,7 +226,7 @@ beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, in
     __syncthreads();
     int above = 0;
     const int n_tops = min(THREADS, lists);
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < n_tops; i++) above += tops[i].before(top);
     if (top.flat >= 0 && above == best - 1) least = top;                 // the best-th largest of the threads' largest
     __syncthreads();
@@ -242,6 +243,7 @@ beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, in
     for (int i = t; i < n; i += THREADS) {
         const Candidate c = found[i];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < n; j++) rank += found[j].before(c);
         if (rank < best) {
             scores_out[(size_t)r * best + rank] = (float)value_of(c);
