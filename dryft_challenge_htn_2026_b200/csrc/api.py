@@ -77,10 +77,11 @@ def _lib(source, defines=None):
         if not torch.cuda.is_available():
             raise KernelError("no CUDA device: the kernels of this library run on an NVIDIA B200 (sm_100a) only")
         _cuda_seen = True
-    key = (source, tuple(sorted((defines or {}).items())))
-    fresh = key not in build._libs
-    lib = build.load_lib(source, defines)
+    key = (source, tuple(sorted(defines.items())) if defines else ())
+    lib = build._libs.get(key)
+    fresh = lib is None
     if fresh:
+        lib = build.load_lib(source, defines)
         lib.dk_set_pdl.argtypes = lib.dk_set_thread_pdl.argtypes = [c_int]
         lib.dk_set_pdl(int(bool(_pdl)))
         lib.dk_error_string.restype = ctypes.c_char_p
@@ -2181,6 +2182,22 @@ def matrix_memory(q, k, v, gate, i_rows, f_rows, i_bias, f_bias, cap, states, we
 
 
 # ------------------------------------------------------- branches: trees of drafted tokens, beams
+_KINDS = {"p": c_void_p, "i": c_int, "q": c_longlong, "f": c_float}
+
+
+def _entry(lib, name, kinds):
+    """An entry point that takes plain numbers: ``kinds`` has a letter an argument (p: address, i, q: whole numbers of 32 and 64 bits, f:
+    float32). Without its types every argument would be wrapped in Python, a third of what a call of twenty costs."""
+    f = getattr(lib, name)
+    if f.argtypes is None:
+        f.argtypes = [_KINDS[k] for k in kinds]
+    return f
+
+
+def _at(t):
+    return 0 if t is None else t.data_ptr()
+
+
 TREE_MAX_NODES = 1024       # nodes of one sequence's tree
 TREE_MAX_GROUP = 64         # query heads a kv head
 MAX_BEAMS, MAX_BEST = 32, 64
@@ -2205,12 +2222,12 @@ def _need_counts(what, n_seq, max_nodes):
 
 @functools.lru_cache(maxsize=None)
 def _tree_plan(head_dim, f32, max_nodes, group):
-    """(whether the tensor-core kernel takes it, blocks of a launch, rows of a tile)."""
+    """(whether the tensor-core kernel takes it, blocks of a launch, rows of a tile, pages of a table up to which tiles are not split)."""
     if not f32 and head_dim in TC_ATTENTION_HEAD_DIMS:
         lib = _lib("attention_tree_tc.cu", {"HD": head_dim})
-        return True, sm_count(), lib.dk_tree_tc_tile_rows()
+        return True, sm_count(), lib.dk_tree_tc_tile_rows(), lib.dk_tree_tc_whole_pages()
     lib = _lib("attention_tree.cu", {"HD": head_dim})
-    return False, lib.dk_attn_tree_blocks(f32, max_nodes, group), lib.dk_tree_tile_rows(max_nodes, group)
+    return False, lib.dk_attn_tree_blocks(f32, max_nodes, group), lib.dk_tree_tile_rows(max_nodes, group), lib.dk_tree_whole_pages()
 
 
 def attention_tree(q, out, k_store, v_store, cu_q, seq_pos0, row_pos, tree, page_table, n_heads, n_kv_heads, head_dim, window, scale,
@@ -2250,21 +2267,22 @@ def attention_tree(q, out, k_store, v_store, cu_q, seq_pos0, row_pos, tree, page
     if rows == 0:
         return
     f32 = int(q.dtype == torch.float32)
-    tc, blocks, tile = _tree_plan(head_dim, f32, max_nodes, n_heads // n_kv_heads)
-    n = 2 * blocks * tile * head_dim
-    ws = torch.empty(n + 4 * blocks * tile, dtype=torch.float32, device=q.device)
-    head = (_p(q), c_longlong(q.stride(0)), _p(out), c_longlong(out.stride(0)))
-    body = (_p(k_store), _p(v_store), n_pages, _p(cu_q), _p(seq_pos0), _p(row_pos), _p(tree), words, _p(page_table), table, n_seq, n_heads,
-            n_kv_heads, int(window or 0), c_float(scale), max_nodes, _p(ws), c_void_p(ws.data_ptr() + 4 * n), blocks)
+    tc, blocks, tile, whole = _tree_plan(head_dim, f32, max_nodes, n_heads // n_kv_heads)
+    n = 0 if whole and table <= whole else 2 * blocks * tile * head_dim          # tiles of a few pages are not split: no parts
+    ws = q.new_empty(n + 4 * blocks * tile, dtype=torch.float32) if n else None
+    parts = _at(ws)
+    head = (q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0))
+    body = (k_store.data_ptr(), v_store.data_ptr(), n_pages, cu_q.data_ptr(), seq_pos0.data_ptr(), row_pos.data_ptr(), tree.data_ptr(), words,
+            page_table.data_ptr(), table, n_seq, n_heads, n_kv_heads, window or 0, scale, max_nodes, parts, parts + 4 * n, blocks)
     if tc:
         if _tc_err is None:
             _tc_err = torch.zeros(1, dtype=torch.int32, device=q.device)
         lib = _lib("attention_tree_tc.cu", {"HD": head_dim})
-        err = lib.dk_attn_tree_tc(*head, c_longlong(rows), *body, _p(_tc_err), _stream())
+        err = _entry(lib, "dk_attn_tree_tc", "pqpqq" + "ppippppipiiiiifippi" + "pp")(*head, rows, *body, _tc_err.data_ptr(), _stream_ptr())
     else:
         lib = _lib("attention_tree.cu", {"HD": head_dim})
-        err = lib.dk_attn_tree(f32, *head, *body, _stream())
-    _check(lib, err, "attention_tree", 2)
+        err = _entry(lib, "dk_attn_tree", "ipqpq" + "ppippppipiiiiifippi" + "p")(f32, *head, *body, _stream_ptr())
+    _check(lib, err, "attention_tree", 2 if n else 1)
 
 
 def tree_accept(logits, tok, parent, cu_q, row_pos, temperature, seeds, path, n_path, next_tok):
@@ -2285,9 +2303,10 @@ def tree_accept(logits, tok, parent, cu_q, row_pos, temperature, seeds, path, n_
                               (n_path, "n_path", torch.int32, (n_seq,)), (next_tok, "next_tok", torch.int32, (n_seq,))))
     lib = _lib("tree_accept.cu")
     n = max(1, rows * lib.dk_tree_accept_pieces(V, n_seq, max_nodes))
-    ws = torch.empty(2 * n, dtype=torch.int32, device=logits.device)
-    _check(lib, lib.dk_tree_accept(_p(logits), V, _p(tok), _p(parent), _p(cu_q), _p(row_pos), _p(temperature), _p(seeds), n_seq, max_nodes,
-                                   _p(ws), c_void_p(ws.data_ptr() + 4 * n), _p(path), _p(n_path), _p(next_tok), _stream()), "tree_accept", 2)
+    ws = tok.new_empty(2 * n).data_ptr()
+    _check(lib, _entry(lib, "dk_tree_accept", "pi" + "p" * 6 + "ii" + "p" * 6)(
+        logits.data_ptr(), V, tok.data_ptr(), parent.data_ptr(), cu_q.data_ptr(), row_pos.data_ptr(), temperature.data_ptr(), seeds.data_ptr(),
+        n_seq, max_nodes, ws, ws + 4 * n, path.data_ptr(), n_path.data_ptr(), next_tok.data_ptr(), _stream_ptr()), "tree_accept", 2)
 
 
 def beam_select(logits, scores, ended, scores_out, beam_out, tok_out):
@@ -2313,9 +2332,10 @@ def beam_select(logits, scores, ended, scores_out, beam_out, tok_out):
     if not lib.dk_beam_select_takes(V, beams, best):
         raise KernelError(f"beam_select: {best} of {beams} beams over {V} tokens need more shared memory than a block has")
     n = requests * beams * pieces
-    ws = torch.empty(n * (best + 2), dtype=torch.int64, device=logits.device)      # pairs of doubles first, then the keys
-    _check(lib, lib.dk_beam_select(_p(logits), V, requests, beams, best, _p(scores), _p(ended), c_void_p(ws.data_ptr() + 16 * n), _p(ws), _p(scores_out),
-                                   _p(beam_out), _p(tok_out), _stream()), "beam_select", 2)
+    ws = scores.new_empty(2 * n * (best + 2)).data_ptr()                  # pairs of doubles first, then the keys: 8 bytes each
+    _check(lib, _entry(lib, "dk_beam_select", "piiii" + "p" * 8)(
+        logits.data_ptr(), V, requests, beams, best, scores.data_ptr(), _at(ended), ws + 16 * n, ws, scores_out.data_ptr(), beam_out.data_ptr(),
+        tok_out.data_ptr(), _stream_ptr()), "beam_select", 2)
 
 
 def _need_store(store, page_table, what):
@@ -2344,8 +2364,9 @@ def kv_keep(store, page_table, seq_pos0, path, n_path):
     _need_all("kv_keep", ((page_table, "page_table", torch.int32, (n_seq, page_table.shape[1])), (seq_pos0, "seq_pos0", torch.int32, (n_seq,)),
                           (path, "path", torch.int32, (n_seq, width)), (n_path, "n_path", torch.int32, (n_seq,))))
     lib = _lib("cache_moves.cu")
-    _check(lib, lib.dk_kv_keep(_p(store), outer, pages, nkv, c_longlong(row), _p(page_table), page_table.shape[1], n_seq, _p(seq_pos0),
-                               _p(path), width, _p(n_path), _stream()), "kv_keep")
+    _check(lib, _entry(lib, "dk_kv_keep", "piiiqpiippipp")(
+        store.data_ptr(), outer, pages, nkv, row, page_table.data_ptr(), page_table.shape[1], n_seq, seq_pos0.data_ptr(), path.data_ptr(), width,
+        n_path.data_ptr(), _stream_ptr()), "kv_keep")
 
 
 def _beams(parent, what):
@@ -2366,8 +2387,9 @@ def kv_reorder(store, page_table, parent, first, last):
     _need_all("kv_reorder", ((page_table, "page_table", torch.int32, (requests * beams, page_table.shape[1])), (parent, "parent", torch.int32,
               (requests, beams)), (first, "first", torch.int32, (requests,)), (last, "last", torch.int32, (requests,))))
     lib = _lib("cache_moves.cu")
-    _check(lib, lib.dk_kv_reorder(_p(store), outer, pages, nkv, c_longlong(row), _p(page_table), page_table.shape[1], requests, beams,
-                                  _p(parent), _p(first), _p(last), _stream()), "kv_reorder")
+    _check(lib, _entry(lib, "dk_kv_reorder", "piiiqpiiipppp")(
+        store.data_ptr(), outer, pages, nkv, row, page_table.data_ptr(), page_table.shape[1], requests, beams, parent.data_ptr(), first.data_ptr(),
+        last.data_ptr(), _stream_ptr()), "kv_reorder")
 
 
 def state_reorder(store, seq_slot, parent):
@@ -2382,5 +2404,6 @@ def state_reorder(store, seq_slot, parent):
     if size % 2 or store.data_ptr() % 2 or store.get_device() != torch.cuda.current_device():
         raise KernelError(f"state_reorder: states of {size} bytes, which must be even, or a store on another device")
     lib = _lib("cache_moves.cu")
-    _check(lib, lib.dk_state_reorder(_p(store), store.shape[0], store.shape[1], c_longlong(size), _p(seq_slot), requests, beams, _p(parent),
-                                     _stream()), "state_reorder")
+    _check(lib, _entry(lib, "dk_state_reorder", "piiqpiipp")(
+        store.data_ptr(), store.shape[0], store.shape[1], size, seq_slot.data_ptr(), requests, beams, parent.data_ptr(), _stream_ptr()),
+        "state_reorder")

@@ -15,6 +15,7 @@ static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multip
 
 namespace {
 
+constexpr int WHOLE_PAGES = 1;                    // tables up to here are not split (see attention_tree.cuh)
 constexpr int THREADS = 256, LDK = HD + 4, LDP = DK_PAGE + 4, CV = HD / 16;
 
 __device__ __forceinline__ void load4(float* dst, const float* src) { *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(src); }
@@ -174,12 +175,10 @@ constexpr size_t tree_smem() {
 template <typename T, int NI>
 int launch(const TreeArgs& a, const void* q, long long ldq, void* out, long long ldo, const void* k_store, const void* v_store, float* ws_acc,
            float* ws_ml, int max_nodes, int blocks, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(tree_kernel<T, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tree_smem<NI>());
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        return (int)e;
-    }
-    int r = dk_launch(tree_kernel<T, NI>, dim3(blocks), dim3(THREADS), tree_smem<NI>(), st, a, (const T*)q, ldq, (T*)out, ldo,
+    static SmemOnce once;
+    int r = once.allow((const void*)tree_kernel<T, NI>, tree_smem<NI>());
+    if (r) return r;
+    r = dk_launch(tree_kernel<T, NI>, dim3(blocks), dim3(THREADS), tree_smem<NI>(), st, a, (const T*)q, ldq, (T*)out, ldo,
                       (const T*)k_store, (const T*)v_store, ws_acc, (float2*)ws_ml);
     if (r) return r;
     return tree_merge<T, HD>(a, ws_acc, ws_ml, out, ldo, 16 * NI, max_nodes, blocks, st);
@@ -192,6 +191,8 @@ DK_EXPORT int dk_tree_tile_rows(int max_nodes, int group) {
     const long long rows = (long long)max_nodes * group;
     return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
+
+DK_EXPORT int dk_tree_whole_pages() { return WHOLE_PAGES; }
 
 // Blocks of a launch: as many as the device holds at once.
 DK_EXPORT int dk_attn_tree_blocks(int f32, int max_nodes, int group) {
@@ -218,7 +219,7 @@ DK_EXPORT int dk_attn_tree(int f32, const void* q, long long ldq, void* out, lon
         return (int)cudaErrorInvalidValue;
     const int G = nh / nkv, rows = dk_tree_tile_rows(max_nodes, G);
     TreeArgs a = {cu_q, seq_pos0, row_pos, page_table, tree, n_seq, words, pt_stride, n_pages, nh, nkv, window, rows / G, rows / G, rows,
-                  pt_stride <= 1, 0, scale * 1.4426950408889634f};
+                  pt_stride <= WHOLE_PAGES, 0, scale * 1.4426950408889634f};
     if (!tree_units_fit(a, max_nodes) || nkv > 65535) return (int)cudaErrorInvalidValue;
 #define DK_TREE(T, NI) launch<T, NI>(a, q, ldq, out, ldo, k_store, v_store, ws_acc, ws_ml, max_nodes, blocks, st)
     if (f32) return rows == 16 ? DK_TREE(float, 1) : rows == 32 ? DK_TREE(float, 2) : DK_TREE(float, 4);

@@ -264,6 +264,20 @@ tree_merge_kernel(TreeArgs a, const float* ws_acc, const float2* ws_ml, T* out, 
     }
 }
 
+// A kernel's permission to use more shared memory than usual, asked for once on each device.
+struct SmemOnce {
+    unsigned long long done[4] = {};
+    int allow(const void* kernel, size_t bytes) {
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if (dev >= 0 && dev < 256 && done[dev >> 6] >> (dev & 63) & 1) return 0;
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e != cudaSuccess) return cudaGetLastError(), (int)e;
+        if (dev >= 0 && dev < 256) done[dev >> 6] |= 1ull << (dev & 63);
+        return 0;
+    }
+};
+
 // Launch of the merge, behind the kernel that leaves the parts (it may start under that one's end: it reads nothing before).
 template <typename T, int D>
 static int tree_merge(const TreeArgs& a, const float* ws_acc, const float* ws_ml, void* out, long long ldo, int tile_rows, int max_nodes,

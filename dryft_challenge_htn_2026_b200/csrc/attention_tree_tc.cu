@@ -615,6 +615,7 @@ int make_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dim
 }  // namespace
 
 DK_EXPORT int dk_tree_tc_tile_rows() { return 2 * BM; }
+DK_EXPORT int dk_tree_tc_whole_pages() { return WHOLE_PAGES; }
 
 // q [n_rows, nh*HD] and out, bf16, rows ldq / ldo elements apart (multiples of 8, 16-byte boundaries); k_store, v_store [n_pages, nkv, 64,
 // HD]; ws_acc: 2 * blocks * 256 * HD floats, ws_ml: 2 * blocks * 256 * 2 floats; err: device int for a wait that ran out.
@@ -629,17 +630,15 @@ DK_EXPORT int dk_attn_tree_tc(const void* q, long long ldq, void* out, long long
     TreeArgs a = {cu_q, seq_pos0, row_pos, page_table, tree, n_seq, words, pt_stride, n_pages, nh, nkv, window, 2 * (BM / G), BM / G, BM,
                   pt_stride <= WHOLE_PAGES, EXTRA, scale * 1.4426950408889634f};
     if (!tree_units_fit(a, max_nodes) || nkv > 65535) return (int)cudaErrorInvalidValue;
-    cudaError_t ce = cudaFuncSetAttribute(tree_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
-    if (ce != cudaSuccess) {
-        cudaGetLastError();
-        return (int)ce;
-    }
+    static SmemOnce once;
+    int e = once.allow((const void*)tree_tc_kernel, SMEM_BYTES);
+    if (e) return e;
     CUtensorMap mq, mk, mv;
     const cuuint64_t q_dims[3] = {HD, (cuuint64_t)nh, (cuuint64_t)n_rows}, q_strides[2] = {HD * 2, (cuuint64_t)ldq * 2};
     const cuuint32_t q_box[3] = {64, (cuuint32_t)G, (cuuint32_t)(BM / G)};
     const cuuint64_t kv_dims[2] = {HD, (cuuint64_t)n_pages * nkv * DK_PAGE}, kv_strides[1] = {HD * 2};
     const cuuint32_t kv_box[2] = {64, DK_PAGE};
-    int e = make_map(&mq, q, 3, q_dims, q_strides, q_box);
+    e = make_map(&mq, q, 3, q_dims, q_strides, q_box);
     if (!e) e = make_map(&mk, k_store, 2, kv_dims, kv_strides, kv_box);
     if (!e) e = make_map(&mv, v_store, 2, kv_dims, kv_strides, kv_box);
     if (e) return e;
