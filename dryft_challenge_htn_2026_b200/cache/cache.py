@@ -12,8 +12,10 @@ The reference keeps one dense [B, nkv, cap, hd] pair per layer per batch shape
 """
 from dataclasses import dataclass
 
+import numpy as np
 import torch
 
+from ..csrc import api
 from ..csrc.api import PAGE
 from .pool import CacheFull, PagePool, SlotTable
 from .requests import KVRequest, StateRequest
@@ -97,8 +99,12 @@ class KVGroup:
         self.pool.free([p for p in self.pages.pop(slot) if p >= 0])
         del self.first[slot]
 
+    def stores(self):
+        """The tensors [.., pages, n_kv, PAGE, size] that hold the group's rows."""
+        return [t for t in (self.store, self.v_store) if t is not None]
+
     def bytes(self):
-        return sum(t.numel() * t.element_size() for t in (self.store, self.v_store) if t is not None)
+        return sum(t.numel() * t.element_size() for t in self.stores())
 
 
 class StateGroup:
@@ -196,6 +202,35 @@ class Cache:
         rows = [g.pages[s] for s in slots]
         width = max([min_width] + [len(r) for r in rows])
         return [r + [-1] * (width - len(r)) for r in rows]
+
+    def reorder(self, slots, parents, first=None):
+        """Sequences take the places of others, as the beams of a search do: ``slots[r][b]`` is beam b of request r, and gets the rows
+        from ``first[r]`` on (None: all) and the states of beam ``parents[r][b]`` as they are now. The beams of a request have equal
+        lengths, and rows before ``first[r]`` in common. Moves within the cache, on the current stream."""
+        beams = len(slots[0])
+        flat = [s for row in slots for s in row]
+        if len(set(flat)) != len(flat) or any(len(row) != beams or len(p) != beams for row, p in zip(slots, parents)) or len(slots) != len(parents):
+            raise ValueError("a slot of its own for every beam, and as many beams and parents for every request")
+        if any(not 0 <= q < beams for p in parents for q in p):
+            raise ValueError(f"parents are numbers of the request's {beams} beams")
+        length = [self.length[row[0]] for row in slots]
+        if any(self.length[s] != n for row, n in zip(slots, length) for s in row):
+            raise ValueError("the beams of a request must have equal lengths")
+        if all(list(p) == list(range(beams)) for p in parents):
+            return
+        arrays = [np.array(a, np.int32) for a in (flat, parents, first or [0] * len(slots), length)]
+        arrays += [np.array(self.page_rows(g, flat), np.int32) for g in range(len(self.groups)) if isinstance(self.groups[g], KVGroup)]
+        store = next(g.store for g in self.groups if g.store is not None)
+        dev = torch.from_numpy(np.concatenate([a.reshape(-1) for a in arrays])).to(store.device)
+        dev = [t.view(a.shape) for t, a in zip(dev.split([a.size for a in arrays]), arrays)]
+        tables = iter(dev[4:])
+        for g in self.groups:
+            if isinstance(g, KVGroup):
+                table = next(tables)
+                for t in g.stores():
+                    api.kv_reorder(t, table, dev[1], dev[2], dev[3])
+            else:
+                api.state_reorder(g.store, dev[0], dev[1])
 
     def state_snapshot(self, slots):
         """Copies of the per-sequence states of ``slots`` (every state group), for a caller that runs a

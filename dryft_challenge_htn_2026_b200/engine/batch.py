@@ -26,12 +26,14 @@ class StepContext:
                              attention kernels' query tiles), on the device
     host                     dict of the same arrays as numpy, for parts that plan on the host; None
                              in a captured decode loop, whose positions advance on the device
+    tree                     None, or in a step of trees of drafted tokens a ``TreeRows``
     """
 
     def __init__(self, scratch_store=None):
         self._scratch = scratch_store if scratch_store is not None else {}
         self.plans = {}
         self.host = None
+        self.tree = None
 
     def sequences(self):
         """(cu_q, tokens cached before the step, sequences) as the kernels with a per-sequence state want them: in a decode
@@ -77,12 +79,44 @@ def _pack(arrays, device, static=None):
     return [dev[o:o + a.size].view(a.shape) for a, o in zip(arrays, offs)]
 
 
-def build_context(cache, entries, device, scratch_store=None, pad_to=None, plans=(), static=None):
+class TreeRows:
+    """What a step of trees of drafted tokens says of its rows beside the context's arrays (``row_pos`` is a node's position, the
+    tokens cached before and its depth):
+
+    place [n_tok]            where the node's key and value go: tokens cached before + its number within its tree
+    parent [n_tok]           the node it was drafted behind, -1 for a tree's root
+    bits [n_tok, words]      the nodes on the way from the root to it, itself included, a bit each (csrc.api.attention_tree)
+    max_nodes                nodes of the largest tree
+    """
+
+    def __init__(self, place, parent, bits, max_nodes):
+        self.place, self.parent, self.bits, self.max_nodes = place, parent, bits, max_nodes
+
+
+def tree_arrays(parents):
+    """(depth [rows], parent [rows], bits [rows, words]) of trees one behind the other; ``parents``: a list a tree, -1 for its root,
+    which comes first, and a smaller number for every other node."""
+    words = (max(len(p) for p in parents) + 31) // 32
+    depth, up, bits = [], [], []
+    for t, p in enumerate(parents):
+        if not len(p) or p[0] != -1 or any(not 0 <= q < i for i, q in enumerate(p) if i):
+            raise ValueError(f"tree {t}: the first node is the root (parent -1), the others come behind their parents")
+        d, seen = [], []
+        for i, q in enumerate(p):
+            d.append(d[q] + 1 if i else 0)
+            seen.append((seen[q] if i else 0) | 1 << i)
+        depth += d
+        up += p
+        bits += [[s >> 32 * w & 0xffffffff for w in range(words)] for s in seen]
+    return np.array(depth, np.int64), np.array(up, np.int64), np.array(bits, np.uint32).reshape(-1, words).view(np.int32)
+
+
+def build_context(cache, entries, device, scratch_store=None, pad_to=None, plans=(), static=None, parents=None):
     """``entries``: list of (slot, tokens, want) with ``want`` positions among these tokens.
     Reserves cache room for the new tokens. ``pad_to``: for decode steps, pad the batch with rows
     of position -1 up to this many rows (a captured graph has a fixed size). ``plans``: the
     ``StepPlan`` objects of the model's parts; each is built once and uploaded with the rest.
-    ``static``: see ``_pack``."""
+    ``static``: see ``_pack``. ``parents``: a list an entry where the tokens are trees (see ``tree_arrays``)."""
     n_seq = len(entries)
     lens = np.array([len(e[1]) for e in entries], dtype=np.int64)
     if n_seq == 0 or (lens < 1).any():
@@ -102,7 +136,12 @@ def build_context(cache, entries, device, scratch_store=None, pad_to=None, plans
             if not 0 <= j < lens[i]:
                 raise ValueError(f"wanted position {j} is outside the {lens[i]} tokens of entry {i}")
             want.append(cu[i] + j)
-    is_decode = bool((lens == 1).all())
+    is_decode = bool((lens == 1).all()) and parents is None
+    extra = []
+    if parents is not None:
+        depth, up, bits = tree_arrays(parents)
+        place, row_pos = row_pos, np.repeat(pos0, lens) + depth
+        extra = [place, up, bits]
     rows = n_tok
     if pad_to is not None and is_decode and pad_to > n_tok:
         pad = pad_to - n_tok
@@ -119,17 +158,19 @@ def build_context(cache, entries, device, scratch_store=None, pad_to=None, plans
         tables.append(t)
     i32 = lambda a: np.ascontiguousarray(a, dtype=np.int32)
     by_key = {}
-    for p in plans:
+    for p in plans if parents is None else ():
         if p.key not in by_key:
             by_key[p.key] = i32(p.build(lens, pos0, is_decode))
     fixed = [i32(tok), i32(row_seq), i32(row_pos), i32(cu), i32(slots), i32(pos0), i32(want)]
-    dev = _pack(fixed + tables + list(by_key.values()), device, static)
+    dev = _pack(fixed + tables + list(by_key.values()) + [i32(a) for a in extra], device, static)
     ctx = StepContext(scratch_store)
     ctx.n_tok, ctx.n_seq, ctx.n_want, ctx.is_decode = rows, n_seq, len(want), is_decode
     ctx.max_position = int((pos0 + lens).max()) - 1
     ctx.tok, ctx.row_seq, ctx.row_pos, ctx.cu_q, ctx.seq_slot, ctx.seq_pos0, ctx.want_rows = dev[:7]
     ctx.tables = dev[7:7 + len(tables)]
     ctx.plans = dict(zip(by_key, dev[7 + len(tables):]))
+    if parents is not None:
+        ctx.tree = TreeRows(*dev[-3:], int(lens.max()))
     ctx.host = dict(lens=lens, pos0=pos0, cu_q=cu, slots=slots, row_seq=row_seq, row_pos=row_pos)
     if is_decode:
         ctx.n_seq = rows  # the decode kernels run one sequence per row, padding rows included

@@ -6,11 +6,12 @@ tokens, and ``generate_all`` runs as many batches one after another as there are
 """
 import torch
 
-from ..csrc.api import PAGE
+from ..csrc.api import MAX_BEAMS, PAGE, TREE_MAX_NODES
 from ..registry import config_from_folder
 from ..sampling import SamplingParams, request_seed
 from ..weights import bind_random, load_weights
 from ..weights.loader import list_tensors
+from .branch import run_beams, run_drafted
 from .generate import GpuBackend, plan_batches, run_batch
 from .model import CausalLM
 from .runner import Runner
@@ -63,6 +64,8 @@ class Engine:
         self.backend = GpuBackend(self.runner, self.use_graph, self.max_prefill_tokens)
 
     def _ensure(self, prompts, max_new_tokens):
+        if any(len(p) == 0 for p in prompts):
+            raise ValueError("every prompt needs at least one token")
         need = sum((len(p) + max_new_tokens + PAGE - 1) // PAGE * PAGE for p in prompts)
         if self.runner is None or self.runner.cache.num_pages * PAGE < need or self.runner.cache.max_slots < len(prompts):
             if self._fixed_tokens is not None:
@@ -75,12 +78,40 @@ class Engine:
         prompts may have different lengths. Greedy unless ``temperature`` > 0."""
         if max_new_tokens <= 0 or not input_ids:
             return
-        if any(len(p) == 0 for p in input_ids):
-            raise ValueError("every prompt needs at least one token")
         params = SamplingParams(max_new_tokens, float(temperature), int(seed), tuple(stop_token_ids))
         self._ensure(input_ids, max_new_tokens)
         seeds = [request_seed(seed, first_index + i) for i in range(len(input_ids))]
         yield from run_batch(self.backend, [list(p) for p in input_ids], params, seeds)
+
+    def generate_drafted(self, input_ids, max_new_tokens, draft, temperature=0.0, seed=0, stop_token_ids=(), max_nodes=64):
+        """``generate`` with tokens that somebody else guesses and the model checks, several a step: the same tokens in fewer steps.
+        ``draft(i, tokens)`` is asked before every step how sequence i goes on behind ``tokens`` (its prompt and what was generated) and
+        answers with a list of tokens, or with (tokens, parents), a tree: ``parents[k]`` is the number of the drafted token that
+        ``tokens[k]`` would follow, -1 for the last of ``tokens``. Up to ``max_nodes`` - 1 tokens. Yields a list of lists, the new
+        tokens of every sequence (none once it has ended). For models whose layers are all attention that takes trees."""
+        if max_new_tokens <= 0 or not input_ids:
+            return
+        if not 1 <= max_nodes <= TREE_MAX_NODES:
+            raise ValueError(f"max_nodes must be between 1 and {TREE_MAX_NODES}")
+        if not self.model.takes_trees:
+            raise ValueError("a layer of this model cannot take trees of drafted tokens (it is no plain attention, or keeps a state)")
+        params = SamplingParams(max_new_tokens, float(temperature), int(seed), tuple(stop_token_ids))
+        self._ensure(input_ids, max_new_tokens + max_nodes)
+        yield from run_drafted(self.runner, [list(p) for p in input_ids], params, [request_seed(seed, i) for i in range(len(input_ids))],
+                               draft, max_nodes, self.max_prefill_tokens)
+
+    def beam_search(self, input_ids, beams, max_new_tokens, stop_token_ids=(), length_penalty=0.0):
+        """The ``beams`` best continuations that a search of that width finds for each prompt: a list a prompt of (tokens, score), best
+        first. The score is the sum of the tokens' log-probabilities over their number to the power ``length_penalty``; the search
+        itself goes by the sum. A continuation ends with a stop token, which is returned, or after ``max_new_tokens``."""
+        if not 1 <= beams <= MAX_BEAMS:
+            raise ValueError(f"beams must be between 1 and {MAX_BEAMS}")
+        if max_new_tokens <= 0 or not input_ids:
+            return [[] for _ in input_ids]
+        self._ensure([p for p in input_ids for _ in range(beams)], max_new_tokens)
+        found = run_beams(self.backend.loop, [list(p) for p in input_ids], beams, max_new_tokens, stop_token_ids, self.max_prefill_tokens)
+        scored = [[(t, v / len(t) ** length_penalty) for t, v in row] for row in found]
+        return [sorted(row, key=lambda x: -x[1]) for row in scored]
 
     def generate_all(self, prompts, max_new_tokens, temperature=0.0, seed=0, stop_token_ids=(), batch_size=64):
         """Token lists for any number of requests, run ``batch_size`` at a time, one batch after

@@ -4,7 +4,7 @@ describes and returns float32 logits at the wanted rows (reference: engine/engin
 """
 import torch
 
-from ..cache.requests import StateRequest
+from ..cache.requests import KVRequest, StateRequest
 from ..csrc import api
 from ..parts import ParamDecl, Runtime, build_part
 from ..parts.block import add_norm
@@ -101,6 +101,12 @@ class CausalLM:
 
     def entry_requests(self):
         return self._entry_requests
+
+    @property
+    def takes_trees(self):
+        """Whether every layer can be given trees of drafted tokens: attention that says so, and no state that moves with the tokens."""
+        return all(getattr(getattr(b, "mixer", None), "takes_trees", False) for b in self.blocks) \
+            and all(isinstance(r, KVRequest) for requests in self._entry_requests for r in requests)
 
     def prepare(self, max_positions):
         """Makes the parts' tables (rotation angles) reach ``max_positions``; they grow by doubling.

@@ -11,6 +11,7 @@ import torch
 
 from ..cache import Cache
 from ..csrc import api
+from ..sampling import seed_words
 from .batch import build_context
 
 GRAPH_MAX_TOKENS = 8192     # steps of more tokens are launched plainly (the reference's bound: engine/engine.py:30)
@@ -57,9 +58,9 @@ class Runner:
         if len({e[0] for e in entries}) != len(entries):
             raise ValueError("a slot appears twice in one step")
 
-    def context(self, entries, pad_to=None, static=None):
+    def context(self, entries, pad_to=None, static=None, parents=None):
         self._check(entries)
-        ctx = build_context(self.cache, entries, self.device, self._scratch, pad_to, self.model.step_plans, static)
+        ctx = build_context(self.cache, entries, self.device, self._scratch, pad_to, self.model.step_plans, static, parents)
         self.model.prepare(ctx.max_position + 1)     # tables grow here, never inside a step
         return ctx
 
@@ -127,3 +128,41 @@ class Runner:
             self.cache.commit(slot, len(tokens))
         api.gemm_tc_check()
         return (sg.logits, sg.ctx) if with_context else sg.logits
+
+    @torch.inference_mode()
+    def step_tree(self, entries, temperature=0.0, seeds=None):
+        """Checks trees of drafted tokens. entries: list of (slot, tokens, parents): ``tokens[0]`` is the sequence's last token, which
+        is not cached yet (``parents[0]`` = -1), ``tokens[i]`` was drafted to follow node ``parents[i]`` < i. One step runs all nodes;
+        from the root on the way goes to the child that holds the token the model chooses (greedy, or drawn with ``temperature`` and the
+        sequence's 64-bit seed in ``seeds``, as the sampler draws at that position), and ends at the first node without one. The nodes on
+        the way stay cached as the sequence's next tokens, the others' rows are given up. Returns a list an entry: the drafted
+        tokens on the way and the token chosen at its end, which is not cached: between 1 and the tree's depth + 1 tokens, the ones that
+        steps of single tokens would have brought. Waits for the step."""
+        if not self.model.takes_trees:
+            raise ValueError("a layer of this model cannot take trees of drafted tokens (it is no plain attention, or keeps a state)")
+        for slot, tokens, parents in entries:
+            if len(tokens) != len(parents) or not 1 <= len(tokens) <= api.TREE_MAX_NODES:
+                raise ValueError(f"slot {slot}: {len(tokens)} tokens, {len(parents)} parents; a tree has 1 to {api.TREE_MAX_NODES} nodes")
+        if seeds is None:
+            seeds = [0] * len(entries)
+        if len(seeds) != len(entries) or temperature < 0:
+            raise ValueError("one seed an entry, and a temperature that is not negative")
+        ctx = self.context([(s, t, range(len(t))) for s, t, _ in entries], parents=[list(p) for _, _, p in entries])
+        logits = self.model.forward(ctx, self.cache)
+        n, width = len(entries), ctx.tree.max_nodes
+        temps = torch.full((n,), float(temperature), device=self.device)
+        words = torch.tensor([seed_words(s) for s in seeds], dtype=torch.int32, device=self.device)
+        found = torch.empty(n * (width + 2), dtype=torch.int32, device=self.device)
+        path, count, token = found[:n * width].view(n, width), found[n * width:n * (width + 1)], found[n * (width + 1):]
+        api.tree_accept(logits, ctx.tok, ctx.tree.parent, ctx.cu_q, ctx.row_pos, temps, words, path, count, token)
+        for g, table in zip(self.cache.groups, ctx.tables):
+            for store in g.stores():
+                api.kv_keep(store, table, ctx.seq_pos0, path, count)
+        found = found.tolist()
+        api.gemm_tc_check()
+        out = []
+        for i, (slot, tokens, _) in enumerate(entries):
+            way = found[i * width:i * width + found[n * width + i]]
+            self.cache.commit(slot, len(way))
+            out.append([tokens[k] for k in way[1:]] + [found[n * (width + 1) + i]])
+        return out

@@ -98,6 +98,7 @@ class GQAAttention(Part):
         group = s.num_heads // s.num_kv_heads
         self.paged_f32 = rt.dtype == torch.float32 and s.head_dim in api.F32_ATTENTION_HEAD_DIMS \
             and group <= api.F32_ATTENTION_MAX_GROUP
+        self.takes_trees = s.head_dim % 16 == 0 and group <= api.TREE_MAX_GROUP
         self.tiles = QueryTiles(api.TC_TILE_ROWS if self.tc_prefill else api.MMA_TILE_ROWS) \
             if rt.dtype == torch.bfloat16 else F32QueryTiles(s.num_heads, s.num_kv_heads, s.window) if self.paged_f32 else None
 
@@ -147,6 +148,8 @@ class GQAAttention(Part):
         cos = sin = None
         if self.position is not None and self.fused_position:
             cos, sin = self.position.tables(max(self.max_positions, ctx.max_position + 1))
+        if ctx.tree is not None:
+            return self._forward_tree(ctx, kv, table, a, writes, qn, kn, eps, cos, sin)
         q = torch.empty((ctx.n_tok, nh * hd), dtype=dtype, device=dev)
         if dtype == torch.bfloat16 and self.fused_position and self._qkv_in_epilogue(a):
             # prefill: the projection's epilogue norms and rotates q and k and writes the cache
@@ -165,6 +168,24 @@ class GQAAttention(Part):
         api.qk_norm_rope_write(qkv, q, qn, kn, cos, sin, ctx.row_pos, ctx.row_seq, table, kv.k, kv.v, nh, nkv, hd, eps,
                                write_kv=writes)
         return self._attend(ctx, kv, table, q)
+
+    def _forward_tree(self, ctx, kv, table, a, writes, qn, kn, eps, cos, sin):
+        """A step of trees of drafted tokens: nodes are rotated by their positions and written to places of their own, which differ."""
+        s = self.spec
+        nh, nkv, hd = s.num_heads, s.num_kv_heads, s.head_dim
+        qkv = linear(a, self.w_qkv, allow_partial=True)
+        if qn is not None or cos is not None or isinstance(qkv, api.Partial):
+            normed = torch.empty((ctx.n_tok, (nh + 2 * nkv) * hd), dtype=self.rt.dtype, device=self.rt.device)
+            api.qk_norm_rope_write(qkv, None, qn, kn, cos, sin, ctx.row_pos, ctx.row_seq, table, kv.k, kv.v, nh, nkv, hd, eps, dense_out=normed)
+            qkv = normed
+        if not self.fused_position:
+            self.position.apply(qkv, ctx, nh, nkv, hd)
+        if writes:
+            api.kv_write(qkv[:, nh * hd:(nh + nkv) * hd], qkv[:, (nh + nkv) * hd:], kv.k, kv.v, ctx.tree.place, ctx.row_seq, table, nkv, hd, hd)
+        o = torch.empty((ctx.n_tok, nh * hd), dtype=self.rt.dtype, device=self.rt.device)
+        api.attention_tree(qkv[:, :nh * hd], o, kv.k, kv.v, ctx.cu_q, ctx.seq_pos0, ctx.row_pos, ctx.tree.bits, table, nh, nkv, hd,
+                           s.window or 0, s.scale, ctx.tree.max_nodes)
+        return linear(o, self.w_o, allow_partial=True)
 
     def _qkv_in_epilogue(self, a):
         """Whether this step's projection runs as the tensor-core product with norm, rotation and

@@ -18,6 +18,7 @@ Interfaces (duck-typed; see the classes in this package for the working examples
                    ``forward(ctx, views, a, writes)`` -> [tokens, hidden] in the compute dtype.
                    ``views`` are the cache views answering the requests, ``ctx`` the step's
                    ``engine.StepContext`` (token rows, their sequences and positions, page tables).
+                   ``takes_trees = True`` if it may be given steps of trees of drafted tokens (``ctx.tree``).
 * feed-forward:    ``forward(ctx, a)`` -> [tokens, hidden].
 
 Every part may also give ``step_weights()`` (the tensors a step reads once whatever the batch: the
