@@ -16,23 +16,122 @@ static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multip
 namespace {
 
 constexpr int WHOLE_PAGES = 1;                    // tables up to here are not split (see attention_tree.cuh)
-constexpr int THREADS = 256, LDK = HD + 4, LDP = DK_PAGE + 4, CV = HD / 16;
+constexpr int THREADS = 256, LDK = HD + 4, LDP = DK_PAGE + 4;
+// columns of a row: in groups of VEC side by side, a group every 16 * VEC
+constexpr int VEC = HD % 64 == 0 ? 4 : HD % 32 == 0 ? 2 : 1, CV = HD / (16 * VEC);
+template <int NI> constexpr int P_FLOATS = 16 * NI * LDP;
+template <int NI> constexpr int K_FLOATS = DK_PAGE * LDK > P_FLOATS<NI> ? DK_PAGE * LDK : P_FLOATS<NI>;          // P goes where K was
 
-__device__ __forceinline__ void load4(float* dst, const float* src) { *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(src); }
+__device__ __forceinline__ void load4(float* dst, const float* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
 __device__ __forceinline__ void load4(float* dst, const bf16* src) {
     const uint2 v = *reinterpret_cast<const uint2*>(src);
     const __nv_bfloat162 *a = reinterpret_cast<const __nv_bfloat162*>(&v.x), *b = reinterpret_cast<const __nv_bfloat162*>(&v.y);
     *reinterpret_cast<float4*>(dst) = make_float4(__low2float(*a), __high2float(*a), __low2float(*b), __high2float(*b));
 }
+__device__ __forceinline__ void copied() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// 256 threads: thread (ty, tx) of 16 x 16 has rows ty + 16 i of the tile (i < NI), keys tx + 16 j of the page, columns tx + 16 c.
+// Rows ty + 16 i (i < N) of a tile against one page, whose keys and values lie in shared memory. Thread (ty, tx) of 16 x 16 has keys tx +
+// 16 j for the scores (each a sum over even and one over odd columns, side by side), then VEC columns from VEC * tx + 16 VEC c on.
+template <int N, int NI>
+__device__ __forceinline__ void page_step(const float* q_s, const float* k_s, const float* v_s, float* p_s, const uint64_t* mask_s, float sl2,
+                                          bool odd, float (&m)[NI], float (&l)[NI], float (&acc)[NI][CV * VEC]) {
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    float2 s2[N][4] = {};
+#pragma unroll 4
+    for (int d = 0; d < HD; d += 4) {
+        float4 qa[N], kb[4];
+#pragma unroll
+        for (int i = 0; i < N; i++) qa[i] = *reinterpret_cast<const float4*>(q_s + (ty + 16 * i) * HD + d);
+#pragma unroll
+        for (int j = 0; j < 4; j++) kb[j] = *reinterpret_cast<const float4*>(k_s + (tx + 16 * j) * LDK + d);
+#pragma unroll
+        for (int i = 0; i < N; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                s2[i][j] = fma2(make_float2(qa[i].x, qa[i].y), make_float2(kb[j].x, kb[j].y), s2[i][j]);
+                s2[i][j] = fma2(make_float2(qa[i].z, qa[i].w), make_float2(kb[j].z, kb[j].w), s2[i][j]);
+            }
+    }
+    __syncthreads();                                                    // P goes where K was
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint64_t seen = mask_s[ty + 16 * i];
+        float sc[4], mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            sc[j] = seen >> (tx + 16 * j) & 1 ? s2[i][j].x + s2[i][j].y : -INFINITY;
+            mx = fmaxf(mx, sc[j]);
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float mn = fmaxf(m[i], mx * sl2), ms = mn == -INFINITY ? 0.f : mn, alpha = exp2f(m[i] - ms);
+        m[i] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float w = exp2f(fmaf(sc[j], sl2, -ms));
+            sum += w;
+            p_s[(ty + 16 * i) * LDP + tx + 16 * j] = w;
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        l[i] = l[i] * alpha + sum;
+#pragma unroll
+        for (int c = 0; c < CV * VEC; c++) acc[i][c] *= alpha;
+    }
+    __syncwarp();                                                       // a row's 16 threads sit in one warp
+    struct alignas(4 * VEC) Group { float x[VEC]; };
+    if (!odd) {
+#pragma unroll 2
+        for (int k = 0; k < DK_PAGE; k += 4) {
+            float4 w4[N];
+#pragma unroll
+            for (int i = 0; i < N; i++) w4[i] = *reinterpret_cast<const float4*>(p_s + (ty + 16 * i) * LDP + k);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+#pragma unroll
+                for (int c = 0; c < CV; c++) {
+                    const Group v = *reinterpret_cast<const Group*>(v_s + (k + e) * HD + (c * 16 + tx) * VEC);
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const float w = reinterpret_cast<const float*>(&w4[i])[e];
+                        float* a = acc[i] + c * VEC;
+                        if (VEC == 1) a[0] = fmaf(w, v.x[0], a[0]);
+                        else
+#pragma unroll
+                            for (int u = 0; u + 1 < VEC; u += 2) {
+                                const float2 r = fma2(make_float2(w, w), make_float2(v.x[u], v.x[u + 1]), make_float2(a[u], a[u + 1]));
+                                a[u] = r.x, a[u + 1] = r.y;
+                            }
+                    }
+                }
+            }
+        }
+    } else {                                                            // a value that is not finite reaches the rows that see it only
+        for (int k = 0; k < DK_PAGE; k++)
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (mask_s[ty + 16 * i] >> k & 1) {
+                    const float w = p_s[(ty + 16 * i) * LDP + k];
+#pragma unroll
+                    for (int c = 0; c < CV; c++)
+#pragma unroll
+                        for (int u = 0; u < VEC; u++) acc[i][c * VEC + u] = fmaf(w, v_s[k * HD + (c * 16 + tx) * VEC + u], acc[i][c * VEC + u]);
+                }
+    }
+}
+
+// 256 threads, two blocks an SM where their shared memory allows it (64 rows of 128 columns: 97 KB): one block's products run beside the
+// other's loads and exponentials.
 template <typename T, int NI>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 2)
 tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const T* k_store, const T* v_store, float* ws_acc, float2* ws_ml) {
     constexpr int TM = 16 * NI;
     extern __shared__ __align__(16) float smem[];
-    float *q_s = smem, *k_s = q_s + TM * HD, *v_s = k_s + DK_PAGE * LDK, *p_s = v_s + DK_PAGE * HD;
-    uint64_t* mask_s = reinterpret_cast<uint64_t*>(p_s + TM * LDP);
+    float *q_s = smem, *k_s = q_s + TM * HD, *v_s = k_s + K_FLOATS<NI>, *p_s = k_s;
+    uint64_t* mask_s = reinterpret_cast<uint64_t*>(v_s + DK_PAGE * HD);
     pdl_wait();
     pdl_launch_dependents();
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, G = a.nh / a.nkv;
@@ -47,12 +146,12 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
             if (r < rows) load4(q_s + r * HD + c, q + (size_t)(flat0 + r / G) * ldq + (kvh * G + r % G) * HD + c);
             else *reinterpret_cast<float4*>(q_s + r * HD + c) = make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        float m[NI], l[NI], acc[NI][CV];
+        float m[NI], l[NI], acc[NI][CV * VEC];
 #pragma unroll
         for (int i = 0; i < NI; i++) {
             m[i] = -INFINITY, l[i] = 0.f;
 #pragma unroll
-            for (int c = 0; c < CV; c++) acc[i][c] = 0.f;
+            for (int c = 0; c < CV * VEC; c++) acc[i][c] = 0.f;
         }
         for (int p = p0; p < p1; p++) {
             const int key0 = (sq.first_page + p) * DK_PAGE;
@@ -60,91 +159,28 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
             const bool held = page >= 0 && page < a.n_pages;           // a page that is none holds no keys
             if (!held) page = 0;
             const size_t off = kv_offset(page, a.nkv, kvh, 0, HD);
-            bool odd = false;                                           // an infinite or undefined value in this page
             for (int i = threadIdx.x; i < DK_PAGE * (HD / 4); i += THREADS) {
                 const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
                 load4(k_s + r * LDK + c, k_store + off + (size_t)i * 4);
-                float* v = v_s + r * HD + c;
-                load4(v, v_store + off + (size_t)i * 4);
-                odd |= !isfinite(v[0]) || !isfinite(v[1]) || !isfinite(v[2]) || !isfinite(v[3]);
+                load4(v_s + i * 4, v_store + off + (size_t)i * 4);
             }
+            bool masked = false;
             if (threadIdx.x < TM) {
                 const int r = threadIdx.x, row = flat0 + r / G;
-                mask_s[r] = held && r < rows ? tree_mask(a, sq, a.tree + (size_t)row * a.words, a.row_pos[row], key0) : 0ull;
+                const uint64_t seen = held && r < rows ? tree_mask(a, sq, a.tree + (size_t)row * a.words, a.row_pos[row], key0) : 0ull;
+                mask_s[r] = seen;
+                masked = r < rows && seen != ~0ull;
             }
-            odd = __syncthreads_or(odd);
-            float sc[NI][4];
-#pragma unroll
-            for (int i = 0; i < NI; i++) sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.f;
-#pragma unroll 4
-            for (int d = 0; d < HD; d += 4) {
-                float4 qa[NI], kb[4];
-#pragma unroll
-                for (int i = 0; i < NI; i++) qa[i] = *reinterpret_cast<const float4*>(q_s + (ty + 16 * i) * HD + d);
-#pragma unroll
-                for (int j = 0; j < 4; j++) kb[j] = *reinterpret_cast<const float4*>(k_s + (tx + 16 * j) * LDK + d);
-#pragma unroll
-                for (int i = 0; i < NI; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        sc[i][j] = fmaf(qa[i].x, kb[j].x, sc[i][j]);
-                        sc[i][j] = fmaf(qa[i].y, kb[j].y, sc[i][j]);
-                        sc[i][j] = fmaf(qa[i].z, kb[j].z, sc[i][j]);
-                        sc[i][j] = fmaf(qa[i].w, kb[j].w, sc[i][j]);
-                    }
+            copied();
+            // a page that some row does not see all of: is there a value in it that is not finite?
+            if (__syncthreads_or(masked)) {
+                masked = false;
+                for (int i = threadIdx.x; i < DK_PAGE * HD; i += THREADS) masked |= !isfinite(v_s[i]);
+                masked = __syncthreads_or(masked);
             }
-            float alpha[NI];
-#pragma unroll
-            for (int i = 0; i < NI; i++) {
-                const uint64_t seen = mask_s[ty + 16 * i];
-                float mx = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if (!(seen >> (tx + 16 * j) & 1)) sc[i][j] = -INFINITY;
-                    mx = fmaxf(mx, sc[i][j]);
-                }
-#pragma unroll
-                for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                const float mn = fmaxf(m[i], mx * a.sl2), ms = mn == -INFINITY ? 0.f : mn;
-                alpha[i] = exp2f(m[i] - ms);
-                m[i] = mn;
-                float sum = 0.f;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float pw = exp2f(fmaf(sc[i][j], a.sl2, -ms));
-                    sum += pw;
-                    p_s[(ty + 16 * i) * LDP + tx + 16 * j] = pw;
-                }
-#pragma unroll
-                for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                l[i] = l[i] * alpha[i] + sum;
-#pragma unroll
-                for (int c = 0; c < CV; c++) acc[i][c] *= alpha[i];
-            }
-            __syncwarp();                                               // a row's 16 threads sit in one warp
-            if (!odd) {
-#pragma unroll 4
-                for (int k = 0; k < DK_PAGE; k++) {
-                    float pw[NI];
-#pragma unroll
-                    for (int i = 0; i < NI; i++) pw[i] = p_s[(ty + 16 * i) * LDP + k];
-#pragma unroll
-                    for (int c = 0; c < CV; c++) {
-                        const float v = v_s[k * HD + tx + 16 * c];
-#pragma unroll
-                        for (int i = 0; i < NI; i++) acc[i][c] = fmaf(pw[i], v, acc[i][c]);
-                    }
-                }
-            } else {
-                for (int k = 0; k < DK_PAGE; k++)
-#pragma unroll
-                    for (int i = 0; i < NI; i++)
-                        if (mask_s[ty + 16 * i] >> k & 1) {
-                            const float pw = p_s[(ty + 16 * i) * LDP + k];
-#pragma unroll
-                            for (int c = 0; c < CV; c++) acc[i][c] = fmaf(pw, v_s[k * HD + tx + 16 * c], acc[i][c]);
-                        }
-            }
+            if (NI >= 4 && rows > 32) page_step<NI, NI>(q_s, k_s, v_s, p_s, mask_s, a.sl2, masked, m, l, acc);
+            else if (NI >= 2 && rows > 16) page_step<(NI < 2 ? NI : 2), NI>(q_s, k_s, v_s, p_s, mask_s, a.sl2, masked, m, l, acc);
+            else page_step<1, NI>(q_s, k_s, v_s, p_s, mask_s, a.sl2, masked, m, l, acc);
             __syncthreads();
         }
         const bool whole = w.all();
@@ -153,15 +189,14 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
         for (int i = 0; i < NI; i++) {
             const int r = ty + 16 * i;
             if (r >= rows) continue;
-            if (whole) {
-                const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
-                T* dst = out + (size_t)(flat0 + r / G) * ldo + (kvh * G + r % G) * HD;
+            const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+            T* dst = out + (size_t)(flat0 + r / G) * ldo + (kvh * G + r % G) * HD;
+            if (!whole && tx == 0) ws_ml[slot + r] = make_float2(m[i], l[i]);
 #pragma unroll
-                for (int c = 0; c < CV; c++) dst[tx + 16 * c] = from_f<T>(acc[i][c] * inv);
-            } else {
-                if (tx == 0) ws_ml[slot + r] = make_float2(m[i], l[i]);
-#pragma unroll
-                for (int c = 0; c < CV; c++) ws_acc[slot * HD + part_at(TM, r, tx + 16 * c)] = acc[i][c];
+            for (int c = 0; c < CV * VEC; c++) {
+                const int d = (c / VEC * 16 + tx) * VEC + c % VEC;
+                if (whole) dst[d] = from_f<T>(acc[i][c] * inv);
+                else ws_acc[slot * HD + part_at(TM, r, d)] = acc[i][c];
             }
         }
     }
@@ -169,7 +204,7 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
 
 template <int NI>
 constexpr size_t tree_smem() {
-    return sizeof(float) * (16 * NI * HD + DK_PAGE * LDK + DK_PAGE * HD + 16 * NI * LDP) + 16 * NI * sizeof(uint64_t);
+    return sizeof(float) * (16 * NI * HD + K_FLOATS<NI> + DK_PAGE * HD) + 16 * NI * sizeof(uint64_t);
 }
 
 template <typename T, int NI>

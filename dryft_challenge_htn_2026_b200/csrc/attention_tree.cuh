@@ -14,6 +14,20 @@
 #pragma once
 #include "common.cuh"
 
+// two numbers at a time: a * b + c, a + b
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; fma.rn.f32x2 x, x, y, z; mov.b64 {%0, %1}, x; }"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 struct TreeArgs {
     const int *cu_q, *seq_pos0, *row_pos, *page_table;
     const uint32_t* tree;                  // [rows, words]
@@ -189,8 +203,7 @@ __global__ void __launch_bounds__(256)
 tree_merge_kernel(TreeArgs a, const float* ws_acc, const float2* ws_ml, T* out, long long ldo, int tile_rows, int blocks) {
     constexpr int WARPS = 8, C = (D / 4 + WARPS - 1) / WARPS;         // fours of columns a warp has: w, w + 8, ..
     __shared__ __align__(16) T rows_s[32][D + 16 / sizeof(T)];
-    pdl_wait();
-    pdl_launch_dependents();
+    // which rows and parts these are hangs on what the kernel before has read as well: worked out before the wait for it
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, s = blockIdx.z, kvh = blockIdx.y, G = a.nh / a.nkv;
     const int groups = (tile_rows + 31) / 32, tile = blockIdx.x / groups, row = blockIdx.x % groups * 32 + lane;
     TreeRun run;
@@ -204,10 +217,11 @@ tree_merge_kernel(TreeArgs a, const float* ws_acc, const float2* ws_ml, T* out, 
         return in < a.half_nodes * G && half < a.tile_nodes && node < q.n ? node : -1;
     };
     const bool mine = node_of(row) >= 0;
-    if (tile >= q.tiles || !__any_sync(0xffffffffu, mine)) return;     // the same for all warps
     u0 += (kvh * q.tiles + tile) * q.length(a);
-    const int b0 = share_of(total, u0 + a.extra, nb), b1 = share_of(total, u0 + q.length(a) - 1, nb);
-    if (b0 == b1) return;
+    const int b0 = tile < q.tiles ? share_of(total, u0 + a.extra, nb) : 0, b1 = tile < q.tiles ? share_of(total, u0 + q.length(a) - 1, nb) : 0;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (b0 == b1 || !__any_sync(0xffffffffu, mine)) return;            // the same for all warps
     auto slot = [&](int b) { return (size_t)(2 * b + (b == b0 ? 1 : 0)) * tile_rows; };
     float m = -INFINITY, l = 0.f, acc[C][4] = {};
     constexpr int AT_ONCE = C <= 4 ? 4 : 2;                            // parts that are asked for together
