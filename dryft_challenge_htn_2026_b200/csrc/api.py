@@ -2233,8 +2233,9 @@ def _tree_plan(head_dim, f32, max_nodes, group):
 def attention_tree(q, out, k_store, v_store, cu_q, seq_pos0, row_pos, tree, page_table, n_heads, n_kv_heads, head_dim, window, scale,
                    max_nodes):
     """Attention of trees of drafted tokens over the paged cache. Sequence s has ``seq_pos0[s]`` cached tokens and brings the nodes of
-    its tree as rows cu_q[s] .. cu_q[s + 1] (at most ``max_nodes``); node i's key and value lie in the cache at place seq_pos0[s] + i,
-    its position is row_pos (seq_pos0[s] + its depth; < 0: a padding row, which sees nothing). It sees the cached tokens and the nodes j
+    its tree as rows cu_q[s] .. cu_q[s + 1] (at most ``max_nodes``: what is more is left out); node i's key and value lie in the cache at
+    place seq_pos0[s] + i, its position is row_pos (seq_pos0[s] + its depth, which is below the number of nodes; < 0: a padding row, which
+    sees nothing). It sees the cached tokens and the nodes j
     whose bit (word j / 32, bit j % 32) is set in its row of ``tree`` [rows, words] int32: of a drafted tree its ancestors and itself,
     but any bits may be set. With a ``window`` it sees only what lies less than that many positions before it. Rows that see nothing
     become zeros, rows behind cu_q's last are left as they were, and what lies at keys a row does not see, NaN included, does not reach

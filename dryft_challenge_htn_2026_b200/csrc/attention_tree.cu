@@ -209,14 +209,14 @@ constexpr size_t tree_smem() {
 
 template <typename T, int NI>
 int launch(const TreeArgs& a, const void* q, long long ldq, void* out, long long ldo, const void* k_store, const void* v_store, float* ws_acc,
-           float* ws_ml, int max_nodes, int blocks, cudaStream_t st) {
+           float* ws_ml, int blocks, cudaStream_t st) {
     static SmemOnce once;
     int r = once.allow((const void*)tree_kernel<T, NI>, tree_smem<NI>());
     if (r) return r;
     r = dk_launch(tree_kernel<T, NI>, dim3(blocks), dim3(THREADS), tree_smem<NI>(), st, a, (const T*)q, ldq, (T*)out, ldo,
                       (const T*)k_store, (const T*)v_store, ws_acc, (float2*)ws_ml);
     if (r) return r;
-    return tree_merge<T, HD>(a, ws_acc, ws_ml, out, ldo, 16 * NI, max_nodes, blocks, st);
+    return tree_merge<T, HD>(a, ws_acc, ws_ml, out, ldo, 16 * NI, blocks, st);
 }
 
 }  // namespace
@@ -253,10 +253,10 @@ DK_EXPORT int dk_attn_tree(int f32, const void* q, long long ldq, void* out, lon
     if (nkv < 1 || nh % nkv || nh / nkv > 64 || n_pages < 1 || pt_stride < 1 || words < 1 || blocks < 1 || max_nodes < 1 || n_seq > 65535)
         return (int)cudaErrorInvalidValue;
     const int G = nh / nkv, rows = dk_tree_tile_rows(max_nodes, G);
-    TreeArgs a = {cu_q, seq_pos0, row_pos, page_table, tree, n_seq, words, pt_stride, n_pages, nh, nkv, window, rows / G, rows / G, rows,
+    TreeArgs a = {cu_q, seq_pos0, row_pos, page_table, tree, n_seq, words, pt_stride, n_pages, nh, nkv, window, max_nodes, rows / G, rows / G, rows,
                   pt_stride <= WHOLE_PAGES, 0, scale * 1.4426950408889634f};
-    if (!tree_units_fit(a, max_nodes) || nkv > 65535) return (int)cudaErrorInvalidValue;
-#define DK_TREE(T, NI) launch<T, NI>(a, q, ldq, out, ldo, k_store, v_store, ws_acc, ws_ml, max_nodes, blocks, st)
+    if (!tree_units_fit(a) || nkv > 65535) return (int)cudaErrorInvalidValue;
+#define DK_TREE(T, NI) launch<T, NI>(a, q, ldq, out, ldo, k_store, v_store, ws_acc, ws_ml, blocks, st)
     if (f32) return rows == 16 ? DK_TREE(float, 1) : rows == 32 ? DK_TREE(float, 2) : DK_TREE(float, 4);
     return rows == 16 ? DK_TREE(bf16, 1) : rows == 32 ? DK_TREE(bf16, 2) : DK_TREE(bf16, 4);
 #undef DK_TREE

@@ -31,7 +31,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 struct TreeArgs {
     const int *cu_q, *seq_pos0, *row_pos, *page_table;
     const uint32_t* tree;                  // [rows, words]
-    int n_seq, words, pt_stride, n_pages, nh, nkv, window, tile_nodes, half_nodes, half_rows, whole, extra;
+    int n_seq, words, pt_stride, n_pages, nh, nkv, window, max_nodes, tile_nodes, half_nodes, half_rows, whole, extra;
     float sl2;                             // scale * log2(e)
 };
 
@@ -40,7 +40,7 @@ struct TreeSeq {
     int n, pos0, first_page, pages, tiles, flat0;
     __device__ __forceinline__ void load(const TreeArgs& a, int s) {
         flat0 = a.cu_q[s];
-        n = max(0, a.cu_q[s + 1] - flat0);
+        n = min(max(0, a.cu_q[s + 1] - flat0), a.max_nodes);
         pos0 = max(0, a.seq_pos0[s]);
         tiles = (n + a.tile_nodes - 1) / a.tile_nodes;
         // pages that the table has no column for hold no keys; one page at least, so that rows without a key are written too
@@ -294,15 +294,15 @@ struct SmemOnce {
 
 // Launch of the merge, behind the kernel that leaves the parts (it may start under that one's end: it reads nothing before).
 template <typename T, int D>
-static int tree_merge(const TreeArgs& a, const float* ws_acc, const float* ws_ml, void* out, long long ldo, int tile_rows, int max_nodes,
-                      int blocks, cudaStream_t st) {
+static int tree_merge(const TreeArgs& a, const float* ws_acc, const float* ws_ml, void* out, long long ldo, int tile_rows, int blocks,
+                      cudaStream_t st) {
     if (a.whole) return 0;
-    const int tiles = (max_nodes + a.tile_nodes - 1) / a.tile_nodes;
+    const int tiles = (a.max_nodes + a.tile_nodes - 1) / a.tile_nodes;
     return dk_launch_as(true, tree_merge_kernel<T, D>, dim3((tile_rows + 31) / 32 * tiles, a.nkv, a.n_seq), dim3(256), 0, st, a, ws_acc,
                         (const float2*)ws_ml, (T*)out, ldo, tile_rows, blocks);
 }
 
 // Whether the largest launch of these sizes has fewer than 2^31 units.
-static inline bool tree_units_fit(const TreeArgs& a, int max_nodes) {
-    return (double)a.n_seq * ((max_nodes + a.tile_nodes - 1) / a.tile_nodes) * a.nkv * (a.pt_stride + a.extra) < 2147483647.0;
+static inline bool tree_units_fit(const TreeArgs& a) {
+    return (double)a.n_seq * ((a.max_nodes + a.tile_nodes - 1) / a.tile_nodes) * a.nkv * (a.pt_stride + a.extra) < 2147483647.0;
 }

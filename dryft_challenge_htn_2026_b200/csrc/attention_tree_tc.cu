@@ -614,9 +614,9 @@ DK_EXPORT int dk_attn_tree_tc(const void* q, long long ldq, void* out, long long
         err == nullptr || ldq % 8 || ldo % 8 || ((uintptr_t)q | (uintptr_t)out) % 16 || (long long)n_pages * nkv * DK_PAGE > 0x7fffffffLL)
         return (int)cudaErrorInvalidValue;
     const int G = nh / nkv;
-    TreeArgs a = {cu_q, seq_pos0, row_pos, page_table, tree, n_seq, words, pt_stride, n_pages, nh, nkv, window, 2 * (BM / G), BM / G, BM,
+    TreeArgs a = {cu_q, seq_pos0, row_pos, page_table, tree, n_seq, words, pt_stride, n_pages, nh, nkv, window, max_nodes, 2 * (BM / G), BM / G, BM,
                   pt_stride <= WHOLE_PAGES, EXTRA, scale * 1.4426950408889634f};
-    if (!tree_units_fit(a, max_nodes) || nkv > 65535) return (int)cudaErrorInvalidValue;
+    if (!tree_units_fit(a) || nkv > 65535) return (int)cudaErrorInvalidValue;
     static SmemOnce once;
     int e = once.allow((const void*)tree_tc_kernel, SMEM_BYTES);
     if (e) return e;
@@ -632,5 +632,5 @@ DK_EXPORT int dk_attn_tree_tc(const void* q, long long ldq, void* out, long long
     e = dk_launch(tree_tc_kernel, dim3(blocks), dim3(THREADS), SMEM_BYTES, st, mq, mk, mv, a, (bf16*)out, ldo, (const bf16*)v_store, ws_acc,
                   (float2*)ws_ml, err);
     if (e) return e;
-    return tree_merge<bf16, HD>(a, ws_acc, ws_ml, out, ldo, 2 * BM, max_nodes, blocks, st);
+    return tree_merge<bf16, HD>(a, ws_acc, ws_ml, out, ldo, 2 * BM, blocks, st);
 }

@@ -155,7 +155,7 @@ def test_tree_attention(dtype, heads, before, nodes):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("heads", [(8, 2, 128), (4, 4, 64), (16, 1, 64), (3, 1, 32)])
+@pytest.mark.parametrize("heads", [(8, 2, 128), (4, 4, 64), (16, 1, 64), (3, 1, 32), (5, 1, 128), (14, 2, 64), (64, 1, 64)])
 def test_tree_attention_long_contexts_and_large_trees(dtype, heads):
     check_attend(tree_case([900, 37, 2500], [12, 130, 3], *heads, dtype, seed=3))
 
@@ -280,6 +280,60 @@ def test_tree_attention_gives_the_same_bits_every_time(hd, nh, nkv, n_seq, conte
     ref, tol = plain_attend(dict(c, before=c["before"][:1], nodes=c["nodes"][:1], masks=c["masks"][:1]))
     rows = c["nodes"][0]
     assert bool(((first.double().cpu() - ref).abs() <= tol)[:rows].all())
+
+
+def test_tree_attention_leaves_out_nodes_above_its_number():
+    for dtype in (torch.bfloat16, torch.float32):
+        c = tree_case([700, 3], [9, 40], 8, 2, 64, dtype, seed=12)
+        got = attend(c, max_nodes=20)
+        few = dict(c, nodes=[9, 20], masks=[c["masks"][0], c["masks"][1][:20, :20]], rows=29, q=c["q"][:29])
+        ref, tol = plain_attend(few)
+        assert bool(((got[:29].double().cpu() - ref).abs() <= tol).all()) and bool((got[29:] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_offsets_beyond_32_bits(dtype):
+    """A store of more than 2^32 bytes and 2^31 numbers whose last pages are used, the rest whatever the memory held."""
+    nkv, hd = 8, 128
+    n_pages = (1 << 31) // (nkv * PAGE * hd) + 9
+    store = torch.empty((1, 2, n_pages, nkv, PAGE, hd), dtype=dtype, device=DEV)
+    c = tree_case([70, 130], [5, 33], 16, nkv, hd, dtype, seed=13)
+    far = c["table"] + (n_pages - c["n_pages"])
+    for page in range(c["n_pages"]):
+        store[0, 0, n_pages - c["n_pages"] + page], store[0, 1, n_pages - c["n_pages"] + page] = c["k"][page], c["v"][page]
+    d = dict(c, k=store[0, 0], v=store[0, 1], page_table=i32(np.where(c["table"] >= 0, far, -1)), n_pages=n_pages)
+    assert torch.equal(attend(d), attend(c))
+    small = torch.stack([c["k"], c["v"]])[None].clone()
+    path, count = i32([[0, 2, 4, -1, -1]] * 2), i32([3, 3])
+    for t, table in ((store, d["page_table"]), (small, c["page_table"])):
+        api.kv_keep(t, table, c["pos0"], path, count)
+        api.kv_reorder(t, table, i32([[1, 0]]), i32([2]), i32([90]))
+    assert torch.equal(store[:, :, -c["n_pages"]:], small)
+    del store, d
+    torch.cuda.empty_cache()
+
+
+def test_calls_on_two_streams_at_once():
+    cases = [tree_case([900, 2000], [40, 7], 8, 2, 128, torch.bfloat16, seed=14 + i) for i in range(2)]
+    logits = [normal((12, 50000), seed=20 + i, scale=3.0) for i in range(2)]
+    scores = torch.zeros((3, 4), device=DEV)
+    tree = ([3] * 12, [[-1] + list(range(11))], list(range(12)), [0.7], [[5, 6]])
+    want = [(attend(c), select(x, scores, None, 8), accept(x, *tree)) for c, x in zip(cases, logits)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for st, c, x in zip(streams, cases, logits):
+            with torch.cuda.stream(st):
+                out = torch.empty_like(c["q"])
+                api.attention_tree(c["q"], out, c["k"], c["v"], c["cu"], c["pos0"], c["pos"], c["tree"], c["page_table"], 8, 2, 128, 0, 128 ** -0.5, 40)
+                best = torch.empty((3, 8), device=DEV), i32(np.zeros((3, 8))), i32(np.zeros((3, 8)))
+                api.beam_select(x, scores, None, *best)
+                got.append((out, best))
+        torch.cuda.synchronize()
+        for (out, best), (a, b, _) in zip(got, want):
+            assert torch.equal(out, a) and all(torch.equal(p.cpu(), q) for p, q in zip(best, b))
+    api.gemm_tc_check()
 
 
 def test_tree_attention_refusals():
