@@ -197,15 +197,17 @@ static __device__ __noinline__ uint64_t tree_mask(const TreeArgs& a, TreeSeq q, 
 }
 
 // Merges the parts of the tiles that more than one block worked on; the others have been written. Grid (row groups of the largest
-// tree, nkv, n_seq), 256 threads: a block has 32 rows of a tile, lane k its k-th, each warp an eighth of the columns.
-template <typename T, int D>
+// tree x column groups, nkv, n_seq), 256 threads: a block has 32 rows of a tile, lane k its k-th, and COLS columns, an eighth of them a
+// warp. What four parts say of a row is asked for together, or eight where a block has 64 columns.
+template <typename T, int D, int COLS>
 __global__ void __launch_bounds__(256)
 tree_merge_kernel(TreeArgs a, const float* ws_acc, const float2* ws_ml, T* out, long long ldo, int tile_rows, int blocks) {
-    constexpr int WARPS = 8, C = (D / 4 + WARPS - 1) / WARPS;         // fours of columns a warp has: w, w + 8, ..
-    __shared__ __align__(16) T rows_s[32][D + 16 / sizeof(T)];
+    constexpr int WARPS = 8, C = (COLS / 4 + WARPS - 1) / WARPS;       // fours of columns a warp has: w, w + 8, ..
+    __shared__ __align__(16) T rows_s[32][COLS + 16 / sizeof(T)];
     // which rows and parts these are hangs on what the kernel before has read as well: worked out before the wait for it
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, s = blockIdx.z, kvh = blockIdx.y, G = a.nh / a.nkv;
-    const int groups = (tile_rows + 31) / 32, tile = blockIdx.x / groups, row = blockIdx.x % groups * 32 + lane;
+    const int groups = (tile_rows + 31) / 32, part = blockIdx.x / (D / COLS), d0 = blockIdx.x % (D / COLS) * COLS;
+    const int tile = part / groups, row = part % groups * 32 + lane;
     TreeRun run;
     run.read(a);
     int u0;
@@ -224,7 +226,7 @@ tree_merge_kernel(TreeArgs a, const float* ws_acc, const float2* ws_ml, T* out, 
     if (b0 == b1 || !__any_sync(0xffffffffu, mine)) return;            // the same for all warps
     auto slot = [&](int b) { return (size_t)(2 * b + (b == b0 ? 1 : 0)) * tile_rows; };
     float m = -INFINITY, l = 0.f, acc[C][4] = {};
-    constexpr int AT_ONCE = C <= 4 ? 4 : 2;                            // parts that are asked for together
+    constexpr int AT_ONCE = C <= 2 ? 8 : C <= 4 ? 4 : 2;
     if (mine)
         for (int b = b0; b <= b1; b += AT_ONCE) {
             float2 p[AT_ONCE];
@@ -235,7 +237,7 @@ tree_merge_kernel(TreeArgs a, const float* ws_acc, const float2* ws_ml, T* out, 
 #pragma unroll
                 for (int c = 0; c < C; c++) {
                     const int d = (c * WARPS + w) * 4;
-                    v[k][c] = d < D && b + k <= b1 ? *reinterpret_cast<const float4*>(ws_acc + slot(b + k) * D + part_at(tile_rows, row, d))
+                    v[k][c] = d < COLS && b + k <= b1 ? *reinterpret_cast<const float4*>(ws_acc + slot(b + k) * D + part_at(tile_rows, row, d0 + d))
                                                    : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
             }
@@ -266,14 +268,14 @@ tree_merge_kernel(TreeArgs a, const float* ws_acc, const float2* ws_ml, T* out, 
         struct alignas(4 * sizeof(T)) Four { T x[4]; } r;
 #pragma unroll
         for (int e = 0; e < 4; e++) r.x[e] = from_f<T>(acc[c][e] * inv);
-        if (d < D) *reinterpret_cast<Four*>(&rows_s[lane][d]) = r;
+        if (d < COLS) *reinterpret_cast<Four*>(&rows_s[lane][d]) = r;
     }
     __syncthreads();
-    constexpr int PIECES = D * (int)sizeof(T) / 16, PER = 16 / (int)sizeof(T);     // 16 bytes a thread, the pieces of a row side by side
+    constexpr int PIECES = COLS * (int)sizeof(T) / 16, PER = 16 / (int)sizeof(T);     // 16 bytes a thread, the pieces of a row side by side
     for (int i = threadIdx.x; i < 32 * PIECES; i += 256) {
         const int k = i / PIECES, c = i % PIECES * PER, r = row - lane + k, node = node_of(r);
         if (node >= 0)
-            *reinterpret_cast<uint4*>(out + (size_t)(q.flat0 + node) * ldo + (kvh * G + r % a.half_rows % G) * D + c) =
+            *reinterpret_cast<uint4*>(out + (size_t)(q.flat0 + node) * ldo + (kvh * G + r % a.half_rows % G) * D + d0 + c) =
                 *reinterpret_cast<const uint4*>(&rows_s[k][c]);
     }
 }
@@ -297,9 +299,15 @@ template <typename T, int D>
 static int tree_merge(const TreeArgs& a, const float* ws_acc, const float* ws_ml, void* out, long long ldo, int tile_rows, int blocks,
                       cudaStream_t st) {
     if (a.whole) return 0;
-    const int tiles = (a.max_nodes + a.tile_nodes - 1) / a.tile_nodes;
-    return dk_launch_as(true, tree_merge_kernel<T, D>, dim3((tile_rows + 31) / 32 * tiles, a.nkv, a.n_seq), dim3(256), 0, st, a, ws_acc,
-                        (const float2*)ws_ml, (T*)out, ldo, tile_rows, blocks);
+    const int tiles = (a.max_nodes + a.tile_nodes - 1) / a.tile_nodes, groups = (tile_rows + 31) / 32 * tiles;
+    // Few tiles, so many parts each: the columns in halves, to have more of them on the way at once (two sequences of 32k tokens, 9 parts:
+    // 61.8 us the whole call with all columns a block, 60.5 with halves; eight of 4k tokens, 2 to 4 parts: 48.5 and 53.3).
+    constexpr int HALF = D % 128 == 0 ? D / 2 : D;
+    if (HALF < D && 4LL * a.n_seq * tiles * a.nkv <= blocks)
+        return dk_launch_as(true, tree_merge_kernel<T, D, HALF>, dim3(groups * (D / HALF), a.nkv, a.n_seq), dim3(256), 0, st, a, ws_acc,
+                            (const float2*)ws_ml, (T*)out, ldo, tile_rows, blocks);
+    return dk_launch_as(true, tree_merge_kernel<T, D, D>, dim3(groups, a.nkv, a.n_seq), dim3(256), 0, st, a, ws_acc, (const float2*)ws_ml,
+                        (T*)out, ldo, tile_rows, blocks);
 }
 
 // Whether the largest launch of these sizes has fewer than 2^31 units.

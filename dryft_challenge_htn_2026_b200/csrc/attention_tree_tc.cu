@@ -345,6 +345,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                             umma_ss(t_sx + b * BN, dqx + (uint64_t)((hh * Q_ATOM_BYTES + k * 32) >> 4),
                                     dkt + (uint64_t)((hh * KV_ATOM_BYTES + k * 32) >> 4), IDESC_S, (hh | k) != 0);
                     umma_commit(bar_s + b);
+                    umma_commit(k_free + rk.slot);
                     if (i + 1 == n) umma_commit(q_free);
                     rk.advance(), k_next++;
                 };
@@ -371,6 +372,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     for (int k = 0; k < BN / 16; k++)
                         umma_ts(t_ox, t_sx + b * BN + k * 8, dvt + (uint64_t)((k * 16 * 128) >> 4), IDESC_PV, (i | k) != 0);   // the first overwrites O
                     umma_commit(bar_o + b);
+                    umma_commit(v_free + rv.slot);
                     rv.advance(), v_next++;
                     // into the buffer whose P was just used: products of one thread run in order
                     if (i + 2 < n) issue_s(i + 2);
@@ -414,11 +416,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 const bool held = page >= 0 && page < a.n_pages;
                 const bool open = held && key0 + BN <= sq.pos0 && key0 >= open_lo;
                 if (!mbar_wait(bar_s + b, ph)) { ok = false; break; }
-                if (r == 0) {                              // S is here, so its keys are free, and P.V of two steps before, which stood ahead of it, is done
-                    mbar_arrive(k_free + rk.ahead(j - w.p0));
-                    // (said before this step's values are waited for: their page may come to lie where those did)
-                    if (i > 1) mbar_arrive(v_free + rv.ahead(w.page_of(x, i - 2)));
-                }
                 uint64_t seen = ~0ull;
                 if (!open) {
                     seen = !held || !valid ? 0ull : j >= tail ? seen_tail[j - tail ? 1 : 0] : tree_mask(a, sq, words, qpos, key0);
@@ -497,8 +494,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             }
             if (ok && n > 0) ok = mbar_wait(bar_o + ((done + n - 1) & 1), ((done + n - 1) >> 1) & 1);
             if (!ok) break;
-            if (r == 0)
-                for (int i = max(0, n - 2); i < n; i++) mbar_arrive(v_free + rv.ahead(w.page_of(x, i)));
             if (!valid) m = -INFINITY, l = 0.f;
             // the factors of the two streams' rows: with rows in both, the own one alone
             float mine = 1.f, other = 0.f;
