@@ -52,7 +52,6 @@ beam_pieces_kernel(const float* logits, int V, int best, uint64_t* ws_key, doubl
     __shared__ double red_s[WARPS];
     __shared__ int count;
     pdl_wait();
-    pdl_launch_dependents();
     const int t = threadIdx.x, lane = t & 31, w = t >> 5;
     const float* z = logits + (size_t)blockIdx.y * V;
     const Piece piece(z, blockIdx.x);
@@ -146,6 +145,9 @@ beam_pieces_kernel(const float* logits, int V, int best, uint64_t* ws_key, doubl
         if (rank < best) out[rank] = key;
     }
     for (int i = n + t; i < best; i += THREADS) out[i] = 0;
+    // the second launch's blocks come in as these leave: called at the start, they stood in the way of blocks still to come (16 searches
+    // of 8 beams: 33 us instead of 25)
+    pdl_launch_dependents();
 }
 
 // A value in double, in the order of its bits, and its place among all beams' tokens; place -1: none.

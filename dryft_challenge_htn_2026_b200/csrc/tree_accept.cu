@@ -36,7 +36,6 @@ accept_pieces_kernel(const float* logits, int V, const int* cu_q, const int* row
     __shared__ float sv[THREADS / 32];
     __shared__ int si[THREADS / 32];
     pdl_wait();
-    pdl_launch_dependents();
     const int s = blockIdx.z, row = cu_q[s] + blockIdx.y;
     if (row >= cu_q[s + 1]) return;
     const float* z = logits + (size_t)row * V;
@@ -82,6 +81,7 @@ accept_pieces_kernel(const float* logits, int V, const int* cu_q, const int* row
             ws_val[at] = bv, ws_idx[at] = bi;
         }
     }
+    pdl_launch_dependents();                                           // (at the start, the second launch's blocks would stand in the way)
 }
 
 // grid (sequences)
