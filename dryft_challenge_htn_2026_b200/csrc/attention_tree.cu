@@ -16,7 +16,7 @@ static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multip
 namespace {
 
 constexpr int WHOLE_PAGES = 1;                    // tables up to here are not split (see attention_tree.cuh)
-constexpr int THREADS = 256, LDK = HD + 4, LDP = DK_PAGE + 4;
+constexpr int THREADS = 256, LDQ = HD + 4, LDK = HD + 4, LDP = DK_PAGE + 4;
 // columns of a row: in groups of VEC side by side, a group every 16 * VEC
 constexpr int VEC = HD % 64 == 0 ? 4 : HD % 32 == 0 ? 2 : 1, CV = HD / (16 * VEC);
 template <int NI> constexpr int P_FLOATS = 16 * NI * LDP;
@@ -30,20 +30,21 @@ __device__ __forceinline__ void load4(float* dst, const bf16* src) {
     const __nv_bfloat162 *a = reinterpret_cast<const __nv_bfloat162*>(&v.x), *b = reinterpret_cast<const __nv_bfloat162*>(&v.y);
     *reinterpret_cast<float4*>(dst) = make_float4(__low2float(*a), __high2float(*a), __low2float(*b), __high2float(*b));
 }
-__device__ __forceinline__ void copied() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copied() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
 // Rows ty + 16 i (i < N) of a tile against one page, whose keys and values lie in shared memory. Thread (ty, tx) of 16 x 16 has keys tx +
 // 16 j for the scores (each a sum over even and one over odd columns, side by side), then VEC columns from VEC * tx + 16 VEC c on.
 template <int N, int NI>
 __device__ __forceinline__ void page_step(const float* q_s, const float* k_s, const float* v_s, float* p_s, const uint64_t* mask_s, float sl2,
-                                          bool odd, float (&m)[NI], float (&l)[NI], float (&acc)[NI][CV * VEC]) {
+                                          bool masked, float (&m)[NI], float (&l)[NI], float (&acc)[NI][CV * VEC]) {
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     float2 s2[N][4] = {};
 #pragma unroll 4
     for (int d = 0; d < HD; d += 4) {
         float4 qa[N], kb[4];
 #pragma unroll
-        for (int i = 0; i < N; i++) qa[i] = *reinterpret_cast<const float4*>(q_s + (ty + 16 * i) * HD + d);
+        for (int i = 0; i < N; i++) qa[i] = *reinterpret_cast<const float4*>(q_s + (ty + 16 * i) * LDQ + d);
 #pragma unroll
         for (int j = 0; j < 4; j++) kb[j] = *reinterpret_cast<const float4*>(k_s + (tx + 16 * j) * LDK + d);
 #pragma unroll
@@ -54,7 +55,13 @@ __device__ __forceinline__ void page_step(const float* q_s, const float* k_s, co
                 s2[i][j] = fma2(make_float2(qa[i].z, qa[i].w), make_float2(kb[j].z, kb[j].w), s2[i][j]);
             }
     }
+    copied<0>();                                                        // the values
     __syncthreads();                                                    // P goes where K was
+    bool odd = false;
+    if (masked) {       // some row does not see all of the page: is there a value in it that is not finite?
+        for (int i = threadIdx.x; i < DK_PAGE * HD; i += THREADS) odd |= !isfinite(v_s[i]);
+        odd = __syncthreads_or(odd);
+    }
 #pragma unroll
     for (int i = 0; i < N; i++) {
         const uint64_t seen = mask_s[ty + 16 * i];
@@ -130,7 +137,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const T* k_store, const T* v_store, float* ws_acc, float2* ws_ml) {
     constexpr int TM = 16 * NI;
     extern __shared__ __align__(16) float smem[];
-    float *q_s = smem, *k_s = q_s + TM * HD, *v_s = k_s + K_FLOATS<NI>, *p_s = k_s;
+    float *q_s = smem, *k_s = q_s + TM * LDQ, *v_s = k_s + K_FLOATS<NI>, *p_s = k_s;
     uint64_t* mask_s = reinterpret_cast<uint64_t*>(v_s + DK_PAGE * HD);
     pdl_wait();
     pdl_launch_dependents();
@@ -143,8 +150,8 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
         const int* pt = w.pt;
         for (int i = threadIdx.x; i < TM * (HD / 4); i += THREADS) {
             const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
-            if (r < rows) load4(q_s + r * HD + c, q + (size_t)(flat0 + r / G) * ldq + (kvh * G + r % G) * HD + c);
-            else *reinterpret_cast<float4*>(q_s + r * HD + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < rows) load4(q_s + r * LDQ + c, q + (size_t)(flat0 + r / G) * ldq + (kvh * G + r % G) * HD + c);
+            else *reinterpret_cast<float4*>(q_s + r * LDQ + c) = make_float4(0.f, 0.f, 0.f, 0.f);
         }
         float m[NI], l[NI], acc[NI][CV * VEC];
 #pragma unroll
@@ -159,11 +166,10 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
             const bool held = page >= 0 && page < a.n_pages;           // a page that is none holds no keys
             if (!held) page = 0;
             const size_t off = kv_offset(page, a.nkv, kvh, 0, HD);
-            for (int i = threadIdx.x; i < DK_PAGE * (HD / 4); i += THREADS) {
-                const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
-                load4(k_s + r * LDK + c, k_store + off + (size_t)i * 4);
-                load4(v_s + i * 4, v_store + off + (size_t)i * 4);
-            }
+            for (int i = threadIdx.x; i < DK_PAGE * (HD / 4); i += THREADS) load4(k_s + i / (HD / 4) * LDK + (i % (HD / 4)) * 4, k_store + off + (size_t)i * 4);
+            copies_end();                                              // the scores wait for the keys (and the tile's queries) alone
+            for (int i = threadIdx.x; i < DK_PAGE * (HD / 4); i += THREADS) load4(v_s + i * 4, v_store + off + (size_t)i * 4);
+            copies_end();
             bool masked = false;
             if (threadIdx.x < TM) {
                 const int r = threadIdx.x, row = flat0 + r / G;
@@ -171,13 +177,8 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
                 mask_s[r] = seen;
                 masked = r < rows && seen != ~0ull;
             }
-            copied();
-            // a page that some row does not see all of: is there a value in it that is not finite?
-            if (__syncthreads_or(masked)) {
-                masked = false;
-                for (int i = threadIdx.x; i < DK_PAGE * HD; i += THREADS) masked |= !isfinite(v_s[i]);
-                masked = __syncthreads_or(masked);
-            }
+            copied<1>();
+            masked = __syncthreads_or(masked);
             if (NI >= 4 && rows > 32) page_step<NI, NI>(q_s, k_s, v_s, p_s, mask_s, a.sl2, masked, m, l, acc);
             else if (NI >= 2 && rows > 16) page_step<(NI < 2 ? NI : 2), NI>(q_s, k_s, v_s, p_s, mask_s, a.sl2, masked, m, l, acc);
             else page_step<1, NI>(q_s, k_s, v_s, p_s, mask_s, a.sl2, masked, m, l, acc);
@@ -204,7 +205,7 @@ tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const 
 
 template <int NI>
 constexpr size_t tree_smem() {
-    return sizeof(float) * (16 * NI * HD + K_FLOATS<NI> + DK_PAGE * HD) + 16 * NI * sizeof(uint64_t);
+    return sizeof(float) * (16 * NI * LDQ + K_FLOATS<NI> + DK_PAGE * HD) + 16 * NI * sizeof(uint64_t);
 }
 
 template <typename T, int NI>
