@@ -18,8 +18,9 @@
 // Nobody waits for a tile's end but for what it leaves: the loader runs on into the next tile's pages, S of the next tile starts while
 // the rows of the last one are written, only P.V into O waits until they are read.
 // Pages of cached tokens that every row sees need no mask. In the others (the tree's own, the first of a window) a row's 64 visible
-// places are one word of bits. P.V adds up 0 * v for what a row does not see: where such a page holds a value that is not finite it is
-// set to zero in shared memory, and at the end the rows that do see it take it up from the cache.
+// places are one word of bits. P.V adds up 0 * v for what a row does not see: where such a page holds a value that is not finite, warp 11
+// sets it to zero in shared memory before the products may have the page, and at the end the rows that do see it take it up from the
+// cache. (Softmax warps that looked the page over themselves took 1.3 us for it, at the end of every tile.)
 // Tensor memory: S of A 0 | 1, S of B 0 | 1, O of A, O of B = 4 x 64 + 2 x 128 columns.
 // Every mbarrier wait is bounded; a wait that runs out stores a code in *err, and the block still frees its tensor memory and returns.
 #include <cuda.h>
@@ -34,8 +35,8 @@ static_assert(HD == 64 || HD == 128, "built for head sizes 64 and 128");
 namespace {
 
 constexpr int BM = 128, BN = DK_PAGE;             // rows of a stream, keys a step (one page)
-constexpr int SOFT = 2 * BM;                      // softmax threads, one a row of each stream; then two mma warps, then the loader warp
-constexpr int THREADS = SOFT + 96, MMA_WARP = SOFT / 32, LOAD_WARP = MMA_WARP + 2;
+constexpr int SOFT = 2 * BM;                      // softmax threads, one a row of each stream; two mma warps, the loader's, the checker's
+constexpr int THREADS = SOFT + 128, MMA_WARP = SOFT / 32, LOAD_WARP = MMA_WARP + 2, CHECK_WARP = MMA_WARP + 3;
 constexpr int TMEM_ALLOC = 512;
 constexpr int OC = 16;                            // columns of a row's result a thread handles at a time
 constexpr int HALVES = HD / 64;                   // 64-column swizzle atoms across the head
@@ -45,8 +46,10 @@ constexpr int WHOLE_PAGES = 8;                    // tables up to here are not s
 constexpr int EXTRA = 5;                          // pages that a tile's beginning and end take as long as
 constexpr int NK = HD == 128 ? 5 : 9, NV = HD == 128 ? 4 : 8;          // pages in the rings
 constexpr int RING = 2 * Q_BYTES, V_RING = RING + NK * KV_BYTES, BARS = V_RING + NV * KV_BYTES;
-constexpr int N_BARS = 2 * NK + 2 * NV + 16 + 5;
-constexpr int ML = BARS + (N_BARS + 4) * 8;       // [2][2][BM] pairs (maximum, sum) that the streams exchange
+constexpr int N_BARS = 2 * NK + 3 * NV + 12 + 5;
+constexpr int MARKS = 16;                         // tiles that the checker may be ahead of the softmax warps: a page each at least, so no more than NV + 1
+static_assert(MARKS > NV + 1, "marks of tiles");
+constexpr int ML = BARS + (N_BARS + 1 + MARKS / 2) * 8;       // [2][2][BM] pairs (maximum, sum) that the streams exchange
 constexpr size_t SMEM_BYTES = 1024 + ML + 4 * BM * 8;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of a block");
 #ifndef DK_WAIT_CYCLES
@@ -220,6 +223,9 @@ __device__ __noinline__ void mend_row(const TreeArgs& a, const Walk& w, const ui
     }
 }
 
+// Pages from this place on, up to the cached tokens' end, are seen by every row: with a window, those behind where the last node's begins.
+__device__ __forceinline__ int open_from(const TreeArgs& a, const TreeSeq& q) { return a.window > 0 ? max(0, q.pos0 + q.n - a.window) : 0; }
+
 // A place in a ring of N barriers, whose slots complete a phase at every turn.
 template <int N>
 struct Ring {
@@ -231,7 +237,7 @@ struct Ring {
     __device__ __forceinline__ uint32_t ahead(uint32_t by) const { return (slot + by) % N; }
 };
 
-// grid SMs, 352 threads. q as [rows][heads][HD] (map_q), map_k / map_v over one layer's store as [pages * nkv * 64, HD].
+// grid SMs, 384 threads. q as [rows][heads][HD] (map_q), map_k / map_v over one layer's store as [pages * nkv * 64, HD].
 __global__ void __launch_bounds__(THREADS, 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                const __grid_constant__ TreeArgs a, bf16* out, long long ldo, const bf16* v_store, float* ws_acc, float2* ws_ml, int* err) {
@@ -240,19 +246,20 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const uint32_t q_s = smem_u32(smem), k_s = q_s + RING, v_s = q_s + V_RING;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + BARS);
     uint64_t *k_full = bars, *k_free = k_full + NK, *v_full = k_free + NK, *v_free = v_full + NV;
-    uint64_t *s_full = v_free + NV, *p_full = s_full + 4, *o_full = p_full + 4, *v_here = o_full + 4;          // [stream][step & 1]
-    uint64_t *q_full = v_here + 4, *q_free = q_full + 1, *o_free = q_full + 2, *both = q_full + 3, *behind = q_full + 4;
+    uint64_t *v_fine = v_free + NV;                                                          // looked over
+    uint64_t *s_full = v_fine + NV, *p_full = s_full + 4, *o_full = p_full + 4;              // [stream][step & 1]
+    uint64_t *q_full = o_full + 4, *q_free = q_full + 1, *o_free = q_full + 2, *both = q_full + 3, *behind = q_full + 4;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
-    volatile int* odd_tile = reinterpret_cast<volatile int*>(bars + N_BARS + 1);       // the last tile with a value that is not finite
+    volatile int* odd_tile = reinterpret_cast<volatile int*>(bars + N_BARS + 1);       // [tile % MARKS]: the last one with a value that is not finite
     float2* ml_s = reinterpret_cast<float2*>(smem + ML);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.nh / a.nkv;
 
     pdl_wait();
     if (threadIdx.x < N_BARS) {
         uint64_t* b = bars + threadIdx.x;
-        const bool two = (b >= k_free && b < v_full) || (b >= v_free && b < s_full) || b == q_free;     // both streams say so
+        const bool two = (b >= k_free && b < v_full) || (b >= v_free && b < v_fine) || b == q_free;     // both streams say so
         mbar_init(b, b >= p_full && b < o_full ? BM : b == o_free ? SOFT + 2 : b == both ? SOFT : two ? 2 : 1);
-        *odd_tile = 0;
+        if (threadIdx.x < MARKS) odd_tile[threadIdx.x] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -307,6 +314,37 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             }
             if (!ok) atomicExch(err, 23);
         }
+    } else if (warp == CHECK_WARP) {  // ----------------------------------------------- pages that some row does not see all of
+        uint32_t tile = 0;
+        Ring<NV> rv;
+        bool ok = !DK_STALLED;
+        for (; ok && w.next(a); tile++) {
+            const int open_lo = open_from(a, w.sq);
+            for (int j = w.p0; j < w.p1 && ok; j++, rv.advance()) {
+                const int key0 = (w.sq.first_page + j) * BN, page = w.pt[j];
+                ok = __all_sync(0xffffffffu, mbar_wait(v_full + rv.slot, rv.phase));
+                if (!ok) break;
+                if (!(key0 + BN <= w.sq.pos0 && key0 >= open_lo && page >= 0 && page < a.n_pages)) {
+                    uint4* vs = reinterpret_cast<uint4*>(smem + V_RING + rv.slot * KV_BYTES);
+                    bool odd = false;
+#pragma unroll 4
+                    for (int k = lane; k < KV_BYTES / 16; k += 32) {
+                        uint4 val = vs[k];
+                        if (no_number(val.x) | no_number(val.y) | no_number(val.z) | no_number(val.w)) {
+                            vs[k] = make_uint4(numbers_of(val.x), numbers_of(val.y), numbers_of(val.z), numbers_of(val.w));
+                            odd = true;
+                        }
+                    }
+                    if (odd) {
+                        odd_tile[tile % MARKS] = (int)tile + 1;
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                    __syncwarp();
+                }
+                if (lane == 0) mbar_arrive(v_fine + rv.slot);
+            }
+        }
+        if (!ok && lane == 0) atomicExch(err, 23);
     } else if (warp >= MMA_WARP) {
         if (lane == 0) {  // ------------------------------------------------------------ a stream's tcgen05.mma
             // (One thread for both streams: a step of the two took 3,300 clocks, of which it was busy issuing for 2,100.)
@@ -361,8 +399,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 if (ok && tile > 0) ok = mbar_wait(o_free, (tile - 1) & 1);
                 for (int i = 0; i < n && ok; i++) {
                     const uint32_t step = done + i, b = step & 1;
-                    if (!see(v_full, v_free, rv, v_next, w.page_of(x, i)) || !mbar_wait(v_full + rv.slot, rv.phase)) { ok = false; break; }
-                    mbar_arrive(v_here + 2 * x + b);       // softmax warps that look at the values wait for this
+                    if (!see(v_fine, v_free, rv, v_next, w.page_of(x, i)) || !mbar_wait(v_fine + rv.slot, rv.phase)) { ok = false; break; }
                     // all that both products wait for, so that they go out in one run
                     if (i + 2 < n && !have_k(i + 2)) { ok = false; break; }
                     if (!mbar_wait(bar_p + b, (step >> 1) & 1)) { ok = false; break; }
@@ -377,7 +414,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     // into the buffer whose P was just used: products of one thread run in order
                     if (i + 2 < n) issue_s(i + 2);
                 }
-                if (ok) ok = see(k_full, k_free, rk, k_next, w.pages()) && see(v_full, v_free, rv, v_next, w.pages());
+                if (ok) ok = see(k_full, k_free, rk, k_next, w.pages()) && see(v_fine, v_free, rv, v_next, w.pages());
                 mbar_arrive(o_free);                       // the tile is not over before this thread has seen the last one's end
                 done += n;
             }
@@ -388,8 +425,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16, t_sx = t_s + lane_off + 2 * x * BN, t_ox = t_o + lane_off + x * 128;
         uint64_t *bar_s = s_full + 2 * x, *bar_p = p_full + 2 * x, *bar_o = o_full + 2 * x;
         uint32_t tile = 0, done = 0, shared_tiles = 0;
-        Ring<NK> rk;                                       // the tile's first page
-        Ring<NV> rv;
         bool ok = true;
         for (; ok && w.next(a); tile++) {
             const TreeSeq& sq = w.sq;
@@ -399,14 +434,13 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             const bool valid = qpos >= 0;
             const uint32_t* words = a.tree + (size_t)(r < rows ? node : sq.flat0) * a.words;
             const bool any_row = (warp & 3) * 32 < rows;               // else the warp has no row of the tile
-            // pages that every row sees: the cached tokens' and, with a window, none that the last node's begins in
-            const int open_lo = a.window > 0 ? max(0, sq.pos0 + sq.n - a.window) : 0;
+            const int open_lo = open_from(a, sq);
             // the places that the row sees in its sequence's last two pages, worked out while the first scores are on their way
             const int tail = max(w.p0, min(w.p1, sq.pages - 2));
             uint64_t seen_tail[2] = {0, 0};
 #pragma unroll
             for (int k = 0; k < 2; k++)
-                if (valid && tail + k < w.p1) seen_tail[k] = tree_mask(a, sq, words, qpos, (sq.first_page + tail + k) * BN);
+                if (tail + k < w.p1 && valid) seen_tail[k] = tree_mask(a, sq, words, qpos, (sq.first_page + tail + k) * BN);
             float m = -INFINITY, l = 0.f;
             int next_page = n > 0 ? w.pt[w.p0 + w.page_of(x, 0)] : 0;
             for (int i = 0; i < n && ok; i++) {
@@ -415,27 +449,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 if (i + 1 < n) next_page = w.pt[w.p0 + w.page_of(x, i + 1)];
                 const bool held = page >= 0 && page < a.n_pages;
                 const bool open = held && key0 + BN <= sq.pos0 && key0 >= open_lo;
-                if (!mbar_wait(bar_s + b, ph)) { ok = false; break; }
                 uint64_t seen = ~0ull;
-                if (!open) {
-                    seen = !held || !valid ? 0ull : j >= tail ? seen_tail[j - tail ? 1 : 0] : tree_mask(a, sq, words, qpos, key0);
-                    if (!mbar_wait(v_here + 2 * x + b, ph)) { ok = false; break; }
-                    // 16 bytes each of the page's values at a time
-                    uint4* vs = reinterpret_cast<uint4*>(smem + V_RING + rv.ahead(j - w.p0) * KV_BYTES);
-                    bool odd = false;
-#pragma unroll 2
-                    for (int k = 0; k < KV_BYTES / 16 / BM; k++) {
-                        uint4 val = vs[k * BM + r];
-                        if (no_number(val.x) | no_number(val.y) | no_number(val.z) | no_number(val.w)) {
-                            // said before it is done: the other stream may look at the page too
-                            *odd_tile = mark;
-                            __threadfence_block();
-                            val = make_uint4(numbers_of(val.x), numbers_of(val.y), numbers_of(val.z), numbers_of(val.w));
-                            vs[k * BM + r] = val, odd = true;
-                        }
-                    }
-                    if (odd) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                }
+                if (!open) seen = !held || !valid ? 0ull : j >= tail ? seen_tail[j - tail ? 1 : 0] : tree_mask(a, sq, words, qpos, key0);
+                if (!mbar_wait(bar_s + b, ph)) { ok = false; break; }
                 if (any_row) {
                     __syncwarp();
                     fence_after();
@@ -513,7 +529,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             if (any_row) {
                 __syncwarp();
                 fence_after();
-                const bool whole = w.all(), mend = *odd_tile == mark, has = n > 0, has_other = !w.pair && w.steps(1 - x) > 0;
+                const bool whole = w.all(), mend = odd_tile[tile % MARKS] == mark, has = n > 0, has_other = !w.pair && w.steps(1 - x) > 0;
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 const size_t slot = (size_t)w.slot() * 2 * BM;
                 const int row = (w.pair ? x * BM : 0) + r;
@@ -555,7 +571,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     mend_row(a, w, words, qpos, open_lo, v_store, c0, c1, whole ? dst : nullptr, ws_acc + slot * HD, row);
             }
             mbar_arrive(o_free);
-            rk.advance(w.pages() % NK), rv.advance(w.pages() % NV), done += n;
+            done += n;
         }
         if (!ok && lane == 0) atomicExch(err, 22);
     }
