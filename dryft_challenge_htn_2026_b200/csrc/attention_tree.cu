@@ -256,7 +256,7 @@ DK_EXPORT int dk_attn_tree(int f32, const void* q, long long ldq, void* out, lon
     const int G = nh / nkv, rows = dk_tree_tile_rows(max_nodes, G);
     TreeArgs a = {cu_q, seq_pos0, row_pos, page_table, tree, n_seq, words, pt_stride, n_pages, nh, nkv, window, max_nodes, rows / G, rows / G, rows,
                   pt_stride <= WHOLE_PAGES, 0, scale * 1.4426950408889634f};
-    if (!tree_units_fit(a) || nkv > 65535) return (int)cudaErrorInvalidValue;
+    if (!tree_units_fit(a) || nkv > 65535 || (!a.whole && (ws_acc == nullptr || ws_ml == nullptr))) return (int)cudaErrorInvalidValue;
 #define DK_TREE(T, NI) launch<T, NI>(a, q, ldq, out, ldo, k_store, v_store, ws_acc, ws_ml, blocks, st)
     if (f32) return rows == 16 ? DK_TREE(float, 1) : rows == 32 ? DK_TREE(float, 2) : DK_TREE(float, 4);
     return rows == 16 ? DK_TREE(bf16, 1) : rows == 32 ? DK_TREE(bf16, 2) : DK_TREE(bf16, 4);

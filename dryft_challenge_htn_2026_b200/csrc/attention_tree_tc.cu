@@ -46,7 +46,7 @@ constexpr int WHOLE_PAGES = 8;                    // tables up to here are not s
 constexpr int EXTRA = 5;                          // pages that a tile's beginning and end take as long as
 constexpr int NK = HD == 128 ? 5 : 9, NV = HD == 128 ? 4 : 8;          // pages in the rings
 constexpr int RING = 2 * Q_BYTES, V_RING = RING + NK * KV_BYTES, BARS = V_RING + NV * KV_BYTES;
-constexpr int N_BARS = 2 * NK + 3 * NV + 12 + 5;
+constexpr int N_BARS = 2 * NK + 3 * NV + 12 + 4;
 constexpr int MARKS = 16;                         // tiles that the checker may be ahead of the softmax warps: a page each at least, so no more than NV + 1
 static_assert(MARKS > NV + 1, "marks of tiles");
 constexpr int ML = BARS + (N_BARS + 1 + MARKS / 2) * 8;       // [2][2][BM] pairs (maximum, sum) that the streams exchange
@@ -248,7 +248,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     uint64_t *k_full = bars, *k_free = k_full + NK, *v_full = k_free + NK, *v_free = v_full + NV;
     uint64_t *v_fine = v_free + NV;                                                          // looked over
     uint64_t *s_full = v_fine + NV, *p_full = s_full + 4, *o_full = p_full + 4;              // [stream][step & 1]
-    uint64_t *q_full = o_full + 4, *q_free = q_full + 1, *o_free = q_full + 2, *both = q_full + 3, *behind = q_full + 4;
+    uint64_t *q_full = o_full + 4, *q_free = q_full + 1, *o_free = q_full + 2, *both = q_full + 3;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
     volatile int* odd_tile = reinterpret_cast<volatile int*>(bars + N_BARS + 1);       // [tile % MARKS]: the last one with a value that is not finite
     float2* ml_s = reinterpret_cast<float2*>(smem + ML);
@@ -388,8 +388,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     rk.advance(), k_next++;
                 };
                 ok = mbar_wait(q_full, tile & 1);
-                // B begins a tile half a step behind A: side by side their warps all reach the exponentials at the same time
-                if (ok && x == 1) ok = mbar_wait(behind, tile & 1);
                 if (ok && n == 0) umma_commit(q_free);     // one page only: nothing for B
                 for (int i = 0; i < min(n, 2) && ok; i++) {
                     ok = have_k(i);
@@ -459,7 +457,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 #pragma unroll
                     for (int c = 0; c < BN; c += 32) tmem_ld32(t_sx + b * BN + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
                     tmem_wait_ld();
-                    if (i == 0 && x == 0 && r == 0) mbar_arrive(behind);
                     float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     if (!open) {
                         const uint32_t half[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
@@ -627,7 +624,7 @@ DK_EXPORT int dk_attn_tree_tc(const void* q, long long ldq, void* out, long long
     const int G = nh / nkv;
     TreeArgs a = {cu_q, seq_pos0, row_pos, page_table, tree, n_seq, words, pt_stride, n_pages, nh, nkv, window, max_nodes, 2 * (BM / G), BM / G, BM,
                   pt_stride <= WHOLE_PAGES, EXTRA, scale * 1.4426950408889634f};
-    if (!tree_units_fit(a) || nkv > 65535) return (int)cudaErrorInvalidValue;
+    if (!tree_units_fit(a) || nkv > 65535 || (!a.whole && (ws_acc == nullptr || ws_ml == nullptr))) return (int)cudaErrorInvalidValue;
     static SmemOnce once;
     int e = once.allow((const void*)tree_tc_kernel, SMEM_BYTES);
     if (e) return e;
