@@ -855,9 +855,10 @@ def gemm_tc_check():
     if _tc_err is not None and not (_tc_err.is_cuda and torch.cuda.is_current_stream_capturing()):
         code = int(_tc_err.item())
         if code:
-            _tc_err.zero_()
-            for t in _attn_sched.values():
-                t.zero_()
+            with torch.inference_mode():       # they may have been made within a model's step, and then are written in that mode only
+                _tc_err.zero_()
+                for t in _attn_sched.values():
+                    t.zero_()
             kernel = "gemm_f32_tc" if 11 <= code <= 15 else "attention_tree" if 21 <= code <= 23 else "gemm_tc or attention_prefill_tc"
             raise KernelError(f"{kernel}: a bounded wait ran out (code {code}); its results are not valid")
 
