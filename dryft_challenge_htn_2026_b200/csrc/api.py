@@ -2199,6 +2199,11 @@ def _at(t):
     return 0 if t is None else t.data_ptr()
 
 
+def _overlap(a, b):
+    """Whether two contiguous tensors have memory in common."""
+    return a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
+
+
 TREE_MAX_NODES = 1024       # nodes of one sequence's tree
 TREE_MAX_GROUP = 64         # query heads a kv head
 MAX_BEAMS, MAX_BEST = 32, 64
@@ -2241,8 +2246,8 @@ def attention_tree(q, out, k_store, v_store, cu_q, seq_pos0, row_pos, tree, page
     but any bits may be set. With a ``window`` it sees only what lies less than that many positions before it. Rows that see nothing
     become zeros, rows behind cu_q's last are left as they were, and what lies at keys a row does not see, NaN included, does not reach
     it. A page id outside the store holds no keys. q and out [rows, heads * head_dim] (rows of wider matrices, 16-byte boundaries),
-    float32 or bfloat16, head sizes in steps of 16 up to 256. The lengths are read on the device: a captured graph may be replayed
-    with other ones, as long as ``max_nodes`` and the table's width hold."""
+    float32 or bfloat16, head sizes in steps of 16 up to 256; out may be q itself. The lengths are read on the device: a captured graph
+    may be replayed with other ones, as long as ``max_nodes`` and the table's width hold."""
     global _tc_err
     _need_rows(q, "q"), _need_rows(out, "out", q.dtype)
     _dt(q)
@@ -2317,7 +2322,7 @@ def beam_select(logits, scores, ended, scores_out, beam_out, tok_out):
     ``tok_out`` (int32), all [requests, best]. ``ended`` [requests, beams] int32 or None: a beam with a number other than 0 is at its
     end and stands for itself alone, its own score with token 0. A logit that is not finite is no candidate and weighs nothing, a beam
     whose score is not finite brings no candidates; where there are fewer than asked for the rest is (-infinity, 0, 0). Up to 32 beams
-    and 64 results, which may not lie in ``scores``."""
+    and 64 results, which may not lie in ``scores`` or ``ended``."""
     if scores.dim() != 2 or scores_out.dim() != 2 or logits.dim() != 2:
         raise KernelError("beam_select: logits, scores and results have two dimensions each")
     (requests, beams), best, V = scores.shape, scores_out.shape[1], logits.shape[1]
@@ -2329,6 +2334,9 @@ def beam_select(logits, scores, ended, scores_out, beam_out, tok_out):
     _need_all("beam_select", ((logits, "logits", torch.float32, (requests * beams, V)), (scores, "scores", torch.float32, one),
                               (ended, "ended", torch.int32, one), (scores_out, "scores_out", torch.float32, out),
                               (beam_out, "beam_out", torch.int32, out), (tok_out, "tok_out", torch.int32, out)))
+    for taken in (scores, ended):
+        if taken is not None and any(_overlap(taken, t) for t in (scores_out, beam_out, tok_out)):
+            raise KernelError("beam_select: results in the memory of scores or ended")
     lib = _lib("beam_select.cu")
     pieces = lib.dk_beam_pieces(V)
     if not lib.dk_beam_select_takes(V, beams, best):

@@ -336,6 +336,79 @@ def test_calls_on_two_streams_at_once():
     api.gemm_tc_check()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("before,width", [(60, 4), (700, 20)])       # tiles that are not split, and such that are
+def test_values_that_are_none_in_some_of_many_tiles(hd, before, width):
+    n_seq, nh, nkv = 70, 8, 4
+    c = tree_case([before + s % 9 for s in range(n_seq)], [1 + s * 7 % 12 for s in range(n_seq)], nh, nkv, hd, torch.bfloat16, seed=9, width=width)
+    clean = attend(c)
+    for s, (b, n) in enumerate(zip(c["before"], c["nodes"])):
+        page, at = c["table"][s, (b + n) // PAGE], (b + n) % PAGE        # the place behind the last node, where there is one
+        if at and s % 3 == 0:
+            c["v"][page, :, at:], c["k"][page, :, at:] = math.nan, math.inf
+    assert torch.equal(attend(c), clean)
+    hurt = torch.zeros((c["rows"], nh, hd), dtype=torch.bool, device=DEV)
+    for s in range(0, n_seq, 4):                                         # the root's value for one kv head, in every fourth sequence
+        b, row = c["before"][s], int(c["cu"][s])
+        c["v"][c["table"][s, b // PAGE], s // 4 % nkv, b % PAGE, s % hd] = -math.inf
+        hurt[row:row + c["nodes"][s], 2 * (s // 4 % nkv):2 * (s // 4 % nkv) + 2, s % hd] = True
+    got = attend(c).view(-1, nh, hd)
+    assert torch.equal(got == -math.inf, hurt) and torch.equal(got[~hurt], clean.view(-1, nh, hd)[~hurt])
+    api.gemm_tc_check()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("before", [30, 900])
+def test_tree_attention_in_place(dtype, before):
+    c = tree_case([before, 7, before + 99], [40, 9, 33], 8, 2, 128, dtype, seed=3, strided=True)
+    want = attend(c)
+    assert torch.equal(attend(c, out=c["q"]), want)
+
+
+def test_operators_one_after_another_captured_and_replayed():
+    """A step's choice and moves as one graph: accept, keep, then select, reorder of pages and states, with other contents each time."""
+    V, n_pages, nkv, hd = 5000, 20, 2, 64
+    rs = np.random.RandomState(1)
+    parents = tree_of(rs, 30)
+    logits, store = torch.zeros((30, V), device=DEV), torch.zeros((2, n_pages, nkv, PAGE, hd), dtype=torch.bfloat16, device=DEV)
+    table, states = i32(rs.permutation(n_pages)[:16].reshape(4, 4)), torch.zeros((3, 6, 40), device=DEV)
+    tok, parent, cu, pos, pos0 = i32(np.zeros(30)), i32(parents), i32([0, 30]), i32(range(100, 130)), i32([100])
+    temp, seeds = torch.zeros(1, device=DEV), i32([[3, 4]])
+    path, count, token = i32(np.zeros((1, 30))), i32([0]), i32([0])
+    scores, slots, first, last = torch.zeros((1, 4), device=DEV), i32([4, 0, 3, 1]), i32([100]), i32([131])
+    best, beam, which = torch.zeros((1, 4), device=DEV), i32(np.zeros((1, 4))), i32(np.zeros((1, 4)))
+
+    def run():
+        api.tree_accept(logits, tok, parent, cu, pos, temp, seeds, path, count, token)
+        api.kv_keep(store, table[:1], pos0, path, count)
+        api.beam_select(logits[:4], scores, None, best, beam, which)
+        api.kv_reorder(store, table, beam, first, last)
+        api.state_reorder(states, slots, beam)
+
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for seed in range(4):
+        logits.copy_(normal((30, V), seed=seed, scale=3.0))
+        scores.copy_(normal((1, 4), seed=seed + 9))
+        choice = logits.argmax(1).tolist()
+        tok.copy_(i32([0] + [choice[p] if i % 4 else 1 for i, p in enumerate(parents) if i]))
+        at = [(normal(tuple(store.shape), torch.bfloat16, seed)), normal(tuple(states.shape), seed=seed)]
+        results = []
+        for call in (run, graph.replay):
+            store.copy_(at[0]), states.copy_(at[1])
+            leave_numbers_behind()
+            call()
+            results.append([t.clone() for t in (store, states, path, count, token, best, beam, which)])
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+        assert results[1][2].tolist() == plain_accept(choice, tok.tolist(), [parents], 30)[0]
+        want = plain_select(logits[:4], scores.cpu(), None, 4)
+        assert np.array_equal(results[1][6].cpu().numpy(), want[1]) and np.array_equal(results[1][7].cpu().numpy(), want[2])
+        b = want[1][0]
+        assert torch.equal(states[:, [4, 0, 3, 1]], at[1][:, [[4, 0, 3, 1][x] for x in b]])
+
+
 def test_tree_attention_refusals():
     c = tree_case([30], [4], 4, 2, 64, torch.bfloat16)
     good = dict(q=c["q"], out=torch.empty_like(c["q"]), k_store=c["k"], v_store=c["v"], cu_q=c["cu"], seq_pos0=c["pos0"], row_pos=c["pos"],
@@ -425,6 +498,20 @@ def test_accept_takes_the_lowest_of_equal_children_ties_and_odd_logits():
     assert accept(logits, [1, 2, 4, 3, 0, 9], parents, [5] * 6, [0.0], [[1, 2]]) == ([[0, 3, -1, -1, -1, -1]], [2], [400])
     assert accept(logits, [1, 3, 3, 3, 0, 0], [[-1, 3, 0, 0, 1, -7]], [5] * 6, [0.0], [[1, 2]])[0] == [[0, 2, -1, -1, -1, -1]]
     assert accept(logits, tok, parents, [-1] * 6, [0.9], [[1, 2]])[1:] == ([1], [0])     # padding rows
+
+
+def test_accept_the_largest_tree():
+    """A line of 1,024 nodes that is right to its end, one that goes wrong on the way, and 1,023 children of one node."""
+    n = api.TREE_MAX_NODES
+    logits = normal((3 * n, 40), seed=6)
+    choice = logits.argmax(1).tolist()
+    line = list(range(-1, n - 1))
+    tok = [0] + choice[:n - 1] + [0] + choice[n:2 * n - 1] + [0] + [40] * (n - 2) + [choice[2 * n]]
+    tok[n + 700] = (tok[n + 700] + 1) % 40
+    parents = [line, line, [-1] + [0] * (n - 1)]
+    args = logits, tok, parents, [5] * (3 * n), [0.0] * 3, [[1, 2]] * 3
+    assert accept(*args) == plain_accept(choice, tok, parents, n)
+    assert accept(*args)[1] == [n, 700, 2]
 
 
 def test_accept_refusals():
@@ -528,7 +615,8 @@ def test_select_refusals():
     for bad in (dict(logits=good["logits"].double()), dict(logits=torch.zeros((5, 30), device=DEV)), dict(scores=torch.zeros((4, 1), device=DEV).half()),
                 dict(ended=i32([[0, 0]])), out(2, 65), out(2, 0), dict(beam_out=i32(np.zeros((2, 2)))), dict(tok_out=good["tok_out"].long()),
                 dict(logits=torch.zeros((66, 3), device=DEV), scores=torch.zeros((2, 33), device=DEV)), dict(logits=torch.zeros((4, 0), device=DEV)),
-                dict(scores=torch.zeros((2, 2))), out(1, 3)):
+                dict(scores=torch.zeros((2, 2))), out(1, 3), dict(scores=good["scores_out"].view(-1)[1:5].view(2, 2)),
+                dict(ended=good["tok_out"].view(-1)[:4].view(2, 2))):
         with pytest.raises(api.KernelError):
             api.beam_select(**{**good, **bad})
 
