@@ -196,6 +196,9 @@ static __device__ __noinline__ uint64_t tree_mask(const TreeArgs& a, TreeSeq q, 
     return m;
 }
 
+// Pages from this place on, up to the cached tokens' end, are seen by every row: with a window, those behind where the last node's begins.
+__device__ __forceinline__ int open_from(const TreeArgs& a, const TreeSeq& q) { return a.window > 0 ? max(0, q.pos0 + q.n - a.window) : 0; }
+
 // Merges the parts of the tiles that more than one block worked on; the others have been written. Grid (row groups of the largest
 // tree x column groups, nkv, n_seq), 256 threads: a block has 32 rows of a tile, lane k its k-th, and COLS columns, an eighth of them a
 // warp. What four parts say of a row is asked for together, or eight where a block has 64 columns.

@@ -223,9 +223,6 @@ __device__ __noinline__ void mend_row(const TreeArgs& a, const Walk& w, const ui
     }
 }
 
-// Pages from this place on, up to the cached tokens' end, are seen by every row: with a window, those behind where the last node's begins.
-__device__ __forceinline__ int open_from(const TreeArgs& a, const TreeSeq& q) { return a.window > 0 ? max(0, q.pos0 + q.n - a.window) : 0; }
-
 // A place in a ring of N barriers, whose slots complete a phase at every turn.
 template <int N>
 struct Ring {
