@@ -32,47 +32,65 @@ __device__ __forceinline__ void load4(float* dst, const bf16* src) {
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void copied() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
-// Rows ty + 16 i (i < N) of a tile against one page's keys. Thread (ty, tx) of 16 x 16 has keys tx + 16 j: each score a sum over even and
-// one over odd columns, side by side.
-template <int N, int NI>
-__device__ __forceinline__ void scores(const float* q_s, const float* k_s, float2 (&s2)[NI][4]) {
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+// How a block's 16 half-warps share a page: with more than 32 rows in the tile a half-warp h has rows h + 16 i (i < 4), with all columns and
+// all keys. With up to 32 (16) rows a warp w has rows 4 w + i (2 w + i, i < 2), its halves take half the columns of the scores, whose sums they
+// exchange, and half the keys of the values, whose sums are added up at the tile's end: what bounds the page step is what shared memory
+// returns to registers (128 bytes a clock), and a thread with four (two) rows reads each key and value for all of them. (With rows h +
+// 16 i throughout a page of 16 rows of 128 columns took 5.4 us of an SM, of 64 rows 7.4.)
+template <int R, bool SPLIT>
+struct Share {
+    static __device__ __forceinline__ int half() { return threadIdx.x >> 4 & 1; }
+    static __device__ __forceinline__ int row(int i) { return SPLIT ? (threadIdx.x >> 5) * R + i : (threadIdx.x >> 4) + 16 * i; }
+    // where the weights of the row that the half-warp reads lie
+    static __device__ __forceinline__ int p_row(int i) { return SPLIT ? 2 * row(i) + half() : row(i); }
+};
+
+// The thread's rows against one page's keys: keys tx + 16 j, each score a sum over even and one over odd columns, side by side.
+template <int R, bool SPLIT>
+__device__ __forceinline__ void scores(const float* q_s, const float* k_s, float (&sc)[R][4]) {
+    typedef Share<R, SPLIT> S;
+    const int tx = threadIdx.x & 15, d0 = SPLIT ? S::half() * (HD / 2) : 0;
+    float2 s2[R][4] = {};
+#pragma unroll 2
+    for (int dd = 0; dd < (SPLIT ? HD / 2 : HD); dd += 4) {
+        const int d = d0 + dd;
+        float4 qa[R], kb[4];
 #pragma unroll
-    for (int i = 0; i < N; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) s2[i][j] = make_float2(0.f, 0.f);
-#pragma unroll 4
-    for (int d = 0; d < HD; d += 4) {
-        float4 qa[N], kb[4];
-#pragma unroll
-        for (int i = 0; i < N; i++) qa[i] = *reinterpret_cast<const float4*>(q_s + (ty + 16 * i) * LDQ + d);
+        for (int i = 0; i < R; i++) qa[i] = *reinterpret_cast<const float4*>(q_s + S::row(i) * LDQ + d);
 #pragma unroll
         for (int j = 0; j < 4; j++) kb[j] = *reinterpret_cast<const float4*>(k_s + (tx + 16 * j) * LDK + d);
 #pragma unroll
-        for (int i = 0; i < N; i++)
+        for (int i = 0; i < R; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 s2[i][j] = fma2(make_float2(qa[i].x, qa[i].y), make_float2(kb[j].x, kb[j].y), s2[i][j]);
                 s2[i][j] = fma2(make_float2(qa[i].z, qa[i].w), make_float2(kb[j].z, kb[j].w), s2[i][j]);
             }
     }
+#pragma unroll
+    for (int i = 0; i < R; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            sc[i][j] = s2[i][j].x + s2[i][j].y;
+            if (SPLIT) sc[i][j] += __shfl_xor_sync(0xffffffffu, sc[i][j], 16);
+        }
 }
 
-// The same rows' weights and the page's values into the running results: thread (ty, tx) has VEC columns from VEC * tx + 16 VEC c on. The
-// weights go through memory of the row's 16 threads, which sit in one warp. odd: a value that is not finite lies in a page that some row
-// does not see all of, and reaches the rows that see it only.
-template <int N, int NI>
-__device__ __forceinline__ void weigh(const float2 (&s2)[NI][4], const float* v_s, float* p_s, const uint64_t* mask_s, float sl2, bool odd,
-                                      float (&m)[NI], float (&l)[NI], float (&acc)[NI][CV * VEC]) {
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float wt[N][4];
+// The same rows' weights and the page's values into the running results: thread tx has VEC columns from VEC * tx + 16 VEC c on. The
+// weights go through memory of the row's 16 threads (32 with SPLIT), which sit in one warp. odd: a value that is not finite lies in a page
+// that some row does not see all of, and reaches the rows that see it only.
+template <int R, bool SPLIT>
+__device__ __forceinline__ void weigh(float (&wt)[R][4], const float* v_s, float* p_s, const uint64_t* mask_s, float sl2, bool odd,
+                                      float (&m)[R], float (&l)[R], float (&acc)[R][CV * VEC]) {
+    typedef Share<R, SPLIT> S;
+    const int tx = threadIdx.x & 15;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const uint64_t seen = mask_s[ty + 16 * i];
+    for (int i = 0; i < R; i++) {
+        const uint64_t seen = mask_s[S::row(i)];
         float mx = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            wt[i][j] = seen >> (tx + 16 * j) & 1 ? s2[i][j].x + s2[i][j].y : -INFINITY;
+            if (!(seen >> (tx + 16 * j) & 1)) wt[i][j] = -INFINITY;
             mx = fmaxf(mx, wt[i][j]);
         }
 #pragma unroll
@@ -93,27 +111,31 @@ __device__ __forceinline__ void weigh(const float2 (&s2)[NI][4], const float* v_
     }
     struct alignas(4 * VEC) Group { float x[VEC]; };
 #pragma unroll
-    for (int half = 0; half < 2; half++) {
+    for (int turn = 0; turn < (SPLIT ? 1 : 2); turn++) {               // half a page of keys a turn, or a half-warp
+        const int half = SPLIT ? S::half() : turn;
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < N; i++)
+        for (int i = 0; i < R; i++)
 #pragma unroll
-            for (int j = 0; j < 2; j++) p_s[(ty + 16 * i) * LDP + tx + 16 * j] = wt[i][2 * half + j];
+            for (int j = 0; j < 2; j++) {
+                const float first = wt[i][j], second = wt[i][2 + j];
+                p_s[S::p_row(i) * LDP + tx + 16 * j] = half ? second : first;
+            }
         __syncwarp();
         const float* v_h = v_s + half * PK * HD;
         if (!odd) {
 #pragma unroll 2
             for (int k = 0; k < PK; k += 4) {
-                float4 w4[N];
+                float4 w4[R];
 #pragma unroll
-                for (int i = 0; i < N; i++) w4[i] = *reinterpret_cast<const float4*>(p_s + (ty + 16 * i) * LDP + k);
+                for (int i = 0; i < R; i++) w4[i] = *reinterpret_cast<const float4*>(p_s + S::p_row(i) * LDP + k);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
 #pragma unroll
                     for (int c = 0; c < CV; c++) {
                         const Group v = *reinterpret_cast<const Group*>(v_h + (k + e) * HD + (c * 16 + tx) * VEC);
 #pragma unroll
-                        for (int i = 0; i < N; i++) {
+                        for (int i = 0; i < R; i++) {
                             const float w = reinterpret_cast<const float*>(&w4[i])[e];
                             float* a = acc[i] + c * VEC;
                             if (VEC == 1) a[0] = fmaf(w, v.x[0], a[0]);
@@ -131,9 +153,9 @@ __device__ __forceinline__ void weigh(const float2 (&s2)[NI][4], const float* v_
 #pragma unroll 1
             for (int k = 0; k < PK; k++)
 #pragma unroll
-                for (int i = 0; i < N; i++)
-                    if (mask_s[ty + 16 * i] >> (half * PK + k) & 1) {
-                        const float w = p_s[(ty + 16 * i) * LDP + k];
+                for (int i = 0; i < R; i++)
+                    if (mask_s[S::row(i)] >> (half * PK + k) & 1) {
+                        const float w = p_s[S::p_row(i) * LDP + k];
 #pragma unroll
                         for (int c = 0; c < CV; c++)
 #pragma unroll
@@ -143,9 +165,111 @@ __device__ __forceinline__ void weigh(const float2 (&s2)[NI][4], const float* v_
     }
 }
 
+// weights: half a page of 64 rows, or a page of up to 32
+template <int NI> constexpr int P_FLOATS = (NI < 4 ? 32 * NI : 64) * LDP;
 template <int NI>
 constexpr size_t tree_smem() {
-    return sizeof(float) * (16 * NI * (LDQ + LDP) + DK_PAGE * (LDK + HD)) + 2 * 16 * NI * sizeof(uint64_t);
+    return sizeof(float) * (16 * NI * LDQ + P_FLOATS<NI> + DK_PAGE * (LDK + HD)) + 2 * 16 * NI * sizeof(uint64_t);
+}
+
+template <int NI>
+struct Block {                                     // a block's shared memory
+    float *q, *k, *v, *p;
+    uint64_t* masks;                               // [page & 1][row]
+    __device__ __forceinline__ Block(float* smem) {
+        q = smem, k = q + 16 * NI * LDQ, v = k + DK_PAGE * LDK, p = v + DK_PAGE * HD;
+        masks = reinterpret_cast<uint64_t*>(p + P_FLOATS<NI>);
+    }
+};
+
+// The pages of a tile that are the block's, and its rows or their part. turn: pages before.
+template <int R, bool SPLIT, int NI, typename T>
+__device__ __forceinline__ void run_tile(const TreeArgs& a, const TreeWalk& w, const Block<NI>& s, uint32_t& turn, const T* q, long long ldq, T* out,
+                                         long long ldo, const T* k_store, const T* v_store, float* ws_acc, float2* ws_ml) {
+    constexpr int TM = 16 * NI;
+    typedef Share<R, SPLIT> S;
+    const TreeSeq& sq = w.sq;
+    const int tx = threadIdx.x & 15, G = a.nh / a.nkv, kvh = w.kvh, rows = w.nodes * G, flat0 = sq.flat0 + w.node0, open_lo = open_from(a, sq);
+    auto held = [&](int page) { return page >= 0 && page < a.n_pages; };                 // a page that is none holds no keys
+    auto load = [&](float* dst, int ld, const T* store, int page) {
+        const T* src = store + kv_offset(held(page) ? page : 0, a.nkv, kvh, 0, HD);
+        for (int i = threadIdx.x; i < DK_PAGE * (HD / 4); i += THREADS) load4(dst + i / (HD / 4) * ld + (i % (HD / 4)) * 4, src + (size_t)i * 4);
+        copies_end();
+    };
+    const int pos = threadIdx.x < rows ? a.row_pos[flat0 + threadIdx.x / G] : -1;       // of row `thread`, whose masks the thread works out
+    // -> whether there is a row that does not see all of page p
+    auto mask = [&](int p, int page) {
+        if (threadIdx.x >= TM) return false;
+        const int key0 = (sq.first_page + p) * DK_PAGE;
+        const bool open = key0 + DK_PAGE <= sq.pos0 && key0 >= open_lo;
+        uint64_t seen = 0;
+        if (pos >= 0 && held(page)) seen = open ? ~0ull : tree_mask(a, sq, a.tree + (size_t)(flat0 + threadIdx.x / G) * a.words, pos, key0);
+        s.masks[(turn & 1) * TM + threadIdx.x] = seen;
+        return threadIdx.x < rows && seen != ~0ull;
+    };
+    int page = w.pt[w.p0];
+    for (int i = threadIdx.x; i < TM * (HD / 4); i += THREADS) {
+        const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
+        if (r < rows) load4(s.q + r * LDQ + c, q + (size_t)(flat0 + r / G) * ldq + (kvh * G + r % G) * HD + c);
+        else *reinterpret_cast<float4*>(s.q + r * LDQ + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    load(s.k, LDK, k_store, page);
+    bool masked = mask(w.p0, page);
+    float m[R], l[R], acc[R][CV * VEC];
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        m[i] = -INFINITY, l[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CV * VEC; c++) acc[i][c] = 0.f;
+    }
+    for (int p = w.p0; p < w.p1; p++) {
+        copied();
+        masked = __syncthreads_or(masked);                              // the keys are here, nobody reads the page before's values
+        load(s.v, HD, v_store, page);
+        const uint64_t* mask_s = s.masks + (turn++ & 1) * TM;
+        page = p + 1 < w.p1 ? w.pt[p + 1] : -1;
+        float sc[R][4];
+        scores<R, SPLIT>(s.q, s.k, sc);
+        copied();
+        __syncthreads();                                                // the values are here, nobody reads the keys
+        bool masked_next = false, odd = false;
+        if (p + 1 < w.p1) {
+            load(s.k, LDK, k_store, page);
+            masked_next = mask(p + 1, page);
+        }
+        if (masked) {
+            for (int i = threadIdx.x; i < DK_PAGE * HD; i += THREADS) odd |= !isfinite(s.v[i]);
+            odd = __syncthreads_or(odd);
+        }
+        weigh<R, SPLIT>(sc, s.v, s.p, mask_s, a.sl2, odd, m, l, acc);
+        masked = masked_next;
+    }
+    if (SPLIT)
+#pragma unroll
+        for (int i = 0; i < R; i++)
+#pragma unroll
+            for (int c = 0; c < CV * VEC; c++) acc[i][c] += __shfl_xor_sync(0xffffffffu, acc[i][c], 16);
+    if (SPLIT && S::half()) return;                                     // both halves have the sums
+    const bool whole = w.all();
+    const size_t slot = (size_t)w.slot() * TM;
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const int r = S::row(i);
+        if (r >= rows) continue;
+        const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+        T* dst = out + (size_t)(flat0 + r / G) * ldo + (kvh * G + r % G) * HD;
+        if (!whole && tx == 0) ws_ml[slot + r] = make_float2(m[i], l[i]);
+#pragma unroll
+        for (int c = 0; c < CV; c++) {
+            const int d = (c * 16 + tx) * VEC;
+            struct alignas(4 * VEC) Part { float x[VEC]; } part;
+            struct alignas(sizeof(T) * VEC) Group { T x[VEC]; } group;
+#pragma unroll
+            for (int u = 0; u < VEC; u++) part.x[u] = acc[i][c * VEC + u], group.x[u] = from_f<T>(part.x[u] * inv);
+            if (whole) *reinterpret_cast<Group*>(dst + d) = group;
+            else *reinterpret_cast<Part*>(ws_acc + slot * HD + part_at(TM, r, d)) = part;
+        }
+    }
 }
 
 // 256 threads, two blocks an SM where their shared memory allows it (64 rows of 128 columns: 111 KB). Keys and values have one buffer each:
@@ -153,98 +277,20 @@ constexpr size_t tree_smem() {
 template <typename T, int NI>
 __global__ void __launch_bounds__(THREADS, tree_smem<NI>() <= 113 * 1024 ? 2 : 1)
 tree_kernel(TreeArgs a, const T* q, long long ldq, T* out, long long ldo, const T* k_store, const T* v_store, float* ws_acc, float2* ws_ml) {
-    constexpr int TM = 16 * NI;
     extern __shared__ __align__(16) float smem[];
-    float *q_s = smem, *k_s = q_s + TM * LDQ, *v_s = k_s + DK_PAGE * LDK, *p_s = v_s + DK_PAGE * HD;
-    uint64_t* masks = reinterpret_cast<uint64_t*>(p_s + TM * LDP);      // [page & 1][row]
+    const Block<NI> s(smem);
     pdl_wait();
     pdl_launch_dependents();
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, G = a.nh / a.nkv;
     TreeWalk w;
     w.begin(a);
-    const TreeSeq& sq = w.sq;
-    uint32_t turn = 0;                                                  // pages before
+    uint32_t turn = 0;
     while (w.next(a)) {
-        const int p0 = w.p0, p1 = w.p1, kvh = w.kvh, rows = w.nodes * G, flat0 = sq.flat0 + w.node0, open_lo = open_from(a, sq);
-        const int* pt = w.pt;
-        auto held = [&](int page) { return page >= 0 && page < a.n_pages; };             // a page that is none holds no keys
-        auto load = [&](float* dst, int ld, const T* store, int page) {
-            const T* src = store + kv_offset(held(page) ? page : 0, a.nkv, kvh, 0, HD);
-            for (int i = threadIdx.x; i < DK_PAGE * (HD / 4); i += THREADS) load4(dst + i / (HD / 4) * ld + (i % (HD / 4)) * 4, src + (size_t)i * 4);
-            copies_end();
-        };
-        const int pos = threadIdx.x < rows ? a.row_pos[flat0 + threadIdx.x / G] : -1;   // of row `thread`, whose masks the thread works out
-        // -> whether there is a row that does not see all of page p
-        auto mask = [&](int p, int page) {
-            if (threadIdx.x >= TM) return false;
-            const int key0 = (sq.first_page + p) * DK_PAGE;
-            const bool open = key0 + DK_PAGE <= sq.pos0 && key0 >= open_lo;
-            uint64_t seen = 0;
-            if (pos >= 0 && held(page)) seen = open ? ~0ull : tree_mask(a, sq, a.tree + (size_t)(flat0 + threadIdx.x / G) * a.words, pos, key0);
-            masks[(turn & 1) * TM + threadIdx.x] = seen;
-            return threadIdx.x < rows && seen != ~0ull;
-        };
-        int page = pt[p0];
-        for (int i = threadIdx.x; i < TM * (HD / 4); i += THREADS) {
-            const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
-            if (r < rows) load4(q_s + r * LDQ + c, q + (size_t)(flat0 + r / G) * ldq + (kvh * G + r % G) * HD + c);
-            else *reinterpret_cast<float4*>(q_s + r * LDQ + c) = make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-        load(k_s, LDK, k_store, page);
-        bool masked = mask(p0, page);
-        float m[NI], l[NI], acc[NI][CV * VEC];
-#pragma unroll
-        for (int i = 0; i < NI; i++) {
-            m[i] = -INFINITY, l[i] = 0.f;
-#pragma unroll
-            for (int c = 0; c < CV * VEC; c++) acc[i][c] = 0.f;
-        }
-        for (int p = p0; p < p1; p++) {
-            copied();
-            masked = __syncthreads_or(masked);                          // the keys are here, nobody reads the page before's values
-            load(v_s, HD, v_store, page);
-            const uint64_t* mask_s = masks + (turn++ & 1) * TM;
-            page = p + 1 < p1 ? pt[p + 1] : -1;
-            float2 s2[NI][4];
-            if (NI >= 4 && rows > 32) scores<NI, NI>(q_s, k_s, s2);
-            else if (NI >= 2 && rows > 16) scores<(NI < 2 ? NI : 2), NI>(q_s, k_s, s2);
-            else scores<1, NI>(q_s, k_s, s2);
-            copied();
-            __syncthreads();                                            // the values are here, nobody reads the keys
-            bool masked_next = false, odd = false;
-            if (p + 1 < p1) {
-                load(k_s, LDK, k_store, page);
-                masked_next = mask(p + 1, page);
-            }
-            if (masked) {
-                for (int i = threadIdx.x; i < DK_PAGE * HD; i += THREADS) odd |= !isfinite(v_s[i]);
-                odd = __syncthreads_or(odd);
-            }
-            if (NI >= 4 && rows > 32) weigh<NI, NI>(s2, v_s, p_s, mask_s, a.sl2, odd, m, l, acc);
-            else if (NI >= 2 && rows > 16) weigh<(NI < 2 ? NI : 2), NI>(s2, v_s, p_s, mask_s, a.sl2, odd, m, l, acc);
-            else weigh<1, NI>(s2, v_s, p_s, mask_s, a.sl2, odd, m, l, acc);
-            masked = masked_next;
-        }
-        const bool whole = w.all();
-        const size_t slot = (size_t)w.slot() * TM;
-#pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const int r = ty + 16 * i;
-            if (r >= rows) continue;
-            const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
-            T* dst = out + (size_t)(flat0 + r / G) * ldo + (kvh * G + r % G) * HD;
-            if (!whole && tx == 0) ws_ml[slot + r] = make_float2(m[i], l[i]);
-#pragma unroll
-            for (int c = 0; c < CV; c++) {
-                const int d = (c * 16 + tx) * VEC;
-                struct alignas(4 * VEC) Part { float x[VEC]; } part;
-                struct alignas(sizeof(T) * VEC) Group { T x[VEC]; } group;
-#pragma unroll
-                for (int u = 0; u < VEC; u++) part.x[u] = acc[i][c * VEC + u], group.x[u] = from_f<T>(part.x[u] * inv);
-                if (whole) *reinterpret_cast<Group*>(dst + d) = group;
-                else *reinterpret_cast<Part*>(ws_acc + slot * HD + part_at(TM, r, d)) = part;
-            }
-        }
+        const int rows = w.nodes * (a.nh / a.nkv);
+#define DK_RUN(R, SPLIT) run_tile<R, SPLIT, NI, T>(a, w, s, turn, q, ldq, out, ldo, k_store, v_store, ws_acc, ws_ml)
+        if (NI == 1 || rows <= 16) DK_RUN(2, true);
+        else if (NI == 2 || rows <= 32) DK_RUN(4, true);
+        else DK_RUN(4, false);
+#undef DK_RUN
     }
 }
 
