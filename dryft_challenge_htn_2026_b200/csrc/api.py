@@ -2199,11 +2199,6 @@ def _at(t):
     return 0 if t is None else t.data_ptr()
 
 
-def _overlap(a, b):
-    """Whether two contiguous tensors have memory in common."""
-    return a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
-
-
 TREE_MAX_NODES = 1024       # nodes of one sequence's tree
 TREE_MAX_GROUP = 64         # query heads a kv head
 MAX_BEAMS, MAX_BEST = 32, 64
@@ -2334,8 +2329,9 @@ def beam_select(logits, scores, ended, scores_out, beam_out, tok_out):
     _need_all("beam_select", ((logits, "logits", torch.float32, (requests * beams, V)), (scores, "scores", torch.float32, one),
                               (ended, "ended", torch.int32, one), (scores_out, "scores_out", torch.float32, out),
                               (beam_out, "beam_out", torch.int32, out), (tok_out, "tok_out", torch.int32, out)))
-    for taken in (scores, ended):
-        if taken is not None and any(_overlap(taken, t) for t in (scores_out, beam_out, tok_out)):
+    given, results = (scores.data_ptr(), _at(ended)), (scores_out.data_ptr(), beam_out.data_ptr(), tok_out.data_ptr())
+    for at in results:                                                   # a result ends before what is given, or begins behind it
+        if -4 * requests * best < at - given[0] < 4 * requests * beams or -4 * requests * best < at - given[1] < 4 * requests * beams:
             raise KernelError("beam_select: results in the memory of scores or ended")
     lib = _lib("beam_select.cu")
     pieces = lib.dk_beam_pieces(V)
@@ -2344,8 +2340,7 @@ def beam_select(logits, scores, ended, scores_out, beam_out, tok_out):
     n = requests * beams * pieces
     ws = scores.new_empty(2 * n * (best + 2)).data_ptr()                  # pairs of doubles first, then the keys: 8 bytes each
     _check(lib, _entry(lib, "dk_beam_select", "piiii" + "p" * 8)(
-        logits.data_ptr(), V, requests, beams, best, scores.data_ptr(), _at(ended), ws + 16 * n, ws, scores_out.data_ptr(), beam_out.data_ptr(),
-        tok_out.data_ptr(), _stream_ptr()), "beam_select", 2)
+        logits.data_ptr(), V, requests, beams, best, *given, ws + 16 * n, ws, *results, _stream_ptr()), "beam_select", 2)
 
 
 def _need_store(store, page_table, what):
