@@ -111,6 +111,12 @@ def tree_arrays(parents):
     return np.array(depth, np.int64), np.array(up, np.int64), np.array(bits, np.uint32).reshape(-1, words).view(np.int32)
 
 
+def tree_table_widths(cache, slots):
+    """Columns of the page tables, a group each, in a step of trees: 8 pages or twice as many until they do, so that a sequence that grows
+    finds the shape of its last steps again."""
+    return [1 << max(3, (max(len(r) for r in cache.page_rows(g, slots)) - 1).bit_length()) for g in range(len(cache.groups))]
+
+
 def build_context(cache, entries, device, scratch_store=None, pad_to=None, plans=(), static=None, parents=None):
     """``entries``: list of (slot, tokens, want) with ``want`` positions among these tokens.
     Reserves cache room for the new tokens. ``pad_to``: for decode steps, pad the batch with rows
@@ -150,9 +156,10 @@ def build_context(cache, entries, device, scratch_store=None, pad_to=None, plans
         row_pos = np.concatenate([row_pos, -np.ones(pad, np.int64)])
         rows = pad_to
     slots = [e[0] for e in entries]
+    widths = [1] * len(cache.groups) if parents is None else tree_table_widths(cache, slots)
     tables = []
     for g in range(len(cache.groups)):
-        t = np.array(cache.page_rows(g, slots), dtype=np.int32)
+        t = np.array(cache.page_rows(g, slots, widths[g]), dtype=np.int32)
         if rows > n_seq and is_decode:   # padding rows index the table by row: give them rows of -1
             t = np.concatenate([t, -np.ones((rows - n_seq, t.shape[1]), np.int32)])
         tables.append(t)

@@ -33,9 +33,10 @@ def draft_tree(last, draft, max_nodes):
 
 
 @torch.inference_mode()
-def run_drafted(runner, prompts, params, seeds, draft, max_nodes, max_prefill_tokens=32768):
+def run_drafted(runner, prompts, params, seeds, draft, max_nodes, max_prefill_tokens=32768, graph=False):
     """Generator over the steps of one batch: yields, per step, a list with the list of new tokens of every sequence (empty once it has
-    ended). ``draft(i, tokens)`` guesses how sequence i goes on behind its prompt and output ``tokens`` (see ``draft_tree``)."""
+    ended). ``draft(i, tokens)`` guesses how sequence i goes on behind its prompt and output ``tokens`` (see ``draft_tree``). ``graph``: see
+    ``Runner.step_tree``."""
     n = len(prompts)
     tracker = BatchTracker(n, params.max_new_tokens, params.stop_token_ids)
     slots = []
@@ -70,7 +71,7 @@ def run_drafted(runner, prompts, params, seeds, draft, max_nodes, max_prefill_to
             if not who:
                 return
             trees = [draft_tree(tracker.outputs[i][-1], draft(i, list(prompts[i]) + tracker.outputs[i]), max_nodes) for i in who]
-            new = runner.step_tree([(slots[i], *t) for i, t in zip(who, trees)], params.temperature, [seeds[i] for i in who])
+            new = runner.step_tree([(slots[i], *t) for i, t in zip(who, trees)], params.temperature, [seeds[i] for i in who], graph)
     finally:
         for s in slots:
             if s is not None:

@@ -98,7 +98,7 @@ class Engine:
         params = SamplingParams(max_new_tokens, float(temperature), int(seed), tuple(stop_token_ids))
         self._ensure(input_ids, max_new_tokens + max_nodes)
         yield from run_drafted(self.runner, [list(p) for p in input_ids], params, [request_seed(seed, i) for i in range(len(input_ids))],
-                               draft, max_nodes, self.max_prefill_tokens)
+                               draft, max_nodes, self.max_prefill_tokens, self.use_graph)
 
     def beam_search(self, input_ids, beams, max_new_tokens, stop_token_ids=(), length_penalty=0.0):
         """The ``beams`` best continuations that a search of that width finds for each prompt: a list a prompt of (tokens, score), best

@@ -12,7 +12,7 @@ import torch
 from ..cache import Cache
 from ..csrc import api
 from ..sampling import seed_words
-from .batch import build_context
+from .batch import build_context, tree_table_widths
 
 GRAPH_MAX_TOKENS = 8192     # steps of more tokens are launched plainly (the reference's bound: engine/engine.py:30)
 GRAPH_KEEP = 12             # captured step shapes kept, least recently used dropped first
@@ -99,19 +99,31 @@ class Runner:
 
     def _graph_step(self, entries, with_context):
         shape = self._shape(entries)
-        if self.model.prepare(max(p + n for n, p in zip(shape[0], shape[1]))) != self._generation:
+        logits, ctx = self._graph_forward(shape, max(p + n for n, p in zip(shape[0], shape[1])), entries)
+        for slot, tokens, _ in entries:
+            self.cache.commit(slot, len(tokens))
+        api.gemm_tc_check()
+        return (logits, ctx) if with_context else logits
+
+    def _graph_forward(self, shape, positions, entries, parents=None):
+        """(logits, context) of a step of ``shape``, which reaches ``positions``; ``parents``: see ``context``."""
+        if self.model.prepare(positions) != self._generation:
             self._generation = self.model.generation
             self._graphs.clear()                      # they hold the addresses of the old tables
         sg = self._graphs.get(shape)
         if sg is None:
-            times = self._seen.pop(shape, 0)
+            times = self._seen.get(shape, 0)
+            if times == 0:                            # the first time plainly: it sizes the kernels' scratch memory
+                ctx = self.context(entries, parents=parents)
+                logits = self.model.forward(ctx, self.cache)
             self._seen[shape] = times + 1
+            self._seen.move_to_end(shape)
             while len(self._seen) > 64:
                 self._seen.popitem(last=False)
-            if times == 0:                            # the first time plainly: it sizes the kernels' scratch memory
-                return self.step(entries, with_context=with_context)
+            if times == 0:
+                return logits, ctx
             sg = _StepGraph()
-            ctx = self.context(entries, static=sg.static)
+            ctx = self.context(entries, static=sg.static, parents=parents)
             torch.cuda.synchronize()
             sg.graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(sg.graph):
@@ -122,22 +134,20 @@ class Runner:
                 self._graphs.popitem(last=False)
         else:
             self._graphs.move_to_end(shape)
-            sg.ctx = self.context(entries, static=sg.static)   # same shape: the same views, new data
+            sg.ctx = self.context(entries, static=sg.static, parents=parents)   # same shape: the same views, new data
         sg.graph.replay()
-        for slot, tokens, _ in entries:
-            self.cache.commit(slot, len(tokens))
-        api.gemm_tc_check()
-        return (sg.logits, sg.ctx) if with_context else sg.logits
+        return sg.logits, sg.ctx
 
     @torch.inference_mode()
-    def step_tree(self, entries, temperature=0.0, seeds=None):
+    def step_tree(self, entries, temperature=0.0, seeds=None, graph=False):
         """Checks trees of drafted tokens. entries: list of (slot, tokens, parents): ``tokens[0]`` is the sequence's last token, which
         is not cached yet (``parents[0]`` = -1), ``tokens[i]`` was drafted to follow node ``parents[i]`` < i. One step runs all nodes;
         from the root on the way goes to the child that holds the token the model chooses (greedy, or drawn with ``temperature`` and the
         sequence's 64-bit seed in ``seeds``, as the sampler draws at that position), and ends at the first node without one. The nodes on
         the way stay cached as the sequence's next tokens, the others' rows are given up. Returns a list an entry: the drafted
         tokens on the way and the token chosen at its end, which is not cached: between 1 and the tree's depth + 1 tokens, the ones that
-        steps of single tokens would have brought. Waits for the step."""
+        steps of single tokens would have brought. Waits for the step. ``graph``: as in ``step``; what fixes the launches of a step of
+        trees is how many sequences and nodes it has, the nodes of the largest tree, and how wide the page tables are."""
         if not self.model.takes_trees:
             raise ValueError("a layer of this model cannot take trees of drafted tokens (it is no plain attention, or keeps a state)")
         for slot, tokens, parents in entries:
@@ -147,8 +157,18 @@ class Runner:
             seeds = [0] * len(entries)
         if len(seeds) != len(entries) or temperature < 0:
             raise ValueError("one seed an entry, and a temperature that is not negative")
-        ctx = self.context([(s, t, range(len(t))) for s, t, _ in entries], parents=[list(p) for _, _, p in entries])
-        logits = self.model.forward(ctx, self.cache)
+        parents, entries = [list(p) for _, _, p in entries], [(s, t, range(len(t))) for s, t, _ in entries]
+        nodes = [len(t) for _, t, _ in entries]
+        if graph and self.device.type == "cuda" and 0 < sum(nodes) <= GRAPH_MAX_TOKENS:
+            self._check(entries)
+            for (slot, _, _), k in zip(entries, nodes):
+                self.cache.reserve(slot, k)
+            widths = tree_table_widths(self.cache, [s for s, _, _ in entries])
+            reach = max(self.cache.length[s] + k for (s, _, _), k in zip(entries, nodes))
+            logits, ctx = self._graph_forward(("trees", len(nodes), sum(nodes), max(nodes), *widths), reach, entries, parents)
+        else:
+            ctx = self.context(entries, parents=parents)
+            logits = self.model.forward(ctx, self.cache)
         n, width = len(entries), ctx.tree.max_nodes
         temps = torch.full((n,), float(temperature), device=self.device)
         words = torch.tensor([seed_words(s) for s in seeds], dtype=torch.int32, device=self.device)

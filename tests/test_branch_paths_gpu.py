@@ -113,6 +113,39 @@ def test_the_cache_behind_a_tree_is_that_of_its_accepted_tokens(tmp_path, name, 
         assert all(f == r.cache.num_pages for f in r.cache.pages_free())
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["A", "C"])
+def test_steps_of_trees_replayed_as_graphs_are_those_that_are_launched(tmp_path, name, dtype):
+    """Steps of one shape with other tokens, parents and lengths each time, over a page table that doubles and angle tables that grow."""
+    vocab = TINY[name]["vocab_size"]
+    model = load_model(make_folder(tmp_path, name, seed=23), getattr(torch, dtype))
+    a, b = Runner(model, 64 * 40), Runner(model, 64 * 40)
+    prompts = [random_tokens(vocab, L, 80 + i) for i, L in enumerate([488, 59, 2])]
+    slots = [[r.begin() for _ in prompts] for r in (a, b)]
+    for r, own in zip((a, b), slots):
+        r.step([(s, p[:-1], []) for s, p in zip(own, prompts)])
+    last, rs, replayed = [p[-1] for p in prompts], np.random.RandomState(6), 0
+    for turn in range(14):
+        sizes = [7, 3, 5] if turn % 5 else [5, 7, 3]            # as many nodes, dealt out in another way
+        trees = [([t] + rs.randint(0, vocab, k - 1).tolist(), [-1] + [int(rs.randint(0, i)) for i in range(1, k)]) for t, k in zip(last, sizes)]
+        held = len(a._graphs)
+        got = a.step_tree([(s, *t) for s, t in zip(slots[0], trees)], 0.7, [1, 2, 3], graph=True)
+        replayed += len(a._graphs) == held > 0
+        assert got == b.step_tree([(s, *t) for s, t in zip(slots[1], trees)], 0.7, [1, 2, 3])
+        last = [g[-1] for g in got]
+        assert [a.length(s) for s in slots[0]] == [b.length(s) for s in slots[1]]
+        # more tokens, as if they had been accepted: the cache grows faster than these guesses make it
+        more = [rs.randint(0, vocab, 3).tolist() for _ in prompts]
+        for r, own in zip((a, b), slots):
+            r.step([(s, [t] + m[:-1], []) for s, t, m in zip(own, last, more)])
+        last = [m[-1] for m in more]
+    assert replayed >= 8 and max(a.length(s) for s in slots[0]) > 512
+    with pytest.raises(ValueError):
+        a.step_tree([(s, [1] * k, [-1] + [k] * (k - 1)) for s, k in zip(slots[0], [7, 3, 5])], graph=True)
+    la, lb = (r.step([(s, [t], [0]) for s, t in zip(own, last)]) for r, own in zip((a, b), slots))
+    assert torch.equal(la, lb)
+
+
 def test_trees_refusals(tmp_path):
     folder = make_folder(tmp_path, "A", seed=20)
     eng = dk.Engine(folder, dtype=torch.float32)
