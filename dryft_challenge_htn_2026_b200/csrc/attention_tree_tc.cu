@@ -43,7 +43,7 @@ static_assert(HD == 64 || HD == 128, "built for head sizes 64 and 128");
 namespace {
 
 constexpr int BM = 128, BN = DK_PAGE;             // rows of a stream, keys a step (one page)
-constexpr int SOFT = 2 * BM;                      // softmax threads, one a row of each stream; two mma warps, the loader's, the checker's
+constexpr int SOFT = 2 * BM;                      // softmax threads, one a row of each stream; two mma warps, the loader's, the one that looks values over
 constexpr int THREADS = SOFT + 128, MMA_WARP = SOFT / 32, LOAD_WARP = MMA_WARP + 2, CHECK_WARP = MMA_WARP + 3;
 constexpr int TMEM_ALLOC = 512;
 constexpr int OC = 16;                            // columns of a row's result a thread handles at a time
@@ -55,7 +55,7 @@ constexpr int EXTRA = 5;                          // pages that a tile's beginni
 constexpr int NK = HD == 128 ? 5 : 9, NV = HD == 128 ? 4 : 8;          // pages in the rings
 constexpr int RING = 2 * Q_BYTES, V_RING = RING + NK * KV_BYTES, BARS = V_RING + NV * KV_BYTES;
 constexpr int N_BARS = 2 * NK + 3 * NV + 12 + 4;
-constexpr int MARKS = 16;                         // tiles that the checker may be ahead of the softmax warps: a page each at least, so no more than NV + 1
+constexpr int MARKS = 16;                         // tiles that the warp that looks values over may be ahead of the softmax warps: a page each at least, so no more than NV + 1
 static_assert(MARKS > NV + 1, "marks of tiles");
 constexpr int ML = BARS + (N_BARS + 1 + MARKS / 2) * 8;       // [2][2][BM] pairs (maximum, sum) that the streams exchange
 constexpr size_t SMEM_BYTES = 1024 + ML + 4 * BM * 8;

@@ -357,6 +357,20 @@ def test_values_that_are_none_in_some_of_many_tiles(hd, before, width):
     api.gemm_tc_check()
 
 
+@pytest.mark.parametrize("hd,dtype", [(64, torch.float32), (128, torch.float32), (48, torch.bfloat16)])
+def test_values_that_are_none_in_tiles_of_all_heights(hd, dtype):
+    """Trees whose tiles have up to 16, up to 32 and up to 64 rows, side by side in a launch."""
+    c = tree_case([61, 130, 5, 200], [40, 7, 13, 20], 4, 2, hd, dtype, seed=4)
+    clean = attend(c)
+    hurt = torch.zeros((c["rows"], 4, hd), dtype=torch.bool, device=DEV)
+    for s, (b, n) in enumerate(zip(c["before"], c["nodes"])):
+        row, j = int(c["cu"][s]), n // 2
+        c["v"][c["table"][s, (b + j) // PAGE], 1, (b + j) % PAGE, 3 + s] = math.inf
+        hurt[row:row + n, 2:, 3 + s] = torch.tensor(c["masks"][s][:, j], device=DEV)[:, None]
+    got = attend(c).view(-1, 4, hd)
+    assert torch.equal(got == math.inf, hurt) and torch.equal(got[~hurt], clean.view(-1, 4, hd)[~hurt])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("before", [30, 900])
 def test_tree_attention_in_place(dtype, before):
