@@ -84,9 +84,9 @@ class TreeRows:
     tokens cached before and its depth):
 
     place [n_tok]            where the node's key and value go: tokens cached before + its number within its tree
-    parent [n_tok]           the node it was drafted behind, -1 for a tree's root
+    parent [n_tok]           the node it was drafted behind, -1 for a tree's root (-2 for padding, whose position and place are -1)
     bits [n_tok, words]      the nodes on the way from the root to it, itself included, a bit each (csrc.api.attention_tree)
-    max_nodes                nodes of the largest tree
+    max_nodes                nodes of the largest tree, or more
     """
 
     def __init__(self, place, parent, bits, max_nodes):
@@ -117,12 +117,20 @@ def tree_table_widths(cache, slots):
     return [1 << max(3, (max(len(r) for r in cache.page_rows(g, slots)) - 1).bit_length()) for g in range(len(cache.groups))]
 
 
-def build_context(cache, entries, device, scratch_store=None, pad_to=None, plans=(), static=None, parents=None):
+def tree_bucket(n):
+    """Rows, or nodes, that a captured step of trees with ``n`` of them has: 1, 2, 4 or a multiple of 8, so that drafts whose lengths
+    differ share a few shapes."""
+    return 1 << (n - 1).bit_length() if n <= 8 else (n + 7) // 8 * 8
+
+
+def build_context(cache, entries, device, scratch_store=None, pad_to=None, plans=(), static=None, parents=None, max_nodes=0):
     """``entries``: list of (slot, tokens, want) with ``want`` positions among these tokens.
     Reserves cache room for the new tokens. ``pad_to``: for decode steps, pad the batch with rows
     of position -1 up to this many rows (a captured graph has a fixed size). ``plans``: the
     ``StepPlan`` objects of the model's parts; each is built once and uploaded with the rest.
-    ``static``: see ``_pack``. ``parents``: a list an entry where the tokens are trees (see ``tree_arrays``)."""
+    ``static``: see ``_pack``. ``parents``: a list an entry where the tokens are trees (see ``tree_arrays``); there ``pad_to`` adds nodes
+    without a position to the last tree, which no other node sees and no path reaches, and ``max_nodes`` is the least that the
+    context says of the largest tree."""
     n_seq = len(entries)
     lens = np.array([len(e[1]) for e in entries], dtype=np.int64)
     if n_seq == 0 or (lens < 1).any():
@@ -147,8 +155,16 @@ def build_context(cache, entries, device, scratch_store=None, pad_to=None, plans
     if parents is not None:
         depth, up, bits = tree_arrays(parents)
         place, row_pos = row_pos, np.repeat(pos0, lens) + depth
-        extra = [place, up, bits]
-    rows = n_tok
+    rows, largest = n_tok, int(lens.max())
+    if parents is not None:
+        pad = max(0, (pad_to or 0) - n_tok)
+        largest = max(largest, int(lens[-1]) + pad, max_nodes)
+        tok, row_seq = np.concatenate([tok, np.zeros(pad, np.int64)]), np.concatenate([row_seq, np.full(pad, n_seq - 1)])
+        row_pos, place, up = (np.concatenate([x, np.full(pad, none)]) for x, none in ((row_pos, -1), (place, -1), (up, -2)))
+        bits = np.pad(bits, ((0, pad), (0, (largest + 31) // 32 - bits.shape[1])))
+        want += range(n_tok, n_tok + pad)
+        cu[-1] += pad
+        rows, extra = n_tok + pad, [place, up, bits]
     if pad_to is not None and is_decode and pad_to > n_tok:
         pad = pad_to - n_tok
         tok = np.concatenate([tok, np.zeros(pad, np.int64)])
@@ -177,7 +193,7 @@ def build_context(cache, entries, device, scratch_store=None, pad_to=None, plans
     ctx.tables = dev[7:7 + len(tables)]
     ctx.plans = dict(zip(by_key, dev[7 + len(tables):]))
     if parents is not None:
-        ctx.tree = TreeRows(*dev[-3:], int(lens.max()))
+        ctx.tree = TreeRows(*dev[-3:], largest)
     ctx.host = dict(lens=lens, pos0=pos0, cu_q=cu, slots=slots, row_seq=row_seq, row_pos=row_pos)
     if is_decode:
         ctx.n_seq = rows  # the decode kernels run one sequence per row, padding rows included

@@ -12,7 +12,7 @@ import torch
 from ..cache import Cache
 from ..csrc import api
 from ..sampling import seed_words
-from .batch import build_context, tree_table_widths
+from .batch import build_context, tree_bucket, tree_table_widths
 
 GRAPH_MAX_TOKENS = 8192     # steps of more tokens are launched plainly (the reference's bound: engine/engine.py:30)
 GRAPH_KEEP = 12             # captured step shapes kept, least recently used dropped first
@@ -58,9 +58,10 @@ class Runner:
         if len({e[0] for e in entries}) != len(entries):
             raise ValueError("a slot appears twice in one step")
 
-    def context(self, entries, pad_to=None, static=None, parents=None):
+    def context(self, entries, pad_to=None, static=None, parents=None, max_nodes=0):
         self._check(entries)
-        ctx = build_context(self.cache, entries, self.device, self._scratch, pad_to, self.model.step_plans, static, parents)
+        ctx = build_context(self.cache, entries, self.device, self._scratch, pad_to, self.model.step_plans, static, parents,
+                            max_nodes)
         self.model.prepare(ctx.max_position + 1)     # tables grow here, never inside a step
         return ctx
 
@@ -105,8 +106,8 @@ class Runner:
         api.gemm_tc_check()
         return (logits, ctx) if with_context else logits
 
-    def _graph_forward(self, shape, positions, entries, parents=None):
-        """(logits, context) of a step of ``shape``, which reaches ``positions``; ``parents``: see ``context``."""
+    def _graph_forward(self, shape, positions, entries, **trees):
+        """(logits, context) of a step of ``shape``, which reaches ``positions``; ``trees``: what ``context`` is told of them."""
         if self.model.prepare(positions) != self._generation:
             self._generation = self.model.generation
             self._graphs.clear()                      # they hold the addresses of the old tables
@@ -114,7 +115,7 @@ class Runner:
         if sg is None:
             times = self._seen.get(shape, 0)
             if times == 0:                            # the first time plainly: it sizes the kernels' scratch memory
-                ctx = self.context(entries, parents=parents)
+                ctx = self.context(entries, **trees)
                 logits = self.model.forward(ctx, self.cache)
             self._seen[shape] = times + 1
             self._seen.move_to_end(shape)
@@ -123,7 +124,7 @@ class Runner:
             if times == 0:
                 return logits, ctx
             sg = _StepGraph()
-            ctx = self.context(entries, static=sg.static, parents=parents)
+            ctx = self.context(entries, static=sg.static, **trees)
             torch.cuda.synchronize()
             sg.graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(sg.graph):
@@ -134,7 +135,7 @@ class Runner:
                 self._graphs.popitem(last=False)
         else:
             self._graphs.move_to_end(shape)
-            sg.ctx = self.context(entries, static=sg.static, parents=parents)   # same shape: the same views, new data
+            sg.ctx = self.context(entries, static=sg.static, **trees)   # same shape: the same views, new data
         sg.graph.replay()
         return sg.logits, sg.ctx
 
@@ -147,7 +148,8 @@ class Runner:
         the way stay cached as the sequence's next tokens, the others' rows are given up. Returns a list an entry: the drafted
         tokens on the way and the token chosen at its end, which is not cached: between 1 and the tree's depth + 1 tokens, the ones that
         steps of single tokens would have brought. Waits for the step. ``graph``: as in ``step``; what fixes the launches of a step of
-        trees is how many sequences and nodes it has, the nodes of the largest tree, and how wide the page tables are."""
+        trees is how many sequences and nodes it has, the nodes of the largest tree, and how wide the page tables are, the latter three
+        rounded up."""
         if not self.model.takes_trees:
             raise ValueError("a layer of this model cannot take trees of drafted tokens (it is no plain attention, or keeps a state)")
         for slot, tokens, parents in entries:
@@ -165,7 +167,12 @@ class Runner:
                 self.cache.reserve(slot, k)
             widths = tree_table_widths(self.cache, [s for s, _, _ in entries])
             reach = max(self.cache.length[s] + k for (s, _, _), k in zip(entries, nodes))
-            logits, ctx = self._graph_forward(("trees", len(nodes), sum(nodes), max(nodes), *widths), reach, entries, parents)
+            rows = tree_bucket(sum(nodes))
+            largest = tree_bucket(max(max(nodes), nodes[-1] + rows - sum(nodes)))
+            if largest > api.TREE_MAX_NODES:
+                rows, largest = sum(nodes), max(nodes)
+            logits, ctx = self._graph_forward(("trees", len(nodes), rows, largest, *widths), reach, entries, parents=parents, pad_to=rows,
+                                              max_nodes=largest)
         else:
             ctx = self.context(entries, parents=parents)
             logits = self.model.forward(ctx, self.cache)

@@ -126,7 +126,7 @@ def test_steps_of_trees_replayed_as_graphs_are_those_that_are_launched(tmp_path,
         r.step([(s, p[:-1], []) for s, p in zip(own, prompts)])
     last, rs, replayed = [p[-1] for p in prompts], np.random.RandomState(6), 0
     for turn in range(14):
-        sizes = [7, 3, 5] if turn % 5 else [5, 7, 3]            # as many nodes, dealt out in another way
+        sizes = [7, 3, 5] if turn % 5 else [5, 2, 3]            # steps of other sizes find the same shape
         trees = [([t] + rs.randint(0, vocab, k - 1).tolist(), [-1] + [int(rs.randint(0, i)) for i in range(1, k)]) for t, k in zip(last, sizes)]
         held = len(a._graphs)
         got = a.step_tree([(s, *t) for s, t in zip(slots[0], trees)], 0.7, [1, 2, 3], graph=True)
@@ -139,7 +139,7 @@ def test_steps_of_trees_replayed_as_graphs_are_those_that_are_launched(tmp_path,
         for r, own in zip((a, b), slots):
             r.step([(s, [t] + m[:-1], []) for s, t, m in zip(own, last, more)])
         last = [m[-1] for m in more]
-    assert replayed >= 8 and max(a.length(s) for s in slots[0]) > 512
+    assert replayed >= 9 and max(a.length(s) for s in slots[0]) > 512
     with pytest.raises(ValueError):
         a.step_tree([(s, [1] * k, [-1] + [k] * (k - 1)) for s, k in zip(slots[0], [7, 3, 5])], graph=True)
     la, lb = (r.step([(s, [t], [0]) for s, t in zip(own, last)]) for r, own in zip((a, b), slots))

@@ -5,7 +5,7 @@ import torch
 
 from dryft_challenge_htn_2026_b200.cache import Cache, KVRequest, StateRequest
 from dryft_challenge_htn_2026_b200.csrc import api
-from dryft_challenge_htn_2026_b200.engine.batch import build_context, tree_arrays
+from dryft_challenge_htn_2026_b200.engine.batch import build_context, tree_arrays, tree_bucket
 from dryft_challenge_htn_2026_b200.engine.branch import draft_tree
 
 KV = KVRequest(2, 16, None, torch.float32)
@@ -32,6 +32,21 @@ def test_context_of_a_step_of_trees():
     one = build_context(cache, [(b, [8], [0])], torch.device("cpu"), parents=[[-1]])
     assert not one.is_decode and one.tree.max_nodes == 1
     assert build_context(cache, [(b, [8], [0])], torch.device("cpu")).tree is None
+
+
+def test_context_of_a_padded_step_of_trees():
+    assert [tree_bucket(n) for n in (1, 2, 3, 4, 5, 8, 9, 16, 17, 1024)] == [1, 2, 4, 4, 8, 8, 16, 16, 24, 1024]
+    cache = Cache([[KV]], max_tokens=64 * 12, max_slots=2, device="cpu")
+    a, b = cache.begin(), cache.begin()
+    cache.reserve(a, 62), cache.commit(a, 62)
+    ctx = build_context(cache, [(b, [8], range(1)), (a, [5, 6], range(2))], torch.device("cpu"), parents=[[-1], [-1, 0]], pad_to=8, max_nodes=40)
+    assert ctx.row_pos.tolist() == [0, 62, 63] + [-1] * 5 and ctx.tree.place.tolist() == [0, 62, 63] + [-1] * 5
+    assert ctx.tree.parent.tolist() == [-1, -1, 0] + [-2] * 5 and ctx.tree.bits.tolist() == [[1, 0], [1, 0], [3, 0]] + [[0, 0]] * 5
+    assert ctx.cu_q.tolist() == [0, 1, 8] and ctx.row_seq.tolist() == [0] + [1] * 7 and ctx.tok.tolist() == [8, 5, 6] + [0] * 5
+    assert ctx.want_rows.tolist() == list(range(8)) and ctx.n_tok == ctx.n_want == 8 and ctx.tree.max_nodes == 40
+    assert ctx.tables[0].shape == (2, 8) and len(cache.groups[0].pages[a]) == 1          # padding asks for no pages
+    few = build_context(cache, [(a, [5, 6], range(2))], torch.device("cpu"), parents=[[-1, 0]], pad_to=8)
+    assert few.tree.max_nodes == 8
 
 
 def test_drafts_as_trees():
