@@ -7,9 +7,10 @@
 // Where there are fewer candidates than asked for, the rest is (-infinity, 0, 0).
 //
 // Within a beam the order of the values is that of the logits, so a piece of a row can give up all but its `best` largest logits
-// before the row's sum is known: one pass over the logits. Across beams the logarithms of the sums decide: exponentials in float32
-// against the piece's maximum, added up in float32 within a thread and in double from there on, values compared in double, so that a
-// rank does not hang on the rounding of the scores (float32 scores around -30 are 2^-19 apart).
+// before the row's sum is known: one pass over the logits. Across beams the logarithms of the sums decide: exponentials in float32 of the
+// logit's distance to the piece's maximum (subtracted before it is scaled: exact where the weight is, finite for every finite logit, and the
+// same whatever is added to all logits of a row), added up in float32 within a thread and in double from there on, values compared in
+// double, so that a rank does not hang on the rounding of the scores (float32 scores around -30 are 2^-19 apart).
 //
 // First launch, a block a piece of 8,192 logits of a row, which stay in registers. A floor under the `best`-th largest: of each warp
 // the best / 8-th largest of its threads' own maxima, the least of these; few logits beside the ones looked for reach it, and these
@@ -90,10 +91,9 @@ beam_pieces_kernel(const float* logits, int V, int best, uint64_t* ws_key, doubl
         bits = top >= low ? reach(low) : 0;
         if (bits) atomicAdd(&count, __popc(bits));
         float sum = 0.f;
-        const float shift = -bm * LOG2E;
         if (bm > -INFINITY)
 #pragma unroll
-            for (int k = 0; k < EACH; k++) sum += ex2(fmaf(v[k], LOG2E, shift));
+            for (int k = 0; k < EACH; k++) sum += ex2((v[k] - bm) * LOG2E);
         double total = sum;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -177,7 +177,7 @@ beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, in
     extern __shared__ __align__(16) unsigned char dyn[];
     Candidate* found = reinterpret_cast<Candidate*>(dyn);
     __shared__ Candidate tops[THREADS], least;
-    __shared__ double offset[MAX_BEAMS];
+    __shared__ double highest[MAX_BEAMS], offset[MAX_BEAMS];            // a live beam: its largest logit, score - log(sum) against that
     __shared__ int kind[MAX_BEAMS];                                      // 0: not live, 1: live, 2: at its end
     __shared__ int count;
     const Candidate none = {0, -1};
@@ -210,7 +210,7 @@ beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, in
         }
         if (lane == 0) {
             kind[b] = !isfinite(score) ? 0 : done ? 2 : sum > 0. ? 1 : 0;
-            offset[b] = kind[b] == 1 ? (double)score - (m + log(sum)) : (double)score;
+            highest[b] = m, offset[b] = kind[b] == 1 ? (double)score - log(sum) : (double)score;
         }
     }
     if (t == 0) count = 0, least = none;
@@ -220,7 +220,7 @@ beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, in
         const int b = l / pieces;
         if (kind[b] == 2) return rank == 0 && l == b * pieces ? candidate(offset[b], b * V) : none;
         const uint64_t key = kind[b] == 1 ? keys[l * best + rank] : 0;
-        return key ? candidate((double)logit_of(key) + offset[b], b * V + index_of(key)) : none;
+        return key ? candidate(((double)logit_of(key) - highest[b]) + offset[b], b * V + index_of(key)) : none;
     };
     Candidate top = none;
     for (int l = t; l < lists; l += THREADS) {

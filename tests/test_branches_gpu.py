@@ -613,6 +613,82 @@ def test_select_ties_masks_and_beams_that_are_not_live():
     check_select(up, torch.tensor([[-1.0, -1.0, -1.5], [-2.0, -1.0, -1.0]], device=DEV), None, 64)
 
 
+def exact_select(logits, scores, best):
+    """``plain_select`` without ends, the maximum taken off before anything else is added, so that numbers of any size keep their differences."""
+    (r, b), z = scores.shape, logits.double().cpu().numpy()
+    V, out = z.shape[1], []
+    for i in range(r):
+        value = np.full((b, V), -math.inf)
+        for j in range(b):
+            x = z[i * b + j]
+            ok = np.isfinite(x)
+            if ok.any():
+                d = x[ok] - x[ok].max()
+                value[j, ok] = d + (float(scores[i, j]) - np.log(np.exp(d).sum()))
+        flat = value.reshape(-1)
+        order = np.lexsort((np.arange(b * V), -flat))[:best]
+        out.append((flat[order], order // V, order % V))
+    return [np.stack(x) for x in zip(*out)]
+
+
+def check_exact_select(logits, scores, best):
+    got, want = select(logits, scores, None, best), exact_select(logits, scores.cpu(), best)
+    assert np.array_equal(got[1].numpy(), want[1]) and np.array_equal(got[2].numpy(), want[2])
+    assert np.all(np.abs(got[0].numpy() - want[0]) <= 2 ** -24 * np.abs(want[0]) + 2 ** -22)      # as in check_select
+
+
+LOWEST = torch.finfo(torch.float32).min
+
+
+@pytest.mark.parametrize("masked", ["a piece", "the last piece", "all but a few", "a whole beam", "one beam's all but one"])
+def test_select_with_the_lowest_number_as_a_mask(masked):
+    """The lowest finite number is a logit like others: it weighs nothing beside ordinary ones, and a piece that holds nothing else costs a
+    beam nothing."""
+    logits = normal((6, 8192 * 2 + 500), seed=4, scale=3.0)
+    scores = torch.tensor([[-3.0, -2.5, -4.0], [-20.0, -21.0, -20.5]], device=DEV)
+    if masked == "a piece":
+        logits[:, :8192 + 4] = LOWEST                       # (a row may begin up to three places into its first piece)
+        logits[1, :], logits[1, 8300:8310] = LOWEST, torch.arange(10, device=DEV).float()
+    elif masked == "the last piece":
+        logits[:, 2 * 8192 - 4:] = LOWEST
+    elif masked == "all but a few":
+        keep = logits[:, [7, 9000, 16800]].clone()
+        logits[:] = LOWEST
+        logits[:, [7, 9000, 16800]] = keep
+        return check_exact_select(logits, scores, 9)        # those of all three beams, and no more
+    elif masked == "a whole beam":
+        logits[1], logits[3] = LOWEST, LOWEST               # equal everywhere: its tokens are the best ones where its score is far above the others
+        scores[0, 1] = 8.0
+    else:
+        logits[2] = LOWEST
+        logits[2, 12000] = 1.5
+    check_exact_select(logits, scores, 16)
+
+
+def test_select_of_the_largest_numbers():
+    logits = normal((4, 20000), seed=5, scale=3.0)
+    logits[0, [5, 9000, 19000]] = torch.tensor([3.3e38, 3.4e38, -3.4e38], device=DEV)      # one token has all the weight
+    logits[3] = logits[3] * 1e37
+    check_exact_select(logits, torch.tensor([[-3.0, -2.0], [-1.0, -50.0]], device=DEV), 3)
+
+
+@pytest.mark.parametrize("above", [0.0, 24.5, 315.25, 1000.125, -3000.5, 32768.0, 1048576.0])
+def test_select_does_not_hang_on_a_number_added_to_all_logits(above):
+    """Logits in steps of 1/8 (2^20 + 16 and that has its 24 bits), so the sum with ``above`` is exact and the log-probabilities are the same. Beams
+    whose scores are one step of float32 apart take turns; their order is the one of the scores whichever of them is moved."""
+    base = (normal((1, 30000), seed=6, scale=3.0) * 8).round() / 8
+    base = base + torch.arange(30000, device=DEV).eq(777) * 4
+    logits = base.repeat(8, 1)
+    logits[1::4] += above
+    logits[2::4] += above
+    logits[3::4] -= above
+    scores = torch.tensor([-20.0, -20.0 - 2 ** -19, -20.0, -20.0 + 2 ** -19, -9.5, -9.5 - 2 ** -20, -9.5 - 2 ** -19, -9.5], device=DEV).view(2, 4)
+    got, same = select(logits, scores, None, 24), select(base.repeat(8, 1), scores, None, 24)
+    assert torch.equal(got[1], same[1]) and torch.equal(got[2], same[2])
+    assert torch.equal(got[0], same[0])
+    check_exact_select(logits, scores, 24)
+
+
 def test_select_from_memory_that_is_not_aligned_and_twice():
     base = normal((1 + 4 * 1000,), seed=3)
     logits = base[1:].view(4, 1000)
