@@ -2240,8 +2240,8 @@ def attention_tree(q, out, k_store, v_store, cu_q, seq_pos0, row_pos, tree, page
     whose bit (word j / 32, bit j % 32) is set in its row of ``tree`` [rows, words] int32: of a drafted tree its ancestors and itself,
     but any bits may be set. With a ``window`` it sees only what lies less than that many positions before it. Rows that see nothing
     become zeros, rows behind cu_q's last are left as they were, and what lies at keys a row does not see, NaN included, does not reach
-    it. A page id outside the store holds no keys. q and out [rows, heads * head_dim] (rows of wider matrices, 16-byte boundaries),
-    float32 or bfloat16, head sizes in steps of 16 up to 256; out may be q itself. The lengths are read on the device: a captured graph
+    it. A page id outside the store holds no keys. q and out [rows, heads * head_dim] (rows of wider matrices) and the stores, on 16-byte
+    boundaries, float32 or bfloat16, head sizes in steps of 16 up to 256; out may be q itself. The lengths are read on the device: a captured graph
     may be replayed with other ones, as long as ``max_nodes`` and the table's width hold."""
     global _tc_err
     _need_rows(q, "q"), _need_rows(out, "out", q.dtype)
@@ -2262,8 +2262,9 @@ def attention_tree(q, out, k_store, v_store, cu_q, seq_pos0, row_pos, tree, page
         raise KernelError("attention_tree: a store, page table or row of tree bits that is empty, or a store of 2^31 rows")
     if not scale > 0 or (window or 0) < 0:
         raise KernelError(f"attention_tree: scale {scale} must be positive, window {window} not negative")
-    if (q.data_ptr() | out.data_ptr() | q.stride(0) * q.element_size() | out.stride(0) * q.element_size()) % 16:
-        raise KernelError("attention_tree: rows of q and out must lie on 16-byte boundaries")
+    k_at, v_at = k_store.data_ptr(), v_store.data_ptr()
+    if (q.data_ptr() | out.data_ptr() | k_at | v_at | q.stride(0) * q.element_size() | out.stride(0) * q.element_size()) % 16:
+        raise KernelError("attention_tree: rows of q and out, k_store and v_store must lie on 16-byte boundaries")
     if q.get_device() != cu_q.get_device() or out.get_device() != cu_q.get_device():
         raise KernelError("attention_tree: q and out must be on the current device")
     if rows == 0:
@@ -2274,7 +2275,7 @@ def attention_tree(q, out, k_store, v_store, cu_q, seq_pos0, row_pos, tree, page
     ws = q.new_empty(n + 4 * blocks * tile, dtype=torch.float32) if n else None
     parts = _at(ws)
     head = (q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0))
-    body = (k_store.data_ptr(), v_store.data_ptr(), n_pages, cu_q.data_ptr(), seq_pos0.data_ptr(), row_pos.data_ptr(), tree.data_ptr(), words,
+    body = (k_at, v_at, n_pages, cu_q.data_ptr(), seq_pos0.data_ptr(), row_pos.data_ptr(), tree.data_ptr(), words,
             page_table.data_ptr(), table, n_seq, n_heads, n_kv_heads, window or 0, scale, max_nodes, parts, parts + 4 * n, blocks)
     if tc:
         if _tc_err is None:

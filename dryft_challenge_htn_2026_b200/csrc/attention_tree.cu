@@ -338,13 +338,15 @@ DK_EXPORT int dk_attn_tree_blocks(int f32, int max_nodes, int group) {
     return (per_sm > 0 ? per_sm : 1) * sms;
 }
 
-// q [rows, nh*HD] and out [rows, nh*HD], rows ldq / ldo elements apart; k_store, v_store [n_pages, nkv, 64, HD]; ws_acc: 2 * blocks *
-// tile rows * HD floats, ws_ml: 2 * blocks * tile rows * 2 floats. f32 != 0: float32 storage, else bfloat16.
+// q [rows, nh*HD] and out [rows, nh*HD], rows ldq / ldo elements apart; k_store, v_store [n_pages, nkv, 64, HD]; all on 16-byte
+// boundaries, q's and out's rows too: what is read and written is 16 bytes (bfloat16: 8) at a time. ws_acc: 2 * blocks * tile rows * HD floats, ws_ml: 2 * blocks * tile rows * 2 floats. f32 != 0: float32 storage, else bfloat16.
 DK_EXPORT int dk_attn_tree(int f32, const void* q, long long ldq, void* out, long long ldo, const void* k_store, const void* v_store,
                            int n_pages, const int* cu_q, const int* seq_pos0, const int* row_pos, const uint32_t* tree, int words,
                            const int* page_table, int pt_stride, int n_seq, int nh, int nkv, int window, float scale, int max_nodes,
                            float* ws_acc, float* ws_ml, int blocks, cudaStream_t st) {
-    if (nkv < 1 || nh % nkv || nh / nkv > 64 || n_pages < 1 || pt_stride < 1 || words < 1 || blocks < 1 || max_nodes < 1 || n_seq > 65535)
+    const int size = f32 ? 4 : 2;
+    if (nkv < 1 || nh % nkv || nh / nkv > 64 || n_pages < 1 || pt_stride < 1 || words < 1 || blocks < 1 || max_nodes < 1 || n_seq > 65535 ||
+        ldq * size % 16 || ldo * size % 16 || ((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_store | (uintptr_t)v_store) % 16)
         return (int)cudaErrorInvalidValue;
     const int G = nh / nkv, rows = dk_tree_tile_rows(max_nodes, G);
     TreeArgs a = {cu_q, seq_pos0, row_pos, page_table, tree, n_seq, words, pt_stride, n_pages, nh, nkv, window, max_nodes, rows / G, rows / G, rows,

@@ -617,14 +617,14 @@ int make_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dim
 DK_EXPORT int dk_tree_tc_tile_rows() { return 2 * BM; }
 DK_EXPORT int dk_tree_tc_whole_pages() { return WHOLE_PAGES; }
 
-// q [n_rows, nh*HD] and out, bf16, rows ldq / ldo elements apart (multiples of 8, 16-byte boundaries); k_store, v_store [n_pages, nkv, 64,
-// HD]; ws_acc: 2 * blocks * 256 * HD floats, ws_ml: 2 * blocks * 256 * 2 floats; err: device int for a wait that ran out.
+// q [n_rows, nh*HD] and out, bf16, rows ldq / ldo elements apart (multiples of 8); k_store, v_store [n_pages, nkv, 64, HD]; all on 16-byte
+// boundaries; ws_acc: 2 * blocks * 256 * HD floats, ws_ml: 2 * blocks * 256 * 2 floats; err: device int for a wait that ran out.
 DK_EXPORT int dk_attn_tree_tc(const void* q, long long ldq, void* out, long long ldo, long long n_rows, const void* k_store,
                               const void* v_store, int n_pages, const int* cu_q, const int* seq_pos0, const int* row_pos,
                               const uint32_t* tree, int words, const int* page_table, int pt_stride, int n_seq, int nh, int nkv, int window,
                               float scale, int max_nodes, float* ws_acc, float* ws_ml, int blocks, int* err, cudaStream_t st) {
     if (nkv < 1 || nh % nkv || nh / nkv > 64 || n_pages < 1 || pt_stride < 1 || words < 1 || blocks < 1 || max_nodes < 1 || n_seq > 65535 ||
-        err == nullptr || ldq % 8 || ldo % 8 || ((uintptr_t)q | (uintptr_t)out) % 16 || (long long)n_pages * nkv * DK_PAGE > 0x7fffffffLL)
+        err == nullptr || ldq % 8 || ldo % 8 || ((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_store | (uintptr_t)v_store) % 16 || (long long)n_pages * nkv * DK_PAGE > 0x7fffffffLL)
         return (int)cudaErrorInvalidValue;
     const int G = nh / nkv;
     TreeArgs a = {cu_q, seq_pos0, row_pos, page_table, tree, n_seq, words, pt_stride, n_pages, nh, nkv, window, max_nodes, 2 * (BM / G), BM / G, BM,

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from dryft_challenge_htn_2026_b200.cache import Cache, KVRequest, StateRequest
-from dryft_challenge_htn_2026_b200.csrc import api
+from dryft_challenge_htn_2026_b200.csrc import api, build
 from dryft_challenge_htn_2026_b200.engine.batch import build_context, tree_arrays, tree_bucket
 from dryft_challenge_htn_2026_b200.engine.branch import draft_tree
 
@@ -91,3 +91,23 @@ def test_refusals_come_before_a_device_is_needed():
         api.kv_reorder(torch.zeros(1, 1, 64, 8), i.view(4, 1), i.view(2, 2), i[:2], i[:2])
     with pytest.raises(api.KernelError):
         api.state_reorder(torch.zeros(1, 4, 8), i, i.view(2, 2))
+
+
+@pytest.mark.parametrize("source,hd", [("attention_tree.cu", 64), ("attention_tree.cu", 16), ("attention_tree_tc.cu", 128)])
+def test_addresses_that_are_not_aligned_are_refused_by_the_entry_points(source, hd):
+    """Every address and row distance that the kernels take in 16 bytes; the answer comes before anything is asked of a device."""
+    lib = build.load_lib(source, {"HD": hd})
+    invalid, at = 1, 1 << 20                                               # cudaErrorInvalidValue; an address that nothing is read from
+
+    def call(q=at, ldq=2 * hd, out=at, ldo=2 * hd, k=at, v=at, f32=0):
+        body = (k, v, 4, at, at, at, at, 1, at, 64, 1, 2, 1, 0, 1.0, 4, at, at, 4)
+        if source == "attention_tree_tc.cu":
+            return api._entry(lib, "dk_attn_tree_tc", "pqpqq" + "ppippppipiiiiifippi" + "pp")(q, ldq, out, ldo, 4, *body, at, 0)
+        return api._entry(lib, "dk_attn_tree", "ipqpq" + "ppippppipiiiiifippi" + "p")(f32, q, ldq, out, ldo, *body, 0)
+
+    for f32 in (0, 1)[:1 if "tc" in source else 2]:
+        for off in (2, 4, 8):
+            for name in ("q", "out", "k", "v"):
+                assert call(**{name: at + off}, f32=f32) == invalid, (name, off)
+        for name in ("ldq", "ldo"):
+            assert call(**{name: 2 * hd + 2}, f32=f32) == invalid, name

@@ -437,6 +437,17 @@ def test_tree_attention_refusals():
             api.attention_tree(**{**good, **bad})
 
 
+@pytest.mark.parametrize("dtype,hd", [(torch.float32, 64), (torch.bfloat16, 48), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("name", ["k", "v"])
+def test_tree_attention_refuses_stores_that_are_not_aligned(dtype, hd, name):
+    c = tree_case([30], [4], 4, 2, hd, dtype)
+    attend(c)
+    for off in (1, 16 // c["k"].element_size() - 1):
+        odd = torch.zeros(c["k"].numel() + 16, dtype=dtype, device=DEV)[off:off + c["k"].numel()].view_as(c["k"])
+        with pytest.raises(api.KernelError, match="16-byte"):
+            attend(dict(c, **{name: odd}))
+
+
 # ------------------------------------------------------------------------------------------------ accept
 def sampler_choice(logits, pos, temperature, seeds):
     """The token ``sample`` chooses for each row."""
