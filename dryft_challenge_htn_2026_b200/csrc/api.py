@@ -2306,10 +2306,11 @@ def tree_accept(logits, tok, parent, cu_q, row_pos, temperature, seeds, path, n_
                               (n_path, "n_path", torch.int32, (n_seq,)), (next_tok, "next_tok", torch.int32, (n_seq,))))
     lib = _lib("tree_accept.cu")
     n = max(1, rows * lib.dk_tree_accept_pieces(V, n_seq, max_nodes))
-    ws = tok.new_empty(2 * n).data_ptr()
+    ws = tok.new_empty(2 * n)                     # held until both launches are made: another thread may ask for memory on this stream meanwhile
+    at = ws.data_ptr()
     _check(lib, _entry(lib, "dk_tree_accept", "pi" + "p" * 6 + "ii" + "p" * 6)(
         logits.data_ptr(), V, tok.data_ptr(), parent.data_ptr(), cu_q.data_ptr(), row_pos.data_ptr(), temperature.data_ptr(), seeds.data_ptr(),
-        n_seq, max_nodes, ws, ws + 4 * n, path.data_ptr(), n_path.data_ptr(), next_tok.data_ptr(), _stream_ptr()), "tree_accept", 2)
+        n_seq, max_nodes, at, at + 4 * n, path.data_ptr(), n_path.data_ptr(), next_tok.data_ptr(), _stream_ptr()), "tree_accept", 2)
 
 
 def beam_select(logits, scores, ended, scores_out, beam_out, tok_out):
@@ -2339,9 +2340,10 @@ def beam_select(logits, scores, ended, scores_out, beam_out, tok_out):
     if not lib.dk_beam_select_takes(V, beams, best):
         raise KernelError(f"beam_select: {best} of {beams} beams over {V} tokens need more shared memory than a block has")
     n = requests * beams * pieces
-    ws = scores.new_empty(2 * n * (best + 2)).data_ptr()                  # pairs of doubles first, then the keys: 8 bytes each
+    ws = scores.new_empty(2 * n * (best + 2))     # pairs of doubles first, then the keys: 8 bytes each; held as in tree_accept
+    at = ws.data_ptr()
     _check(lib, _entry(lib, "dk_beam_select", "piiii" + "p" * 8)(
-        logits.data_ptr(), V, requests, beams, best, *given, ws + 16 * n, ws, *results, _stream_ptr()), "beam_select", 2)
+        logits.data_ptr(), V, requests, beams, best, *given, at + 16 * n, at, *results, _stream_ptr()), "beam_select", 2)
 
 
 def _need_store(store, page_table, what):

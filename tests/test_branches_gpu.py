@@ -1,6 +1,7 @@
 """Trees of drafted tokens and beams: attention of a tree over the cache, the path that is accepted, the best continuations of beams,
 and the moves of cache rows and states, each against a plain implementation in 64 bits (moves: against the same moves on the host)."""
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -334,6 +335,54 @@ def test_calls_on_two_streams_at_once():
         for (out, best), (a, b, _) in zip(got, want):
             assert torch.equal(out, a) and all(torch.equal(p.cpu(), q) for p, q in zip(best, b))
     api.gemm_tc_check()
+
+
+def test_scratch_memory_is_held_until_the_launches_are_made(monkeypatch):
+    """Memory that is given back before the C entry is called is another thread's to take, on the same stream too: its first launch would lie
+    between the two of this call."""
+    real, held = api._entry, []
+
+    def entry(lib, name, kinds):
+        def call(*args):
+            for size in [1 << k for k in range(9, 24)] * 8:              # what another thread may ask for meanwhile
+                held.append(torch.empty(size, dtype=torch.uint8, device=DEV))
+            took = [(t.data_ptr(), t.data_ptr() + t.numel()) for t in held]
+            lost = [a for a in args if isinstance(a, int) and any(lo <= a < hi for lo, hi in took)]
+            assert not lost, f"{name}: its scratch memory was taken"
+            return real(lib, name, kinds)(*args)
+        return call
+
+    monkeypatch.setattr(api, "_entry", entry)
+    cases = [lambda: attend(tree_case([900, 2000], [40, 7], 8, 2, 128, torch.bfloat16)),
+             lambda: attend(tree_case([900, 2000], [40, 7], 8, 2, 64, torch.float32)),
+             lambda: accept(normal((12, 50000), seed=2), [3] * 12, [[-1] + list(range(11))], list(range(12)), [0.7], [[5, 6]]),
+             lambda: select(normal((12, 50000), seed=2), torch.zeros((3, 4), device=DEV), None, 8)]
+    for case in cases:
+        held.clear()
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        case()
+
+
+def test_two_threads_on_one_stream():
+    logits = [normal((64, 20000), seed=20 + i, scale=3.0) for i in range(2)]
+    scores = torch.zeros((16, 4), device=DEV)
+    tree = ([3] * 64, [[-1] + list(range(63))], list(range(64)), [0.7], [[5, 6]])
+    want = [(select(x, scores, None, 16), accept(x, *tree)) for x in logits]
+    wrong = []
+
+    def work(k):
+        for _ in range(200):
+            got = select(logits[k], scores, None, 16), accept(logits[k], *tree)
+            if not all(torch.equal(a, b) for a, b in zip(got[0], want[k][0])) or got[1] != want[k][1]:
+                wrong.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 @pytest.mark.parametrize("hd", [64, 128])
