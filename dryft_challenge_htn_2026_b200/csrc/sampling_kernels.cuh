@@ -17,7 +17,9 @@ __device__ __forceinline__ float gumbel(uint32_t seed_lo, uint32_t seed_hi, uint
     uint32_t x = mix32(idx ^ 0x9E3779B9u);
     x = mix32(x + pos * 0x85EBCA6Bu + seed_lo);
     x = mix32(x ^ seed_hi);
-    const float u = ((float)(x >> 8) + 0.5f) * (1.0f / 16777216.0f);
+    // below 1: the largest hash value rounds up to 2^24, and with u = 1 the noise would be infinite. (At one logit in 2^24 that is every
+    // 110th token of a vocabulary of 151,936 drawn whatever its logit is.)
+    const float u = fminf(((float)(x >> 8) + 0.5f) * (1.0f / 16777216.0f), 0.99999994f);
     return -logf(-logf(u));
 }
 

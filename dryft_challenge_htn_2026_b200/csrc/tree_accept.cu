@@ -62,10 +62,10 @@ accept_pieces_kernel(const float* logits, int V, const int* cu_q, const int* row
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int i = piece.at(q) + e;
-                const uint32_t x = mix32(mix32(mix32((uint32_t)i ^ 0x9E3779B9u) + mid) ^ hi) >> 8, d = 0xffffffu - x;   // as gumbel() makes them
-                // u is (x + 0.5) / 2^24 to the nearest float32, so 1 - u is d / 2^24 at least; where d is 0, u is 1 and the noise infinite
+                const uint32_t x = mix32(mix32(mix32((uint32_t)i ^ 0x9E3779B9u) + mid) ^ hi) >> 8, d = max(0xffffffu - x, 1u);   // as gumbel() makes them
+                // u is (x + 0.5) / 2^24 to the nearest float32, 1 - 2^-24 at most, so 1 - u is d / 2^24 at least
                 const float most = 0.6931472f * (24.f - __log2f((float)d)) + 1e-3f;
-                if (d == 0 || v[e] * inv_t + most >= bv) better(bv, bi, v[e] * inv_t + gumbel(lo, hi, (uint32_t)(pos + 1), (uint32_t)i), i);
+                if (v[e] * inv_t + most >= bv) better(bv, bi, v[e] * inv_t + gumbel(lo, hi, (uint32_t)(pos + 1), (uint32_t)i), i);
             }
         }
     }

@@ -558,6 +558,59 @@ def test_accept(vocab, temperature):
     assert max(got[1]) > 3 or vocab > 10 ** 9
 
 
+def noise_words(lo, hi, pos, V):
+    """The top 24 bits of the sampler's hash of tokens 0 to V (the noise is -log(-log u), u = (word + 1/2) / 2^24)."""
+    u32, m = np.uint32, 0xffffffff
+
+    def mix(x):
+        x = (x ^ x >> u32(16)) * u32(0x7FEB352D)
+        x = (x ^ x >> u32(15)) * u32(0x846CA68B)
+        return x ^ x >> u32(16)
+
+    x = mix(np.arange(V, dtype=u32) ^ u32(0x9E3779B9))
+    return mix(mix(x + u32((pos * 0x85EBCA6B + lo) & m)) ^ u32(hi)) >> u32(8)
+
+
+def test_drawn_tokens_are_never_ones_that_have_no_chance():
+    """All but 500 of 50,001 tokens are e^40 times less likely than the others. Among the hash values are some whose u would be 1 if it were
+    rounded, and the noise infinite; the largest noise there may be is -log(-log(1 - 2^-24)) = 16.6."""
+    V, rows, lo, hi = 50001, 1000, 12345, 0x9abcdef0
+    logits = torch.full((rows, V), -40.0, device=DEV)
+    logits[:, :500] = normal((rows, 500), seed=8)
+    words = [noise_words(lo, hi, p + 1, V) for p in range(rows)]
+    assert sum(int((w[500:] == 0xffffff).any()) for w in words) >= 2
+    seeds = i32(np.array([[lo, hi]], np.uint32).view(np.int32))
+    got = np.array(sampler_choice(logits, i32(range(rows)), torch.ones(rows, device=DEV), seeds.repeat(rows, 1)))
+    assert got.max() < 500
+    u = np.minimum((np.stack(words)[:, :500] + 0.5) / 2 ** 24, 1 - 2.0 ** -24)
+    noise = -np.log(-np.log(u))
+    value = logits[:, :500].double().cpu().numpy() + noise
+    # u in float32 is off by half a step of 2^-24 at most, the noise by that over -u log u: 2.5e-4 where the noise is below 9; two tokens
+    gap, row, best = value.max(1) - value[np.arange(rows), got], np.arange(rows), value.argmax(1)
+    assert np.all((gap < 1e-3) | (np.maximum(noise[row, got], noise[row, best]) > 9)) and (gap == 0).mean() > 0.98
+    for at in [p for p, w in enumerate(words) if (w == 0xffffff).any()] + list(range(0, rows, 97)):
+        one = accept(logits[at:at + 1], [0], [[-1]], [at], [1.0], seeds.tolist())
+        assert one == ([[0]], [1], [int(got[at])])
+
+
+def test_the_largest_noise_wins_where_it_is_enough():
+    """The token with the largest hash value has the noise -log(-log(1 - 2^-24)), in both operators: more than any other's."""
+    V, lo, hi = 151936, 77, 0x1234567
+    at = next(p for p in range(2000) if (noise_words(lo, hi, p + 1, V) == 0xffffff).any())
+    token = int(np.flatnonzero(noise_words(lo, hi, at + 1, V) == 0xffffff)[0])
+    u = np.minimum((noise_words(lo, hi, at + 1, V) + 0.5) / 2 ** 24, 1 - 2.0 ** -24)
+    noise = -np.log(-np.log(u))
+    second = np.sort(noise)[-2]
+    seeds = i32([[lo, hi]])
+    for temperature in (1.0, 0.5):
+        for below in (-1.0, 1.0):                            # by so much the others' best falls short of the token, or is ahead of it
+            logits = torch.zeros((1, V), device=DEV)
+            logits[0, token] = (second - noise[token] - below) * temperature
+            want = token if below < 0 else int(np.argsort(noise)[-2])
+            assert sampler_choice(logits, i32([at]), torch.tensor([temperature], device=DEV), seeds) == [want]
+            assert accept(logits, [0], [[-1]], [at], [temperature], [[lo, hi]]) == ([[0]], [1], [want])
+
+
 def test_accept_takes_the_lowest_of_equal_children_ties_and_odd_logits():
     logits = torch.zeros((6, 500), device=DEV)
     logits[0, [7, 3]] = 5.0                              # a tie: the lower token
