@@ -86,7 +86,7 @@ class TreeRows:
     place [n_tok]            where the node's key and value go: tokens cached before + its number within its tree
     parent [n_tok]           the node it was drafted behind, -1 for a tree's root (-2 for padding, whose position and place are -1)
     bits [n_tok, words]      the nodes on the way from the root to it, itself included, a bit each (csrc.api.attention_tree)
-    max_nodes                nodes of the largest tree, or more
+    max_nodes                nodes of the largest tree, or more; what the last tree has beyond them is padding that attention leaves out
     """
 
     def __init__(self, place, parent, bits, max_nodes):
@@ -118,9 +118,17 @@ def tree_table_widths(cache, slots):
 
 
 def tree_bucket(n):
-    """Rows, or nodes, that a captured step of trees with ``n`` of them has: 1, 2, 4 or a multiple of 8, so that drafts whose lengths
-    differ share a few shapes."""
-    return 1 << (n - 1).bit_length() if n <= 8 else (n + 7) // 8 * 8
+    """Rows that a captured step of trees with ``n`` nodes has: a power of two, or from 16 on half as much again, so that drafts whose
+    lengths differ share a few shapes."""
+    p = 1 << (n - 1).bit_length()
+    return p * 3 // 4 if p >= 32 and n <= p * 3 // 4 else p
+
+
+def tree_shape(nodes):
+    """(rows, nodes of the largest tree or more) that a captured step of trees of ``nodes`` nodes each is made for. (With rows in eights and
+    the padding counted to the last tree, eight drafts of up to 63 tokens found a new shape at every other step.)"""
+    rows = tree_bucket(sum(nodes))
+    return rows, min(rows, 1 << (max(nodes) - 1).bit_length())
 
 
 def build_context(cache, entries, device, scratch_store=None, pad_to=None, plans=(), static=None, parents=None, max_nodes=0):
@@ -130,7 +138,7 @@ def build_context(cache, entries, device, scratch_store=None, pad_to=None, plans
     ``StepPlan`` objects of the model's parts; each is built once and uploaded with the rest.
     ``static``: see ``_pack``. ``parents``: a list an entry where the tokens are trees (see ``tree_arrays``); there ``pad_to`` adds nodes
     without a position to the last tree, which no other node sees and no path reaches, and ``max_nodes`` is the least that the
-    context says of the largest tree."""
+    context says of the largest tree (0: all of the last one's padding is counted too)."""
     n_seq = len(entries)
     lens = np.array([len(e[1]) for e in entries], dtype=np.int64)
     if n_seq == 0 or (lens < 1).any():
@@ -158,7 +166,7 @@ def build_context(cache, entries, device, scratch_store=None, pad_to=None, plans
     rows, largest = n_tok, int(lens.max())
     if parents is not None:
         pad = max(0, (pad_to or 0) - n_tok)
-        largest = max(largest, int(lens[-1]) + pad, max_nodes)
+        largest = max(largest, max_nodes or int(lens[-1]) + pad)
         tok, row_seq = np.concatenate([tok, np.zeros(pad, np.int64)]), np.concatenate([row_seq, np.full(pad, n_seq - 1)])
         row_pos, place, up = (np.concatenate([x, np.full(pad, none)]) for x, none in ((row_pos, -1), (place, -1), (up, -2)))
         bits = np.pad(bits, ((0, pad), (0, (largest + 31) // 32 - bits.shape[1])))

@@ -12,10 +12,11 @@ import torch
 from ..cache import Cache
 from ..csrc import api
 from ..sampling import seed_words
-from .batch import build_context, tree_bucket, tree_table_widths
+from .batch import build_context, tree_shape, tree_table_widths
 
 GRAPH_MAX_TOKENS = 8192     # steps of more tokens are launched plainly (the reference's bound: engine/engine.py:30)
-GRAPH_KEEP = 12             # captured step shapes kept, least recently used dropped first
+GRAPH_KEEP = 12             # captured step shapes kept, of steps and of steps of trees each, least recently used dropped first
+TREE_GRAPH_BYTES = 1 << 30  # logits that the captured steps of trees may hold together (one of 512 nodes over 151,936 tokens: 311 MB)
 
 
 class _StepGraph:
@@ -131,13 +132,22 @@ class Runner:
                 sg.logits = self.model.forward(ctx, self.cache)
             sg.ctx = ctx
             self._graphs[shape] = sg
-            while len(self._graphs) > GRAPH_KEEP:
-                self._graphs.popitem(last=False)
+            self._drop_graphs(bool(trees))
         else:
             self._graphs.move_to_end(shape)
             sg.ctx = self.context(entries, static=sg.static, **trees)   # same shape: the same views, new data
         sg.graph.replay()
         return sg.logits, sg.ctx
+
+    def _drop_graphs(self, trees):
+        """Keeps the graphs of steps (of trees, or the others) within their number, and those of trees within their bytes; the newest stays.
+        A shape that was dropped is launched plainly when it comes next: capturing it each time would cost more than the launches."""
+        own = [s for s in self._graphs if (s[0] == "trees") == trees]              # the least recently used first
+        size = lambda s: self._graphs[s].logits.numel() * self._graphs[s].logits.element_size()
+        while len(own) > 1 and (len(own) > GRAPH_KEEP or trees and sum(map(size, own)) > TREE_GRAPH_BYTES):
+            shape = own.pop(0)
+            del self._graphs[shape]
+            self._seen.pop(shape, None)
 
     @torch.inference_mode()
     def step_tree(self, entries, temperature=0.0, seeds=None, graph=False):
@@ -167,10 +177,7 @@ class Runner:
                 self.cache.reserve(slot, k)
             widths = tree_table_widths(self.cache, [s for s, _, _ in entries])
             reach = max(self.cache.length[s] + k for (s, _, _), k in zip(entries, nodes))
-            rows = tree_bucket(sum(nodes))
-            largest = tree_bucket(max(max(nodes), nodes[-1] + rows - sum(nodes)))
-            if largest > api.TREE_MAX_NODES:
-                rows, largest = sum(nodes), max(nodes)
+            rows, largest = tree_shape(nodes)
             logits, ctx = self._graph_forward(("trees", len(nodes), rows, largest, *widths), reach, entries, parents=parents, pad_to=rows,
                                               max_nodes=largest)
         else:

@@ -9,6 +9,7 @@ import torch
 import dryft_challenge_htn_2026_b200 as dk
 import plain_qwen3 as plain
 from dryft_challenge_htn_2026_b200.engine import Runner, load_model
+from dryft_challenge_htn_2026_b200.engine import runner as runner_module
 from helpers import TINY, make_folder, random_tokens, tolerance
 from test_generate_gpu import teacher_forced_gap
 from test_nilivik_gpu import make_model
@@ -144,6 +145,58 @@ def test_steps_of_trees_replayed_as_graphs_are_those_that_are_launched(tmp_path,
         a.step_tree([(s, [1] * k, [-1] + [k] * (k - 1)) for s, k in zip(slots[0], [7, 3, 5])], graph=True)
     la, lb = (r.step([(s, [t], [0]) for s, t in zip(own, last)]) for r, own in zip((a, b), slots))
     assert torch.equal(la, lb)
+
+
+@pytest.mark.parametrize("name", ["A", "E"])
+def test_drafts_of_all_lengths_find_captured_steps(tmp_path, monkeypatch, name):
+    """Eight drafts of 0 to 39 tokens a step: few captures, the captured prompt step stays, the tokens are those of launched steps."""
+    vocab = TINY[name]["vocab_size"]
+    model = load_model(make_folder(tmp_path, name, seed=24), torch.float32)
+    a, b = Runner(model, 64 * 60), Runner(model, 64 * 60)
+    captures, real = [], torch.cuda.CUDAGraph
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", lambda *args, **kw: captures.append(1) or real(*args, **kw))
+    prompts = [random_tokens(vocab, 3 + 5 * i, 90 + i) for i in range(8)]
+    for _ in range(2):                                        # a prompt step of this shape is captured the second time
+        slots = [a.begin() for _ in prompts]
+        a.step([(s, p[:-1], []) for s, p in zip(slots, prompts)], graph=True)
+        for s in slots:
+            a.end(s)
+    prompt_step = next(iter(a._graphs))
+    assert len(captures) == 1
+    slots = [[r.begin() for _ in prompts] for r in (a, b)]
+    for r, own in zip((a, b), slots):
+        r.step([(s, p[:-1], []) for s, p in zip(own, prompts)])
+    last, rs = [p[-1] for p in prompts], np.random.RandomState(7)
+    for turn in range(60):
+        trees = []
+        for t in last:
+            k = int(rs.randint(1, 41))
+            trees.append(([t] + rs.randint(0, vocab, k - 1).tolist(), [-1] + [int(rs.randint(0, i)) for i in range(1, k)]))
+        got = a.step_tree([(s, *t) for s, t in zip(slots[0], trees)], 0.8, list(range(8)), graph=True)
+        assert got == b.step_tree([(s, *t) for s, t in zip(slots[1], trees)], 0.8, list(range(8)))
+        last = [g[-1] for g in got]
+    assert 1 <= len(captures) - 1 <= 8 and prompt_step in a._graphs
+    la, lb = (r.step([(s, [t], [0]) for s, t in zip(own, last)]) for r, own in zip((a, b), slots))
+    assert float((la - lb).abs().max()) <= tolerance("float32", lb)
+
+
+def test_captured_steps_of_trees_stay_within_their_bytes(tmp_path, monkeypatch):
+    """Shapes that take turns where the logits of one alone fit: never more than that, and a shape that was dropped is launched before it is
+    captured again."""
+    vocab = TINY["A"]["vocab_size"]
+    model = load_model(make_folder(tmp_path, "A", seed=25), torch.float32)
+    r, alone = Runner(model, 64 * 20), Runner(model, 64 * 20)
+    monkeypatch.setattr(runner_module, "TREE_GRAPH_BYTES", 40 * vocab * 4)
+    captures, real = [], torch.cuda.CUDAGraph
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", lambda *args, **kw: captures.append(1) or real(*args, **kw))
+    (s, u), last, rs = (x.begin() for x in (r, alone)), 5, np.random.RandomState(8)
+    for turn in range(12):
+        k = (32, 20)[turn // 2 % 2]                            # twice each in turn: launched, then captured
+        tokens, parents = [last] + rs.randint(0, vocab, k - 1).tolist(), [-1] + [int(rs.randint(0, i)) for i in range(1, k)]
+        got = r.step_tree([(s, tokens, parents)], graph=True)
+        assert got == alone.step_tree([(u, tokens, parents)])
+        last = got[0][-1]
+        assert len(r._graphs) <= 1 and len(captures) == (turn + 1) // 2
 
 
 def test_trees_refusals(tmp_path):

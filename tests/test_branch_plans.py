@@ -5,7 +5,7 @@ import torch
 
 from dryft_challenge_htn_2026_b200.cache import Cache, KVRequest, StateRequest
 from dryft_challenge_htn_2026_b200.csrc import api, build
-from dryft_challenge_htn_2026_b200.engine.batch import build_context, tree_arrays, tree_bucket
+from dryft_challenge_htn_2026_b200.engine.batch import build_context, tree_arrays, tree_bucket, tree_shape
 from dryft_challenge_htn_2026_b200.engine.branch import draft_tree
 
 KV = KVRequest(2, 16, None, torch.float32)
@@ -111,3 +111,30 @@ def test_addresses_that_are_not_aligned_are_refused_by_the_entry_points(source, 
                 assert call(**{name: at + off}, f32=f32) == invalid, (name, off)
         for name in ("ldq", "ldo"):
             assert call(**{name: 2 * hd + 2}, f32=f32) == invalid, name
+
+
+def test_shapes_of_captured_steps_of_trees_are_few():
+    """Eight trees of 1 to 64 nodes, a thousand times: a handful of shapes, and the order of the trees makes no difference."""
+    rs, shapes = np.random.RandomState(0), set()
+    for _ in range(1000):
+        nodes = rs.randint(1, 65, 8).tolist()
+        rows, largest = tree_shape(nodes)
+        assert sum(nodes) <= rows <= max(16, 1.5 * sum(nodes)) and max(nodes) <= largest <= min(rows, 2 * max(nodes))
+        assert tree_shape(sorted(nodes)) == tree_shape(nodes[::-1]) == (rows, largest)
+        shapes.add((rows, largest))
+    assert len(shapes) <= 8
+    assert [tree_shape([n]) for n in (1, 3, 17, 1024)] == [(1, 1), (4, 4), (24, 24), (1024, 1024)]
+    assert tree_shape([1024] * 7) == (8192, 1024) and tree_shape([1, 1, 1]) == (4, 1)
+
+
+def test_context_of_padding_beyond_the_largest_tree():
+    """Padding that no tree has room for is not counted to the largest tree: its rows stand behind the last tree's real nodes."""
+    cache = Cache([[KV]], max_tokens=64 * 12, max_slots=3, device="cpu")
+    a, b = cache.begin(), cache.begin()
+    ctx = build_context(cache, [(a, list(range(14)), range(14)), (b, [5, 6], range(2))], torch.device("cpu"),
+                        parents=[list(range(-1, 13)), [-1, 0]], pad_to=24, max_nodes=16)
+    assert ctx.tree.max_nodes == 16 and ctx.cu_q.tolist() == [0, 14, 24] and ctx.n_tok == 24
+    assert ctx.row_pos.tolist()[14:] == [0, 1] + [-1] * 8 and ctx.tree.place.tolist()[14:] == [0, 1] + [-1] * 8 and ctx.tree.bits.shape == (24, 1)
+    small = build_context(cache, [(a, list(range(14)), range(14)), (b, [5], range(1))], torch.device("cpu"),
+                          parents=[list(range(-1, 13)), [-1]], pad_to=64, max_nodes=16)
+    assert small.tree.max_nodes == 16 and small.cu_q.tolist() == [0, 14, 64]
