@@ -2337,8 +2337,6 @@ def beam_select(logits, scores, ended, scores_out, beam_out, tok_out):
             raise KernelError("beam_select: results in the memory of scores or ended")
     lib = _lib("beam_select.cu")
     pieces = lib.dk_beam_pieces(V)
-    if not lib.dk_beam_select_takes(V, beams, best):
-        raise KernelError(f"beam_select: {best} of {beams} beams over {V} tokens need more shared memory than a block has")
     n = requests * beams * pieces
     ws = scores.new_empty(2 * n * (best + 2))     # pairs of doubles first, then the keys: 8 bytes each; held as in tree_accept
     at = ws.data_ptr()

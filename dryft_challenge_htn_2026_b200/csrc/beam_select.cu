@@ -170,13 +170,47 @@ __device__ __forceinline__ double value_of(const Candidate& c) {
 
 constexpr int KEYS = 4096;                                              // keys that are brought into shared memory at once, if there are no more
 
-// grid (requests). Dynamic shared memory: best * best * ceil(lists / THREADS) candidates, then the keys where they are KEYS at most.
+// The sum of a block's numbers, in all threads. red: WARPS numbers of shared memory.
+__device__ __forceinline__ int block_sum(int n, int* red) {
+    n = __reduce_add_sync(0xffffffffu, n);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < WARPS; i++) n += red[i];
+    return n;
+}
+
+// The best-th candidate of all lists (or one that all stand before, where there are fewer), found bit by bit: its value, then its place
+// among those of that value. counted(c): how many stand before c or are it.
+template <typename F>
+__device__ __forceinline__ Candidate best_th(int best, const F& counted) {
+    Candidate c = {0, 0x7fffffff};
+    for (int bit = 63; bit >= 0; bit--) {
+        const Candidate mid = {c.order | 1ull << bit, 0x7fffffff};
+        const int n = counted(mid);
+        if (n == best) return mid;
+        if (n > best) c.order = mid.order;
+    }
+    if (c.order == 0) return c;                                          // fewer than asked for
+    c.flat = 0;
+    for (int bit = 30; bit >= 0; bit--)
+        if (counted(Candidate{c.order, (c.flat | 1 << bit) - 1}) < best) c.flat |= 1 << bit;
+    return c;
+}
+
+// grid (requests). Dynamic shared memory: best * best * ceil(lists / THREADS) candidates, then the keys where they are KEYS at most. MANY:
+// where that is more than a block has (32 beams and 64 results from 25 pieces on): `best` candidates, which best_th has counted off before
+// they are taken: up to 95 looks at the lists instead of one (32 beams over 200,003 tokens, 64 results: 137 us a call; over 190,000 27).
+template <bool MANY>
 __global__ void __launch_bounds__(THREADS)
 beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, int V, int beams, int best, const float* scores,
                    const int* ended, float* scores_out, int* beam_out, int* tok_out) {
     extern __shared__ __align__(16) unsigned char dyn[];
     Candidate* found = reinterpret_cast<Candidate*>(dyn);
-    __shared__ Candidate tops[THREADS], least;
+    __shared__ Candidate tops[MANY ? 1 : THREADS], least;
+    __shared__ int red[WARPS];
     __shared__ double highest[MAX_BEAMS], offset[MAX_BEAMS];            // a live beam: its largest logit, score - log(sum) against that
     __shared__ int kind[MAX_BEAMS];                                      // 0: not live, 1: live, 2: at its end
     __shared__ int count;
@@ -186,7 +220,7 @@ beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, in
     const int r = blockIdx.x, t = threadIdx.x, lane = t & 31, w = t >> 5;
     const int lists = beams * pieces;
     const uint64_t* keys = ws_key + (size_t)r * lists * best;
-    if (lists * best <= KEYS) {
+    if (!MANY && lists * best <= KEYS) {
         uint64_t* here = reinterpret_cast<uint64_t*>(found + best * best * ((lists + THREADS - 1) / THREADS));
 #pragma unroll 8
         for (int i = t; i < lists * best; i += THREADS) here[i] = keys[i];
@@ -222,21 +256,41 @@ beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, in
         const uint64_t key = kind[b] == 1 ? keys[l * best + rank] : 0;
         return key ? candidate(((double)logit_of(key) - highest[b]) + offset[b], b * V + index_of(key)) : none;
     };
-    Candidate top = none;
-    for (int l = t; l < lists; l += THREADS) {
-        const Candidate c = item(l, 0);
-        if (c.before(top)) top = c;
-    }
-    tops[t] = top;
-    __syncthreads();
-    int above = 0;
-    const int n_tops = min(THREADS, lists);
+    Candidate low;
+    bool some = true;                                                    // whether the thread's lists may hold one
+    if (MANY) {
+        low = best_th(best, [&](const Candidate& c) {
+            int n = 0;
+            for (int l = t; l < lists; l += THREADS) {
+                int lo = 0, hi = best;                                   // the list's first `lo` stand before c or are it, those from hi on do not
+                while (lo < hi) {
+                    const int mid = lo == 0 ? 0 : (lo + hi) / 2;         // few lists hold any
+                    const Candidate x = item(l, mid);
+                    if (x.flat >= 0 && !c.before(x)) lo = mid + 1;
+                    else hi = mid;
+                }
+                n += lo;
+            }
+            return block_sum(n, red);
+        });
+    } else {
+        Candidate top = none;
+        for (int l = t; l < lists; l += THREADS) {
+            const Candidate c = item(l, 0);
+            if (c.before(top)) top = c;
+        }
+        tops[t] = top;
+        __syncthreads();
+        int above = 0;
+        const int n_tops = min(THREADS, lists);
 #pragma unroll 8
-    for (int i = 0; i < n_tops; i++) above += tops[i].before(top);
-    if (top.flat >= 0 && above == best - 1) least = top;                 // the best-th largest of the threads' largest
-    __syncthreads();
-    const Candidate low = least;
-    if (top.flat >= 0 && !low.before(top))
+        for (int i = 0; i < n_tops; i++) above += tops[i].before(top);
+        if (top.flat >= 0 && above == best - 1) least = top;             // the best-th largest of the threads' largest
+        __syncthreads();
+        low = least;
+        some = top.flat >= 0 && !low.before(top);
+    }
+    if (some)
         for (int l = t; l < lists; l += THREADS)
             for (int rank = 0; rank < best; rank++) {
                 const Candidate c = item(l, rank);
@@ -260,6 +314,8 @@ beam_select_kernel(const uint64_t* ws_key, const double2* ws_sum, int pieces, in
         scores_out[(size_t)r * best + i] = -INFINITY, beam_out[(size_t)r * best + i] = 0, tok_out[(size_t)r * best + i] = 0;
 }
 
+constexpr size_t SELECT_ROOM = 200 * 1024;
+
 size_t select_smem(int beams, int pieces, int best) {
     const long long lists = (long long)beams * pieces;
     return (size_t)(best * best * ((lists + THREADS - 1) / THREADS)) * sizeof(Candidate) + (lists * best <= KEYS ? (size_t)(lists * best) * 8 : 0);
@@ -268,7 +324,6 @@ size_t select_smem(int beams, int pieces, int best) {
 }  // namespace
 
 DK_EXPORT int dk_beam_pieces(int V) { return logit_pieces(V, Piece::SIZE); }
-DK_EXPORT int dk_beam_select_takes(int V, int beams, int best) { return select_smem(beams, dk_beam_pieces(V), best) <= 200 * 1024; }
 
 // logits [requests * beams, V] float32, scores [requests, beams], ended [requests, beams] or null; ws_key: requests * beams * pieces *
 // best 8-byte words, ws_sum: requests * beams * pieces pairs of doubles; results [requests, best].
@@ -278,10 +333,11 @@ DK_EXPORT int dk_beam_select(const float* logits, int V, int requests, int beams
         (long long)requests * beams > 65535)
         return (int)cudaErrorInvalidValue;
     const int pieces = dk_beam_pieces(V);
-    const size_t smem = select_smem(beams, pieces, best);
-    if (smem > 200 * 1024) return (int)cudaErrorInvalidValue;
+    size_t smem = select_smem(beams, pieces, best);
+    const bool many = smem > SELECT_ROOM;
+    if (many) smem = best * sizeof(Candidate);
     if (smem > 32 * 1024) {
-        cudaError_t ce = cudaFuncSetAttribute(beam_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+        cudaError_t ce = cudaFuncSetAttribute(beam_select_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SELECT_ROOM);
         if (ce != cudaSuccess) {
             cudaGetLastError();
             return (int)ce;
@@ -290,6 +346,6 @@ DK_EXPORT int dk_beam_select(const float* logits, int V, int requests, int beams
     int e = dk_launch(beam_pieces_kernel, dim3(pieces, requests * beams), dim3(THREADS), 0, st, logits, V, best, ws_key, (double2*)ws_sum);
     if (e) return e;
     // (may start under the end of the first: it reads nothing before)
-    return dk_launch_as(true, beam_select_kernel, dim3(requests), dim3(THREADS), smem, st, (const uint64_t*)ws_key, (const double2*)ws_sum, pieces,
+    return dk_launch_as(true, many ? beam_select_kernel<true> : beam_select_kernel<false>, dim3(requests), dim3(THREADS), smem, st, (const uint64_t*)ws_key, (const double2*)ws_sum, pieces,
                         V, beams, best, scores, ended, scores_out, beam_out, tok_out);
 }

@@ -802,6 +802,25 @@ def test_select_does_not_hang_on_a_number_added_to_all_logits(above):
     check_exact_select(logits, scores, 24)
 
 
+@pytest.mark.parametrize("vocab,beams,best", [(200003, 32, 64), (300000, 32, 57), (6500000, 1, 64), (2200000, 3, 64)])
+def test_select_from_more_lists_than_a_block_has_room_for(vocab, beams, best):
+    """The most beams and results over vocabularies from 196,606 on, or fewer beams over larger ones."""
+    logits = normal((beams, vocab), seed=vocab, scale=3.0)
+    scores = -20 - 2 * torch.rand((1, beams), generator=torch.Generator().manual_seed(best)).to(DEV)
+    check_select(logits, scores, None, best)
+    check_select(logits, scores, i32(np.arange(beams)[None] % 3 == 1), best)
+    if beams == 32:
+        two = torch.cat([logits, logits.flip(0)])               # two requests in a call
+        both = select(two, torch.cat([scores, scores.flip(1)]), None, best)
+        assert torch.equal(both[2][0], both[2][1]) and torch.equal(both[1][0], beams - 1 - both[1][1]) and torch.equal(both[0][0], both[0][1])
+    logits = torch.zeros((beams, vocab), device=DEV)            # equal everywhere: the lower beam, then the lower token
+    check_select(logits, torch.full((1, beams), -1.0, device=DEV), None, best)
+    logits[:] = -math.inf
+    logits[0, [5, vocab - 1, vocab // 2]], logits[beams - 1, 77] = 1.0, 2.0
+    check_select(logits, torch.full((1, beams), -1.0, device=DEV), None, best)          # fewer candidates than asked for
+    check_select(logits, torch.full((1, beams), -math.inf, device=DEV), None, best)
+
+
 def test_select_from_memory_that_is_not_aligned_and_twice():
     base = normal((1 + 4 * 1000,), seed=3)
     logits = base[1:].view(4, 1000)
