@@ -87,10 +87,11 @@ class TreeRows:
     parent [n_tok]           the node it was drafted behind, -1 for a tree's root (-2 for padding, whose position and place are -1)
     bits [n_tok, words]      the nodes on the way from the root to it, itself included, a bit each (csrc.api.attention_tree)
     max_nodes                nodes of the largest tree, or more; what the last tree has beyond them is padding that attention leaves out
+    padded                   whether there may be padding (a captured step)
     """
 
-    def __init__(self, place, parent, bits, max_nodes):
-        self.place, self.parent, self.bits, self.max_nodes = place, parent, bits, max_nodes
+    def __init__(self, place, parent, bits, max_nodes, padded):
+        self.place, self.parent, self.bits, self.max_nodes, self.padded = place, parent, bits, max_nodes, padded
 
 
 def tree_arrays(parents):
@@ -201,7 +202,7 @@ def build_context(cache, entries, device, scratch_store=None, pad_to=None, plans
     ctx.tables = dev[7:7 + len(tables)]
     ctx.plans = dict(zip(by_key, dev[7 + len(tables):]))
     if parents is not None:
-        ctx.tree = TreeRows(*dev[-3:], largest)
+        ctx.tree = TreeRows(*dev[-3:], largest, pad_to is not None)
     ctx.host = dict(lens=lens, pos0=pos0, cu_q=cu, slots=slots, row_seq=row_seq, row_pos=row_pos)
     if is_decode:
         ctx.n_seq = rows  # the decode kernels run one sequence per row, padding rows included

@@ -182,9 +182,10 @@ class GQAAttention(Part):
             self.position.apply(qkv, ctx, nh, nkv, hd)
         if writes:
             api.kv_write(qkv[:, nh * hd:(nh + nkv) * hd], qkv[:, (nh + nkv) * hd:], kv.k, kv.v, ctx.tree.place, ctx.row_seq, table, nkv, hd, hd)
-        # rows of padding beyond max_nodes are not written: they hold what a step before left there, and zeros at first
-        o = ctx.scratch(("tree_rows", ctx.n_tok, nh * hd, self.rt.dtype),
-                        lambda: torch.zeros((ctx.n_tok, nh * hd), dtype=self.rt.dtype, device=self.rt.device))
+        if ctx.tree.padded:      # padding beyond max_nodes is not written: there a buffer that holds zeros, or what a step before left
+            o = ctx.scratch(("tree_rows", ctx.n_tok, nh * hd), lambda: torch.zeros((ctx.n_tok, nh * hd), dtype=self.rt.dtype, device=self.rt.device))
+        else:
+            o = torch.empty((ctx.n_tok, nh * hd), dtype=self.rt.dtype, device=self.rt.device)
         api.attention_tree(qkv[:, :nh * hd], o, kv.k, kv.v, ctx.cu_q, ctx.seq_pos0, ctx.row_pos, ctx.tree.bits, table, nh, nkv, hd,
                            s.window or 0, s.scale, ctx.tree.max_nodes)
         return linear(o, self.w_o, allow_partial=True)

@@ -199,6 +199,17 @@ def test_captured_steps_of_trees_stay_within_their_bytes(tmp_path, monkeypatch):
         assert len(r._graphs) <= 1 and len(captures) == (turn + 1) // 2
 
 
+def test_launched_steps_of_trees_keep_no_buffers(tmp_path):
+    model = load_model(make_folder(tmp_path, "A", seed=26), torch.float32)
+    r = Runner(model, 64 * 20)
+    s = r.begin()
+    r.step_tree([(s, [1, 2], [-1, 0])])
+    held = len(r._scratch)
+    for k in range(3, 20):
+        r.step_tree([(s, [1] * k, list(range(-1, k - 1)))])
+    assert len(r._scratch) == held
+
+
 def test_trees_refusals(tmp_path):
     folder = make_folder(tmp_path, "A", seed=20)
     eng = dk.Engine(folder, dtype=torch.float32)
