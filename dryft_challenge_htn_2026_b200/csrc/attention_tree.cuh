@@ -303,10 +303,12 @@ static int tree_merge(const TreeArgs& a, const float* ws_acc, const float* ws_ml
                       cudaStream_t st) {
     if (a.whole) return 0;
     const int tiles = (a.max_nodes + a.tile_nodes - 1) / a.tile_nodes, groups = (tile_rows + 31) / 32 * tiles;
-    // Few tiles, so many parts each: the columns in halves, to have more of them on the way at once (two sequences of 32k tokens, 9 parts:
-    // 61.8 us the whole call with all columns a block, 60.5 with halves; eight of 4k tokens, 2 to 4 parts: 48.5 and 53.3).
+    // Few tiles, so many parts each (six or more): the columns in halves, to have more of them on the way at once. The whole call, 32 heads on
+    // 8 of 128, bfloat16, 148 blocks, all columns a block / halves: one tree of 24 behind 32,768 tokens (8 tiles) 43.7 / 40.8 us, two 61.5 / 60.5,
+    // three 81.1 / 81.0, four 101.2 / 101.7; one tree of 64 behind 4,096 24.3 / 21.5, four (32 tiles) 34.0 / 36.7, eight 54.3 / 59.3. float32,
+    // 296 blocks: trees of 16 behind 4,096, one (8 tiles) 52.1 / 49.7, six (48) 183.5 / 182.9, four of 40 (96) 344.3 / 345.2.
     constexpr int HALF = D % 128 == 0 ? D / 2 : D;
-    if (HALF < D && 4LL * a.n_seq * tiles * a.nkv <= blocks)
+    if (HALF < D && 6LL * a.n_seq * tiles * a.nkv <= blocks)
         return dk_launch_as(true, tree_merge_kernel<T, D, HALF>, dim3(groups * (D / HALF), a.nkv, a.n_seq), dim3(256), 0, st, a, ws_acc,
                             (const float2*)ws_ml, (T*)out, ldo, tile_rows, blocks);
     return dk_launch_as(true, tree_merge_kernel<T, D, D>, dim3(groups, a.nkv, a.n_seq), dim3(256), 0, st, a, ws_acc, (const float2*)ws_ml,
