@@ -2240,7 +2240,7 @@ def attention_tree(q, out, k_store, v_store, cu_q, seq_pos0, row_pos, tree, page
     whose bit (word j / 32, bit j % 32) is set in its row of ``tree`` [rows, words] int32: of a drafted tree its ancestors and itself,
     but any bits may be set. With a ``window`` it sees only what lies less than that many positions before it. Rows that see nothing
     become zeros, rows behind cu_q's last are left as they were, and what lies at keys a row does not see, NaN included, does not reach
-    it. A page id outside the store holds no keys. q and out [rows, heads * head_dim] (rows of wider matrices) and the stores, on 16-byte
+    it; an infinite value that it does see makes its columns infinite, or NaN where its weight is too small for float32. A page id outside the store holds no keys. q and out [rows, heads * head_dim] (rows of wider matrices) and the stores, on 16-byte
     boundaries, float32 or bfloat16, head sizes in steps of 16 up to 256; out may be q itself. The lengths are read on the device: a captured graph
     may be replayed with other ones, as long as ``max_nodes`` and the table's width hold."""
     global _tc_err

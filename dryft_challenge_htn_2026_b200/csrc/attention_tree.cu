@@ -5,7 +5,8 @@
 //   out[i, h] = sum_j w_j v_j / sum_j w_j,  w_j = exp2(scale * log2(e) * q[i, h].k_j - m),  j over the keys node i sees
 //
 // with the running maximum m and both sums in float32, one pass over the keys. A node that sees no key gives zeros. What lies at a
-// key that a row does not see, be it NaN or infinite, does not reach the row.
+// key that a row does not see, be it NaN or infinite, does not reach the row. An infinite value that it does see gives NaN where its
+// weight has become 0 in float32.
 //
 // What bounds a page step is what shared memory returns to registers, 128 bytes a clock: a thread with 4 rows reads 8 x 16 bytes for 64
 // products of the scores and 12 for 128 of the values, 14,300 clocks (7.4 us of an SM) for 64 rows of 128 columns against 8,200 of

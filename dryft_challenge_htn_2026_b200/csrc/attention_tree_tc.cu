@@ -28,7 +28,7 @@
 // rows a page step takes 1.2 us whatever the softmax does: S, P.V and the next S of a stream are chains of 8 + 4 tcgen05.mma that one
 // thread issues, 60 to 100 clocks each, and both streams run in step. With up to 128 rows a step is two pages, 0.72 to 0.84 us a page
 // against 0.74 us that its 32 KB take at the copy rate. Around the pages: about 4 us until the first products, 2 us to leave the parts, 6 us for
-// the merge. One block an SM with two streams instead of two blocks an SM: 47.6 us for 55.6 in the first case, as a page is read once for
+// the merge. One block an SM with two streams instead of two blocks an SM: 51.7 us for 55.6 in the first case, as a page is read once for
 // 256 rows. The rings are as deep as shared memory allows, so that both streams can be a page apart.
 // Every mbarrier wait is bounded; a wait that runs out stores a code in *err, and the block still frees its tensor memory and returns.
 #include <cuda.h>
@@ -94,9 +94,9 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// the clock is read only when the barrier is not through yet (most waits of the mma thread find it through)
-// try_wait lets the hardware suspend the thread for a while instead of having it poll: a polling
-// thread takes issue slots from the softmax warps of the other block on its scheduler
+// the clock is read only when the barrier is not through yet (most waits of the mma threads find it through)
+// try_wait lets the hardware suspend the thread for a while instead of having it poll: a polling thread takes
+// issue slots from the softmax warps on its scheduler
 __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
@@ -212,7 +212,8 @@ struct Walk : TreeWalk {
 };
 
 // Values that are not finite were left out of the products: the columns [c0, c1) of a row that sees some become their sum, which the
-// rest of the row's sum does not change. To dst (the row's result) or, if that is null, to its part.
+// rest of the row's sum does not change, be their weights ever so small. (In pages that every row sees they go through the products, and
+// an infinite one gives NaN where its weight has become 0.) To dst (the row's result) or, if that is null, to its part.
 __device__ __noinline__ void mend_row(const TreeArgs& a, const Walk& w, const uint32_t* words, int pos, int open_lo, const bf16* v_store,
                                       int c0, int c1, bf16* dst, float* part, int row) {
     for (int c = c0; c < c1; c++) {

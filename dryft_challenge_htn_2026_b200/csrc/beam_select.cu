@@ -18,9 +18,10 @@
 // takes its place, above which `best` threads have all there is. (That one alone, 256 comparisons a thread, took two thirds of the
 // kernel's time: 47 us for 128 rows of 100,003.) Second launch, a block a request: the same over the pieces' lists, which are in order.
 //
-// Measured: four beams over 151,936 tokens 8.9 us, 16 x 8 beams over 100,003 tokens 24.8 us (51 MB, 7.8 us at the copy rate), 16 x 8
-// over 200,003 36.6: about 13 us of latency (a block's load, its rounds of barriers, the second launch) and 4.3 TB/s above that. Threads
-// with 16 logits, twice as many a block, have looser floors (35 us); 5 or 6 blocks an SM with fewer registers were no faster (25.3, 26.8).
+// Measured: four beams over 151,936 tokens 8.7 us, 16 x 8 beams over 100,003 tokens 25.3 us (51 MB, 7.8 us at the copy rate), 16 x 8
+// over 200,003 36.3: about 14 us of latency (a block's load, its rounds of barriers, the second launch) and 4.6 TB/s above that. Threads
+// with 16 logits, twice as many a block, have looser floors (35 us, when this form took 24.8); 5 or 6 blocks an SM with fewer registers were
+// no faster (25.3, 26.8).
 #include "logit_rows.cuh"
 
 namespace {

@@ -11,8 +11,8 @@
 // by reading them where the choice is greedy); then a block a sequence puts the pieces together and walks the path. Drawing costs a
 // hash and two logarithms a logit. Most logits are spared the logarithms: -log(u) >= 1 - u, so the noise is at most -log(1 - u), and
 // what does not reach the thread's best so far with that much cannot win.
-// Measured: eight trees of 40 to 64 nodes over 151,936 tokens, greedy, 42 us (252 MB, 6.0 TB/s, 92 % of the copy rate); five nodes, drawn, 9.2 us on
-// the device, of which the logits are 0.5 and the two launches most; a call of this size is bound by the host's 15 us.
+// Measured: eight trees of 40 to 64 nodes over 151,936 tokens, greedy, 42 us (252 MB, 6.0 TB/s, 92 % of the copy rate); five nodes, drawn, 8.7 us on
+// the device, of which the logits are 0.5 and the two launches most; a call of this size takes the host 23 us.
 #include "logit_rows.cuh"
 #include "sampling_kernels.cuh"
 
@@ -130,8 +130,9 @@ accept_path_kernel(const float* ws_val, const int* ws_idx, int pieces, const int
 
 }  // namespace
 
-// Logits a thread of the first launch takes: 32, or 8 where that leaves SMs without a block, as with a handful of nodes (5 nodes of
-// 151,936, drawn: 13.5 us with 32, 8.5 with 16).
+// Logits a thread of the first launch takes: 32, or 8 where that leaves SMs without a block, as with a handful of nodes. With 8 / 32, nodes of
+// 151,936 logits: drawn, 5 nodes 8.6 / 12.0 us, 16 15.2 / 18.0, 32 (where the rule changes) 24.6 / 26.5, 64 45.7 / 46.7, 8 x 64 305 / 281;
+// greedy 5 nodes 5.3 / 4.8, 16 6.3 / 5.3, 32 8.0 / 6.5, 64 14.8 / 12.3.
 static int each_for(int V, long long rows) {
     static int sms = 0;
     if (sms == 0) {

@@ -84,7 +84,8 @@ class Engine:
         yield from run_batch(self.backend, [list(p) for p in input_ids], params, seeds)
 
     def generate_drafted(self, input_ids, max_new_tokens, draft, temperature=0.0, seed=0, stop_token_ids=(), max_nodes=64):
-        """``generate`` with tokens that somebody else guesses and the model checks, several a step: the same tokens in fewer steps.
+        """``generate`` with tokens that somebody else guesses and the model checks, several a step: the same tokens in fewer steps (up to the
+        rounding of the logits: other numbers of rows take other product kernels, so in bfloat16 a near tie may fall the other way).
         ``draft(i, tokens)`` is asked before every step how sequence i goes on behind ``tokens`` (its prompt and what was generated) and
         answers with a list of tokens, or with (tokens, parents), a tree: ``parents[k]`` is the number of the drafted token that
         ``tokens[k]`` would follow, -1 for the last of ``tokens``. Up to ``max_nodes`` - 1 tokens. Yields a list of lists, the new
